@@ -92,6 +92,63 @@ int intra_b200_decode(const void* q, const void* k, const void* v, const void* m
                       int64_t mask_batch_stride, int64_t mask_token_stride,
                       float softmax_scale, int device, void* cuda_stream);
 
+/* intra_b200_decode for caches of which each key's received attention is accumulated:
+ * weights[b][hk][j] += the sum of key j's probabilities over KV head hk's query heads, fp32 by strides (in elements; unit
+ * stride over keys), keys the token does not see being left as they are. `lengths` is NULL or B ints: the keys before
+ * the token's own, which sees keys 0 .. lengths[b] (brought into 0 .. S - 1). Strides {batch, token, head}; the mask's
+ * {batch, token}. Always wants scratch (see above): the scores pass through it. */
+int intra_b200_decode_accumulate(const void* q, const void* k, const void* v, const void* mask, const int* lengths, void* out,
+                                 float* weights, void* scratch, int64_t scratch_bytes, int64_t* scratch_needed, int B, int S,
+                                 int H, int Hkv, const int64_t q_strides[3], const int64_t k_strides[3],
+                                 const int64_t v_strides[3], const int64_t mask_strides[2], int64_t weights_batch_stride,
+                                 int64_t weights_head_stride, float softmax_scale, int device, void* cuda_stream);
+
+/* Attention of n (1..64) new tokens per sequence over its KV cache, their own keys included: drafted tokens that form a
+ * tree, or a chain. q is B x n x H rows by strides {batch, token, head}, out (B, n, H, 128) contiguous, k and v as for the
+ * decode step. The tokens' own keys are rows lengths[b] .. lengths[b] + n - 1 of the cache (lengths NULL: its last n;
+ * brought into 0 .. S - n). Token i sees the keys before those, its ancestors and itself: parents[b][i] is the token that
+ * comes before it, an earlier one, or negative; NULL: i - 1. With all_own != 0 it sees all n own keys instead (`mask` is to
+ * decide alone). `mask` is NULL or B x n x S bytes by strides {batch, token, key}
+ * (0 repeats), nonzero = visible. Keys that no token of the sequence sees are not read; a token that sees nothing gets
+ * zeros. Scratch as for the decode step. */
+int intra_b200_tree_attn(const void* q, const void* k, const void* v, const int* parents, const int* lengths, const void* mask,
+                         void* out, void* scratch, int64_t scratch_bytes, int64_t* scratch_needed, int B, int S, int H, int Hkv,
+                         int n, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                         int64_t parents_batch_stride, int all_own, const int64_t mask_strides[3], float softmax_scale,
+                         int device, void* cuda_stream);
+
+/* Verification of drafted tokens against the target model's probabilities. Per sequence n (1..64) nodes; node 0 is the
+ * token sampled last, parents as above. target[b][i] is the target's distribution over V tokens behind node i, draft[b][i]
+ * the one its children were drawn from (n or n - 1 rows), both of type `prob_type`; draft NULL: drafts are certain. Child c of
+ * the current node, in index order, is accepted iff uniform[b][c] * q(x) * Z < R(x), R and Z being p and 1; a rejection turns
+ * R into max(R / Z - q, 0) and Z into its sum, where that is not zero. At the end one token is drawn from R: the
+ * smallest t with R(0) + .. + R(t) > uniform[b][0] * sum R. Sums in 64 bits. Outputs, contiguous: accepted[b], the number
+ * of accepted drafts m; path[b] = 0 and the accepted nodes, then -1; out_tokens[b]: the accepted tokens, the drawn one
+ * at place m, then -1. Drafts outside 0 .. V - 1 are rejected. Strides in elements {batch, node}; unit stride over V. */
+#define INTRA_PROB_F32 0
+#define INTRA_PROB_BF16 1
+#define INTRA_PROB_F16 2
+int intra_b200_verify_drafts(const void* tokens, int tokens_int64, const void* target, const void* draft, int prob_type,
+                             const float* uniform, const int* parents, int* accepted, int* path, int64_t* out_tokens, int B, int n,
+                             int V, const int64_t target_strides[2], const int64_t draft_strides[2], int64_t tokens_batch_stride,
+                             int64_t uniform_batch_stride, int64_t parents_batch_stride, int device, void* cuda_stream);
+
+/* Moves the rows of accepted tokens together, in place, in n_caches K or V caches of B x S x Hkv rows (strides: three per
+ * cache, positive; the caches must not overlap): row lengths[b] + path[b][i] becomes row lengths[b] + i for every i < n with
+ * path[b][i] in 0 .. n - 1, whatever the order; nothing moves for a sequence whose lengths[b] is not in 0 .. S - n. */
+int intra_b200_keep_drafts(void* const* caches, const int64_t* strides, int n_caches, const int* lengths, const int* path,
+                           int64_t path_batch_stride, int B, int S, int Hkv, int n, int device, void* cuda_stream);
+
+/* Cuts a cache down to its heaviest keys. Of the lengths[b] (NULL: S; brought into 0 .. S) rows in use of each head, the last
+ * `recent` and the heaviest of the others by weights[b][hk][j] stay, `keep` in all, in their order, ties going to the
+ * lower row, NaN counting as the heaviest; all stay where there are no more than that. Writes row i of the kept ones to row i
+ * of k_out, v_out and weights_out and its old place to kept[b][hk][i] (contiguous), and, for i past them and below `keep`,
+ * zeros and -1. Output rows from `keep` on are left alone. Outputs must not overlap inputs. */
+int intra_b200_evict(const void* k, const void* v, const float* weights, const int* lengths, void* k_out, void* v_out,
+                     float* weights_out, int* kept, int B, int S, int Hkv, int keep, int recent, const int64_t k_strides[3],
+                     const int64_t v_strides[3], const int64_t weights_strides[2], const int64_t k_out_strides[3],
+                     const int64_t v_out_strides[3], const int64_t weights_out_strides[2], int device, void* cuda_stream);
+
 /* Text for a status code; replaces the reference's TORCH_CHECK messages
  * (csrc/flash_attn/flash_api.cpp:377-394, 576-597). */
 const char* intra_b200_strerror(int status);

@@ -32,6 +32,15 @@ SIGNATURES = {
                                         _i, _i, _i, _f, _i, _vp, ctypes.POINTER(_i)]),
     "intra_b200_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, ctypes.POINTER(_i64), _i, _i, _i, _i,
                                _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _i, _vp]),
+    "intra_b200_decode_accumulate": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, ctypes.POINTER(_i64), _i, _i, _i, _i,
+                                          _I64x3, _I64x3, _I64x3, _I64x3, _i64, _i64, _f, _i, _vp]),
+    "intra_b200_tree_attn": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, ctypes.POINTER(_i64), _i, _i, _i, _i, _i,
+                                  _I64x3, _I64x3, _I64x3, _i64, _i, _I64x3, _f, _i, _vp]),
+    "intra_b200_verify_drafts": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _I64x3, _I64x3,
+                                      _i64, _i64, _i64, _i, _vp]),
+    "intra_b200_keep_drafts": (_i, [ctypes.POINTER(_vp), _I64x3, _i, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
+    "intra_b200_evict": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _I64x3, _I64x3, _I64x3,
+                              _I64x3, _I64x3, _I64x3, _i, _vp]),
     "intra_b200_strerror": (ctypes.c_char_p, [_i]),
     "intra_b200_last_cuda_error": (_i, []),
     "intra_b200_device_status": (_i, [_i, ctypes.POINTER(_i), _i]),

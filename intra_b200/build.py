@@ -12,12 +12,13 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libintra_b200.so")
-SOURCES = [os.path.join(CSRC, "capi.cu")]
+SOURCES = [os.path.join(CSRC, f) for f in ("capi.cu", "serving.cu")]
 # every header next to the sources counts: an edit to any of them must trigger a rebuild
 HEADERS = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))) + [
     os.path.join(PKG_DIR, "..", "include", "intra_b200.h")]
@@ -41,12 +42,20 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
-    cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
-           "-shared", "-Xcompiler", "-fPIC", "-Xptxas", "-v", "-o", LIB_PATH] + SOURCES
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or proc.returncode != 0:
-        sys.stderr.write(proc.stdout + proc.stderr)
-    if proc.returncode != 0:
+    flags = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC"]
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, os.path.basename(f) + ".o") for f in SOURCES]
+        cmds = [flags + ["-c", "-Xptxas", "-v", "-o", obj, src] for src, obj in zip(SOURCES, objects)]
+        procs = [subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for cmd in cmds]
+        said = [p.communicate()[0] for p in procs]          # the sources compile side by side
+        failed = any(p.returncode != 0 for p in procs)
+        if not failed:
+            link = subprocess.run(flags + ["-shared", "-o", LIB_PATH] + objects, capture_output=True, text=True)
+            said.append(link.stdout + link.stderr)
+            failed = link.returncode != 0
+    if verbose or failed:
+        sys.stderr.write("".join(said))
+    if failed:
         raise RuntimeError("nvcc failed building libintra_b200.so")
     return LIB_PATH
 

@@ -31,6 +31,7 @@
 #include <stdint.h>
 
 #include "attn_kernel.cuh"
+#include "warp_mma.cuh"
 
 namespace intra {
 
@@ -55,6 +56,12 @@ struct DecodeParams {
   const uint8_t* mask;         // (B, S) by strides, nonzero = visible; null: every key is
   __nv_bfloat16* o;            // (B, H, 128) contiguous
   float* scratch;              // n_clusters > 1: DEC_PARTIAL floats per cluster
+  const int* lengths;          // ACCUMULATE: keys before the token's own per sequence, null: S - 1
+  float* weights;              // ACCUMULATE: (B, Hkv, S) by strides, unit stride over keys
+  int64_t weights_sb, weights_sh;
+  float* scores;               // ACCUMULATE: of every visible key, [unit][key][score_heads], times scale_log2
+  float2* stats;               // ACCUMULATE: (B, H) maximum and inverse sum of each head's probabilities
+  int score_heads;
   int64_t q_sb, q_sh;
   TensorView ks, vs;
   int64_t mask_sb, mask_ss;
@@ -65,37 +72,10 @@ struct DecodeParams {
   float scale_log2;
 };
 
-__device__ __forceinline__ void mma_m16n8k16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                             uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-// Byte offset of 16-byte piece `piece` of key row `row` in a block: the piece index is xor-ed with the row so
-// that eight rows' pieces of one column lie in different banks.
-__device__ __forceinline__ uint32_t dec_offset(int row, int piece) { return row * 256 + ((piece ^ (row & 7)) << 4); }
-// Two probabilities as a bf16 pair and the pair of their rounding errors.
-__device__ __forceinline__ void split_bf16(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-  hi = ptx::pack_bf16(p0, p1);
-  lo = ptx::pack_bf16(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
-}
-// Sum of the results of P's high and low parts. An infinite value row makes the high one infinite (or NaN, where
-// infinities meet); the low one, a rounding error of either sign or zero times infinity, must not turn it into NaN.
-__device__ __forceinline__ float join_parts(float hi, float lo) { return fabsf(hi) < CUDART_INF_F ? hi + lo : hi; }
-// Factor that brings a partial result taken against maximum m to maximum m_all (0 for an empty one).
-__device__ __forceinline__ float merge_weight(float m, float m_all) {
-  return m == -CUDART_INF_F ? 0.f : ptx::ex2(m - m_all);
-}
+// Keys a sequence's token sees, before any mask.
+__device__ __forceinline__ int decode_keys(const DecodeParams& p, int b) { return p.lengths ? min(max(p.lengths[b], 0), p.S - 1) + 1 : p.S; }
 
+template <bool ACCUMULATE>
 __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(const __grid_constant__ DecodeParams p) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(1024) uint8_t dec_smem[];            // the rings; at the end the warps' partial results
@@ -121,9 +101,10 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(co
   // ---- this CTA's key blocks: every n_dealt-th one, without those a mask hides entirely ------------------
   const int n_dealt = p.cluster * p.n_clusters;
   const int first_blk = (group % p.n_clusters) * p.cluster + rank;
-  const int n_blk = (p.S + DEC_BLOCK - 1) / DEC_BLOCK;
+  const int n_keys = ACCUMULATE ? decode_keys(p, b) : p.S;
+  const int n_blk = (n_keys + DEC_BLOCK - 1) / DEC_BLOCK;
   int n_live = first_blk < n_blk ? (n_blk - 1 - first_blk) / n_dealt + 1 : 0;
-  auto block_bits = [&](int key0) { return p.S - key0 >= DEC_BLOCK ? 0xffffu : (1u << (p.S - key0)) - 1u; };
+  auto block_bits = [&](int key0) { return n_keys - key0 >= DEC_BLOCK ? 0xffffu : (1u << (n_keys - key0)) - 1u; };
   if (p.mask != nullptr) {
     uint32_t bits = 0;
     int key0 = 0;
@@ -176,7 +157,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(co
 #pragma unroll
       for (int i = 0; i < DEC_BLOCK; i += 2) {                     // masked keys become zeros and are not read
         const uint32_t n = (seen >> (i + half)) & 1u ? 16u : 0u;
-        const uint32_t off = dec_offset(i + half, piece);
+        const uint32_t off = row_piece(i + half, piece);
         ptx::cp_async_16(dst + off, n ? kr + i * p.ks.ss : p.k, n);
         ptx::cp_async_16(dst + DEC_TILE + off, n ? vr + i * p.vs.ss : p.v, n);
       }
@@ -215,17 +196,18 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(co
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       uint32_t r[4];
-      ldmatrix_x4(kt + dec_offset(k_row, 2 * t + (mi & 1)), r);
+      ldmatrix_x4(kt + row_piece(k_row, 2 * t + (mi & 1)), r);
       mma_m16n8k16(s[0], qf[t][0], 0u, qf[t][1], 0u, r[0], r[1]);
       mma_m16n8k16(s[1], qf[t][0], 0u, qf[t][1], 0u, r[2], r[3]);
     }
     uint32_t seen;
-    block(e, seen);
+    const int key0 = block(e, seen);
     float x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int key = 2 * j + (i & 1) + 8 * (i >> 1);
       x[i] = (seen >> key) & 1u ? s[i >> 1][i & 1] * p.scale_log2 : -CUDART_INF_F;
+      if (ACCUMULATE && g < n_heads && (seen >> key) & 1u) p.scores[(int64_t(u) * p.S + key0 + key) * p.score_heads + g] = x[i];
     }
     float m_blk = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
     m_blk = fmaxf(m_blk, __shfl_xor_sync(0xffffffffu, m_blk, 1));
@@ -253,7 +235,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(co
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       uint32_t r[4];
-      ldmatrix_x4_trans(vt + dec_offset(v_row, 2 * t + (mi >> 1)), r);
+      ldmatrix_x4_trans(vt + row_piece(v_row, 2 * t + (mi >> 1)), r);
       mma_m16n8k16(o[2 * t], hi0, lo0, hi1, lo1, r[0], r[1]);
       mma_m16n8k16(o[2 * t + 1], hi0, lo0, hi1, lo1, r[2], r[3]);
     }
@@ -301,6 +283,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(co
     }
     if (p.n_clusters == 1) {
       p.o[(int64_t(b) * p.H + h0 + h) * HEAD_DIM + tid] = __float2bfloat16(l_all == 0.f ? 0.f : acc / l_all);
+      if (ACCUMULATE && tid == 0) p.stats[int64_t(b) * p.H + h0 + h] = make_float2(m_all, 1.f / l_all);
     } else {
       float* part = p.scratch + int64_t(group) * DEC_PARTIAL + h * (HEAD_DIM + 2);
       part[tid] = acc;
@@ -311,6 +294,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(co
 }
 
 // The clusters' partial results of one query head -> output row. One CTA per (batch, head), thread = dim.
+template <bool ACCUMULATE>
 __global__ void __launch_bounds__(HEAD_DIM) decode_merge_kernel(const __grid_constant__ DecodeParams p) {
   const int h = blockIdx.x % p.H, b = blockIdx.x / p.H;
   const int rep = p.H / p.Hkv;
@@ -328,6 +312,28 @@ __global__ void __launch_bounds__(HEAD_DIM) decode_merge_kernel(const __grid_con
     l_all += f * pc[HEAD_DIM + 1];
   }
   p.o[(int64_t(b) * p.H + h) * HEAD_DIM + threadIdx.x] = __float2bfloat16(l_all == 0.f ? 0.f : acc / l_all);
+  if (ACCUMULATE && threadIdx.x == 0) p.stats[blockIdx.x] = make_float2(m_all, 1.f / l_all);
+}
+
+// weights += each visible key's probabilities summed over its KV head's query heads, from the scores and every head's
+// maximum and sum. A thread per key, so the order of the sum is fixed.
+constexpr int DEC_WEIGHT_THREADS = 256;
+__global__ void __launch_bounds__(DEC_WEIGHT_THREADS) decode_weights_kernel(const __grid_constant__ DecodeParams p) {
+  const int hk = blockIdx.y % p.Hkv, b = blockIdx.y / p.Hkv;
+  const int key = blockIdx.x * DEC_WEIGHT_THREADS + threadIdx.x;
+  if (key >= decode_keys(p, b) || (p.mask != nullptr && p.mask[b * p.mask_sb + key * p.mask_ss] == 0)) return;
+  const int rep = p.H / p.Hkv;
+  const float2* const stats = p.stats + int64_t(b) * p.H + hk * rep;
+  float sum = 0.f;
+  for (int hg = 0; hg < p.head_groups; ++hg) {
+    const float* const x = p.scores + ((int64_t(blockIdx.y) * p.head_groups + hg) * p.S + key) * p.score_heads;
+    const int heads = min(rep - hg * DEC_HEADS, DEC_HEADS);
+    for (int h = 0; h < heads; ++h) {
+      const float2 st = stats[hg * DEC_HEADS + h];
+      sum += ptx::ex2(x[h] - st.x) * st.y;
+    }
+  }
+  p.weights[b * p.weights_sb + hk * p.weights_sh + key] += sum;
 }
 
 }  // namespace intra

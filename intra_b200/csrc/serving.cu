@@ -1,0 +1,269 @@
+// Host side of the serving operators behind the C ABI of include/intra_b200.h: attention of drafted tokens over a cache,
+// their verification, and what happens to the cache between two steps. Argument checks, how the work is split, launches.
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstring>
+#include <mutex>
+
+#include "cache_kernel.cuh"
+#include "host.h"
+#include "tree_kernel.cuh"
+#include "verify_kernel.cuh"
+
+namespace {
+
+using namespace intra;
+
+struct ServingState {
+  std::once_flag once;
+  int init_status = INTRA_OK;
+  int sm_count = 0;
+};
+ServingState g_serving[MAX_DEVICES];
+
+constexpr int TREE_MASK_TOKENS = 32 * 2;         // rows of mask bits the largest launch holds
+
+// Runs once per device with that device current. Allocates nothing, so a first call may be captured.
+void init_serving(int device) {
+  ServingState& st = g_serving[device];
+  int major = 0;
+  cudaError_t e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
+  if (e != cudaSuccess) { st.init_status = cuda_fail(e); return; }
+  if (major != 10) { st.init_status = INTRA_ERR_DEVICE; return; }
+  e = cudaDeviceGetAttribute(&st.sm_count, cudaDevAttrMultiProcessorCount, device);
+  if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<1>, tree_smem_bytes<1>(TREE_MASK_TOKENS));
+  if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<2>, tree_smem_bytes<2>(TREE_MASK_TOKENS));
+  if (e == cudaSuccess) e = opt_in_smem(evict_select_kernel, EVICT_SMEM_KEYS * 4);
+  if (e != cudaSuccess) st.init_status = cuda_fail(e);
+}
+
+// The device's state, set up on the first call; `guard` has made the device current.
+int serving_device(int device, const DeviceGuard& guard, const ServingState** st) {
+  if (!guard.ok) return cuda_fail(cudaGetLastError());
+  std::call_once(g_serving[device].once, init_serving, device);
+  *st = &g_serving[device];
+  return (*st)->init_status;
+}
+
+bool rows_aligned(const int64_t s[3]) { return ((s[0] | s[1] | s[2]) & 7) == 0; }
+TensorView view_of(const int64_t s[3]) { return {s[0], s[1], s[2]}; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+template <typename K, typename P>
+cudaError_t launch_cluster(K kernel, int64_t clusters, int cluster, int threads, int smem, cudaStream_t stream, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {unsigned(cluster), 1, 1};
+  cfg.gridDim = dim3(unsigned(clusters * cluster));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// How a cache of S keys is dealt out: CTAs per cluster and clusters per unit (a KV head's rows that one pass takes). As
+// many CTAs as are resident at once, two key blocks each at least; more where a CTA would get more blocks than it can list.
+void plan_tree(int64_t units, int S, int sm_count, int* cluster, int* n_clusters) {
+  const int n_blk = (S + TREE_BLOCK - 1) / TREE_BLOCK;
+  const int64_t slots = int64_t(sm_count) * TREE_CTAS_PER_SM;
+  int c = 1;
+  while (c < 8 && units * 2 * c <= slots && n_blk >= 4 * c) c *= 2;
+  while (c < 8 && n_blk > c * TREE_MAX_BLOCKS) c *= 2;
+  int n = ceil_div(n_blk, c * TREE_MAX_BLOCKS);
+  const int64_t fits = slots / (units * c);
+  n = imax(n, imin(n_blk / (16 * c), fits < 4096 ? int(fits) : 4096));
+  *cluster = c;
+  *n_clusters = n;
+}
+
+template <int MT>
+int launch_tree_mma(TreeParams& p, int B, const ServingState& st, int64_t scratch_bytes, int64_t* scratch_needed, cudaStream_t stream) {
+  const int rows = p.n * (p.H / p.Hkv);
+  p.row_groups = ceil_div(rows, 16 * MT);
+  const int64_t units = int64_t(B) * p.Hkv * p.row_groups;
+  plan_tree(units, p.S, st.sm_count, &p.cluster, &p.n_clusters);
+  const int64_t clusters = units * p.n_clusters;
+  if (clusters * p.cluster > 0x7fffffffLL || int64_t(B) * p.n * p.H > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
+  *scratch_needed = p.n_clusters > 1 ? clusters * TREE_PARTIAL<MT> * int64_t(sizeof(float)) : 0;
+  if (*scratch_needed > 0 && (!p.scratch || scratch_bytes < *scratch_needed)) return INTRA_NEED_SCRATCH;
+  const int smem = tree_smem_bytes<MT>(p.mask ? (p.mask_sn ? p.n : 1) : 0);
+  cudaError_t e = launch_cluster(tree_mma_kernel<MT>, clusters, p.cluster, TREE_THREADS, smem, stream, p);
+  if (e == cudaSuccess && p.n_clusters > 1) {
+    tree_merge_kernel<MT><<<unsigned(B) * unsigned(p.n) * unsigned(p.H), HEAD_DIM, 0, stream>>>(p);
+    e = cudaGetLastError();
+  }
+  return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
+}
+
+}  // namespace
+
+extern "C" {
+
+int intra_b200_tree_attn(const void* q, const void* k, const void* v, const int* parents, const int* lengths, const void* mask,
+                         void* out, void* scratch, int64_t scratch_bytes, int64_t* scratch_needed, int B, int S, int H, int Hkv,
+                         int n, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                         int64_t parents_batch_stride, int all_own, const int64_t mask_strides[3], float softmax_scale,
+                         int device, void* cuda_stream) {
+  if (!q || !k || !v || !out || !scratch_needed || !q_strides || !k_strides || !v_strides || (mask && !mask_strides) || B <= 0 ||
+      S <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || n <= 0 || n > S || !(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
+    return INTRA_ERR_BAD_ARG;
+  if (n > TREE_MAX_TOKENS) return INTRA_ERR_UNSUPPORTED;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(scratch) || !aligned4(parents) ||
+      !aligned4(lengths) || !rows_aligned(q_strides) || !rows_aligned(k_strides) || !rows_aligned(v_strides))
+    return INTRA_ERR_ALIGNMENT;
+  if (device < 0 || device >= MAX_DEVICES) return INTRA_ERR_BAD_ARG;
+  DeviceGuard guard(device);
+  const ServingState* st;
+  const int rc = serving_device(device, guard, &st);
+  if (rc != INTRA_OK) return rc;
+  TreeParams p = {};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.parents = parents;
+  p.lengths = lengths;
+  p.mask = static_cast<const uint8_t*>(mask);
+  p.o = static_cast<__nv_bfloat16*>(out);
+  p.scratch = static_cast<float*>(scratch);
+  p.q_sb = q_strides[0]; p.q_sn = q_strides[1]; p.q_sh = q_strides[2];
+  p.ks = view_of(k_strides);
+  p.vs = view_of(v_strides);
+  p.parents_sb = parents_batch_stride;
+  p.all_own = all_own != 0;
+  if (mask) {
+    p.mask_sb = mask_strides[0]; p.mask_sn = mask_strides[1]; p.mask_ss = mask_strides[2];
+    p.mask_vec = p.mask_ss == 1 && aligned16(mask) && ((p.mask_sb | p.mask_sn) & 15) == 0;
+  }
+  p.S = S; p.H = H; p.Hkv = Hkv; p.n = n;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  if (n * (H / Hkv) <= 16) return launch_tree_mma<1>(p, B, *st, scratch_bytes, scratch_needed, stream);
+  return launch_tree_mma<2>(p, B, *st, scratch_bytes, scratch_needed, stream);
+}
+
+int intra_b200_verify_drafts(const void* tokens, int tokens_int64, const void* target, const void* draft, int prob_type,
+                             const float* uniform, const int* parents, int* accepted, int* path, int64_t* out_tokens, int B, int n,
+                             int V, const int64_t target_strides[2], const int64_t draft_strides[2], int64_t tokens_batch_stride,
+                             int64_t uniform_batch_stride, int64_t parents_batch_stride, int device, void* cuda_stream) {
+  if (!tokens || !target || !uniform || !accepted || !path || !out_tokens || !target_strides || (draft && !draft_strides) ||
+      B <= 0 || n <= 0 || V <= 0 || prob_type < 0 || prob_type > 2)
+    return INTRA_ERR_BAD_ARG;
+  if (n > VERIFY_MAX_TOKENS || B > 0x7fffffff / VERIFY_MAX_CLUSTER) return INTRA_ERR_UNSUPPORTED;
+  const uintptr_t size = prob_type == INTRA_PROB_F32 ? 4 : 2, token_size = tokens_int64 ? 8 : 4;
+  if (reinterpret_cast<uintptr_t>(target) % size || reinterpret_cast<uintptr_t>(draft) % size || !aligned4(uniform) ||
+      !aligned4(parents) || !aligned4(accepted) || !aligned4(path) || reinterpret_cast<uintptr_t>(out_tokens) % 8 ||
+      reinterpret_cast<uintptr_t>(tokens) % token_size)
+    return INTRA_ERR_ALIGNMENT;
+  if (device < 0 || device >= MAX_DEVICES) return INTRA_ERR_BAD_ARG;
+  DeviceGuard guard(device);
+  const ServingState* st;
+  const int rc = serving_device(device, guard, &st);
+  if (rc != INTRA_OK) return rc;
+  VerifyParams p = {};
+  p.tokens = tokens; p.tokens_wide = tokens_int64 != 0;
+  p.target = target; p.draft = draft; p.uniform = uniform; p.parents = parents;
+  p.accepted = accepted; p.path = path; p.out_tokens = reinterpret_cast<long long*>(out_tokens);
+  p.target_sb = target_strides[0]; p.target_sn = target_strides[1];
+  if (draft) { p.draft_sb = draft_strides[0]; p.draft_sn = draft_strides[1]; }
+  p.tokens_sb = tokens_batch_stride; p.uniform_sb = uniform_batch_stride; p.parents_sb = parents_batch_stride;
+  p.n = n; p.V = V;
+  int c = 1;
+  while (c < VERIFY_MAX_CLUSTER && int64_t(B) * 2 * c <= 4 * st->sm_count && V >= 2048 * c) c *= 2;
+  p.cluster = c;
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  cudaError_t e;
+  if (prob_type == INTRA_PROB_F32) e = launch_cluster(verify_kernel<float>, B, c, VERIFY_THREADS, 0, stream, p);
+  else if (prob_type == INTRA_PROB_BF16) e = launch_cluster(verify_kernel<__nv_bfloat16>, B, c, VERIFY_THREADS, 0, stream, p);
+  else e = launch_cluster(verify_kernel<__half>, B, c, VERIFY_THREADS, 0, stream, p);
+  return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
+}
+
+int intra_b200_keep_drafts(void* const* caches, const int64_t* strides, int n_caches, const int* lengths, const int* path,
+                           int64_t path_batch_stride, int B, int S, int Hkv, int n, int device, void* cuda_stream) {
+  if (!caches || !strides || !lengths || !path || n_caches <= 0 || B <= 0 || S <= 0 || Hkv <= 0 || n <= 0 || n > S)
+    return INTRA_ERR_BAD_ARG;
+  if (n > KEEP_MAX_TOKENS || int64_t(B) * Hkv > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
+  if (!aligned4(lengths) || !aligned4(path)) return INTRA_ERR_ALIGNMENT;
+  for (int i = 0; i < n_caches; ++i) {
+    if (!caches[i]) return INTRA_ERR_BAD_ARG;
+    const int64_t* s = strides + 3 * i;
+    if (s[0] <= 0 || s[1] <= 0 || s[2] <= 0) return INTRA_ERR_BAD_ARG;       // rows that share memory cannot be moved apart
+    if (!aligned16(caches[i]) || !rows_aligned(s)) return INTRA_ERR_ALIGNMENT;
+  }
+  if (device < 0 || device >= MAX_DEVICES) return INTRA_ERR_BAD_ARG;
+  DeviceGuard guard(device);
+  const ServingState* st;
+  const int rc = serving_device(device, guard, &st);
+  if (rc != INTRA_OK) return rc;
+  KeepParams p;
+  p.lengths = lengths; p.path = path; p.path_sb = path_batch_stride;
+  p.S = S; p.Hkv = Hkv; p.n = n;
+  for (int first = 0; first < n_caches; first += KEEP_TENSORS) {
+    const int count = imin(n_caches - first, KEEP_TENSORS);
+    for (int i = 0; i < count; ++i) {
+      p.cache[i] = static_cast<__nv_bfloat16*>(caches[first + i]);
+      p.s[i] = view_of(strides + 3 * (first + i));
+    }
+    keep_rows_kernel<<<dim3(unsigned(B * Hkv), unsigned(count)), KEEP_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e);
+  }
+  return INTRA_OK;
+}
+
+int intra_b200_evict(const void* k, const void* v, const float* weights, const int* lengths, void* k_out, void* v_out,
+                     float* weights_out, int* kept, int B, int S, int Hkv, int keep, int recent, const int64_t k_strides[3],
+                     const int64_t v_strides[3], const int64_t weights_strides[2], const int64_t k_out_strides[3],
+                     const int64_t v_out_strides[3], const int64_t weights_out_strides[2], int device, void* cuda_stream) {
+  if (!k || !v || !weights || !k_out || !v_out || !weights_out || !kept || !k_strides || !v_strides || !weights_strides ||
+      !k_out_strides || !v_out_strides || !weights_out_strides || B <= 0 || S <= 0 || Hkv <= 0 || keep <= 0 || recent < 0 ||
+      recent > keep)
+    return INTRA_ERR_BAD_ARG;
+  for (int i = 0; i < 3; ++i)
+    if (k_out_strides[i] <= 0 || v_out_strides[i] <= 0) return INTRA_ERR_BAD_ARG;
+  if (weights_out_strides[0] <= 0 || weights_out_strides[1] <= 0) return INTRA_ERR_BAD_ARG;
+  if (!aligned16(k) || !aligned16(v) || !aligned16(k_out) || !aligned16(v_out) || !aligned4(weights) || !aligned4(weights_out) ||
+      !aligned4(lengths) || !aligned4(kept) || !rows_aligned(k_strides) || !rows_aligned(v_strides) ||
+      !rows_aligned(k_out_strides) || !rows_aligned(v_out_strides))
+    return INTRA_ERR_ALIGNMENT;
+  if (device < 0 || device >= MAX_DEVICES) return INTRA_ERR_BAD_ARG;
+  const int64_t units = int64_t(B) * Hkv;
+  const int64_t copies = units * ceil_div(keep, EVICT_COPY_THREADS / 16 * EVICT_ROWS);
+  if (units * EVICT_MAX_CLUSTER > 0x7fffffffLL || copies > 0x7fffffffLL || int64_t(S) + EVICT_THREADS * EVICT_MAX_CLUSTER > 0x7fffffffLL ||
+      int64_t(keep) + EVICT_THREADS * EVICT_MAX_CLUSTER > 0x7fffffffLL)
+    return INTRA_ERR_UNSUPPORTED;
+  DeviceGuard guard(device);
+  const ServingState* st;
+  const int rc = serving_device(device, guard, &st);
+  if (rc != INTRA_OK) return rc;
+  EvictParams p = {};
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.weights = weights; p.lengths = lengths;
+  p.k2 = static_cast<__nv_bfloat16*>(k_out);
+  p.v2 = static_cast<__nv_bfloat16*>(v_out);
+  p.weights2 = weights_out; p.kept = kept;
+  p.ks = view_of(k_strides); p.vs = view_of(v_strides); p.k2s = view_of(k_out_strides); p.v2s = view_of(v_out_strides);
+  p.weights_sb = weights_strides[0]; p.weights_sh = weights_strides[1];
+  p.weights2_sb = weights_out_strides[0]; p.weights2_sh = weights_out_strides[1];
+  p.S = S; p.Hkv = Hkv; p.keep = keep; p.recent = recent;
+  int c = 1;
+  while (c < EVICT_MAX_CLUSTER && units * 2 * c <= 2 * st->sm_count && S >= 2048 * c) c *= 2;
+  while (c < EVICT_MAX_CLUSTER && ceil_div(S, c) > EVICT_SMEM_KEYS) c *= 2;
+  p.cluster = c;
+  p.part = ceil_div(S, c);
+  p.in_smem = p.part <= EVICT_SMEM_KEYS;
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  cudaError_t e = launch_cluster(evict_select_kernel, units, c, EVICT_THREADS, p.in_smem ? p.part * 4 : 0, stream, p);
+  if (e == cudaSuccess) {
+    evict_copy_kernel<<<unsigned(copies), EVICT_COPY_THREADS, 0, stream>>>(p);
+    e = cudaGetLastError();
+  }
+  return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
+}
+
+}  // extern "C"

@@ -7,7 +7,9 @@ steps because the patterns are prefill-only. This module offers the same callabl
 running on the B200 kernels: query/key/value arrive as (B, H, S, D) and are handed to the kernel as
 (B, S, H, D) views without copies. The decode step is dense over the cache, as in the reference: on the
 library's decode kernel for bf16 caches with or without a padding mask, else, and for multi-head caches that
-SDPA is quicker on, one SDPA call.
+SDPA is quicker on, one SDPA call. A few tokens behind a cache (2 to 64, e.g. the drafts of assisted generation), which
+the reference's callable has no path for, are dense as well, on the kernel of `serving.tree_attn`: causal where there is
+no mask, else as the boolean mask (B or 1, 1, tokens or 1, keys) says.
 
     from transformers import AttentionInterface
     AttentionInterface.register("intra_b200", make_intra_attention())
@@ -19,6 +21,7 @@ import torch
 import torch.nn.functional as F
 
 from .interface import _llm, decode_attn
+from .serving import MAX_TOKENS, _tree
 
 NUM_GROUPS = 8          # intra_token_attn.py:22-24
 WINDOW_BACK = 512
@@ -72,6 +75,10 @@ def make_intra_attention(num_groups: int = NUM_GROUPS, back: int = WINDOW_BACK, 
             am = attention_mask[:, :, :, : k2.shape[-2]] if attention_mask is not None else None
             o = F.scaled_dot_product_attention(query, k2, v2, attn_mask=am, scale=scaling, is_causal=False)
             return o.transpose(1, 2).contiguous(), None
+        if 1 < query.shape[2] < key.shape[2] and query.shape[2] <= MAX_TOKENS:     # drafted tokens behind a cache: dense, too
+            if torch.is_grad_enabled():
+                query, key, value = query.detach(), key.detach(), value.detach()
+            return _tree(query, key, value, None, None, attention_mask, scaling, attention_mask is not None), None
         mt = force_masktype if force_masktype is not None else layer_masktype(getattr(module, "layer_idx", 0))
         if torch.is_grad_enabled():          # the kernels are forward-only; this callable is, too
             query, key, value = query.detach(), key.detach(), value.detach()
