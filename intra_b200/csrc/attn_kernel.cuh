@@ -102,4 +102,25 @@ __device__ __forceinline__ void issue_pv(uint32_t p_tmem, uint32_t v_smem, uint3
   issue_pv_desc(p_tmem, tile_desc_mnmajor(v_smem), o_tmem, accumulate);
 }
 
+// S = Q K^T and O (+)= P V of one tile as rolled loops over the eight 16-deep steps; a step's issue takes less
+// than its MMA.
+__device__ __forceinline__ void issue_qk_loop(uint64_t q_desc, uint64_t k_desc, uint32_t s_tmem) {
+  constexpr uint32_t idesc = ptx::idesc_bf16_f32(TILE_M, TILE_N, 0, 0);
+#pragma unroll 1
+  for (int s = 0; s < HEAD_DIM / 16; ++s) {
+    ptx::mma_ss(s_tmem, q_desc, k_desc, idesc, s);
+    const uint64_t step = s == 3 ? (HALF_BYTES - 3 * 32) >> 4 : 32 >> 4;
+    q_desc += step;
+    k_desc += step;
+  }
+}
+__device__ __forceinline__ void issue_pv_loop(uint32_t p_tmem, uint64_t v_desc, uint32_t o_tmem, uint32_t accumulate) {
+  constexpr uint32_t idesc = ptx::idesc_bf16_f32(TILE_M, HEAD_DIM, 0, 1);
+#pragma unroll 1
+  for (int s = 0; s < TILE_N / 16; ++s) {
+    ptx::mma_ts(o_tmem, p_tmem + s * 8, v_desc, idesc, accumulate | s);
+    v_desc += 2048 >> 4;
+  }
+}
+
 }  // namespace intra

@@ -144,27 +144,6 @@ __device__ __forceinline__ void fetch_kv_tile(const TmaMaps& maps, int operand, 
   ptx::tma_load_5d_at(dst + HALF_BYTES, m, bar, 64, c1, c2, head, batch);
 }
 
-// S = Q K^T and O (+)= P V of one tile as rolled loops over the eight 16-deep steps (attn_kernel.cuh has the
-// operand layouts); a step's issue takes less than its MMA.
-__device__ __forceinline__ void issue_qk_loop(uint64_t q_desc, uint64_t k_desc, uint32_t s_tmem) {
-  constexpr uint32_t idesc = ptx::idesc_bf16_f32(TILE_M, TILE_N, 0, 0);
-#pragma unroll 1
-  for (int s = 0; s < HEAD_DIM / 16; ++s) {
-    ptx::mma_ss(s_tmem, q_desc, k_desc, idesc, s);
-    const uint64_t step = s == 3 ? (HALF_BYTES - 3 * 32) >> 4 : 32 >> 4;
-    q_desc += step;
-    k_desc += step;
-  }
-}
-__device__ __forceinline__ void issue_pv_loop(uint32_t p_tmem, uint64_t v_desc, uint32_t o_tmem, uint32_t accumulate) {
-  constexpr uint32_t idesc = ptx::idesc_bf16_f32(TILE_M, HEAD_DIM, 0, 1);
-#pragma unroll 1
-  for (int s = 0; s < TILE_N / 16; ++s) {
-    ptx::mma_ts(o_tmem, p_tmem + s * 8, v_desc, idesc, accumulate | s);
-    v_desc += 2048 >> 4;
-  }
-}
-
 // Split key lists (Gather-0): which of the two K (or V) buffers the next tile goes to, and when that one is free.
 // Image tiles: each sub-tile's own. Text tiles are the same for both sub-tiles: one load for both, 20 loads for
 // the 14 products of a patch item instead of 28 (at four tiles per step the copies alone took 3,700 cycles,

@@ -20,6 +20,7 @@
 #include "gather_kernel.cuh"
 #include "host.h"
 #include "selftest.cuh"
+#include "tma_encode.h"
 
 thread_local int intra::g_last_cuda_error = 0;
 
@@ -104,36 +105,6 @@ int problem_from(int family, int pattern, int S, int param, Problem* prob) {
 }
 
 // ---- tensor maps ------------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// cuTensorMapEncodeTiled through the runtime, so the library does not link against libcuda.
-EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess ||
-        r != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<EncodeTiledFn>(f);
-  }();
-  return fn;
-}
-
-bool encode_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides_bytes,
-                const cuuint32_t* box, const cuuint32_t* estr) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return false;
-  for (int i = 0; i < rank; ++i)
-    if (dims[i] == 0 || dims[i] > 0xffffffffull || box[i] == 0 || box[i] > 256) return false;
-  for (int i = 0; i + 1 < rank; ++i)
-    if (strides_bytes[i] == 0 || strides_bytes[i] % 16 != 0 || strides_bytes[i] >= (1ull << 40)) return false;
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides_bytes, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // The views of tma_maps.h for one (batch, token, head, 128) tensor with `heads` heads; operand 0 q, 1 k, 2 v, 3 the
 // output, whose boxes have 32 rows and which only the language-model patterns store through views.
 bool build_maps(const Problem& p, const __nv_bfloat16* ptr, const TensorView& tv, int heads, int B, int operand, TmaMaps* maps) {
@@ -660,6 +631,12 @@ int intra_b200_device_status(int device, int* status_word, int reset) {
   cudaError_t e = cudaDeviceSynchronize();
   if (e == cudaSuccess) e = cudaMemcpy(status_word, g_dev[device].status_word, sizeof(int), cudaMemcpyDeviceToHost);
   if (e == cudaSuccess && reset && *status_word != 0) e = cudaMemset(g_dev[device].status_word, 0, sizeof(int));
+  int* serving = nullptr;         // the kernels of serving.cu have a word of their own
+  int serving_word = 0;
+  if (e == cudaSuccess) e = serving_status_word(&serving);
+  if (e == cudaSuccess) e = cudaMemcpy(&serving_word, serving, sizeof(int), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess && reset && serving_word != 0) e = cudaMemset(serving, 0, sizeof(int));
+  if (e == cudaSuccess && *status_word == 0) *status_word = serving_word;
   if (e != cudaSuccess) return cuda_fail(e);
   return *status_word == 0 ? INTRA_OK : INTRA_ERR_KERNEL;
 }

@@ -9,6 +9,9 @@ namespace intra {
 
 extern thread_local int g_last_cuda_error;      // capi.cu
 
+// The current device's status word of the kernels of serving.cu.
+cudaError_t serving_status_word(int** word);
+
 constexpr int MAX_DEVICES = 64;
 
 // Every failure is reported once: the runtime's own record of it is cleared, or the check after the next launch

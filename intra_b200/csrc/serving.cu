@@ -8,17 +8,23 @@
 
 #include "cache_kernel.cuh"
 #include "host.h"
+#include "tma_encode.h"
 #include "tree_kernel.cuh"
+#include "tree_umma_kernel.cuh"
 #include "verify_kernel.cuh"
 
 namespace {
 
 using namespace intra;
 
+// Where this file's kernels record a bounded wait that ran out. Part of the library image, so that nothing is allocated.
+__device__ int g_serving_status;
+
 struct ServingState {
   std::once_flag once;
   int init_status = INTRA_OK;
   int sm_count = 0;
+  int* status_word = nullptr;     // g_serving_status on this device
 };
 ServingState g_serving[MAX_DEVICES];
 
@@ -34,6 +40,11 @@ void init_serving(int device) {
   e = cudaDeviceGetAttribute(&st.sm_count, cudaDevAttrMultiProcessorCount, device);
   if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<1>, tree_smem_bytes<1>(TREE_MASK_TOKENS));
   if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<2>, tree_smem_bytes<2>(TREE_MASK_TOKENS));
+  if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<false>, UMMA_SMEM_BYTES<false>);
+  if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<true>, UMMA_SMEM_BYTES<true>);
+  void* word = nullptr;
+  if (e == cudaSuccess) e = cudaGetSymbolAddress(&word, g_serving_status);
+  st.status_word = static_cast<int*>(word);
   if (e == cudaSuccess) e = opt_in_smem(evict_select_kernel, EVICT_SMEM_KEYS * 4);
   if (e != cudaSuccess) st.init_status = cuda_fail(e);
 }
@@ -99,7 +110,47 @@ int launch_tree_mma(TreeParams& p, int B, const ServingState& st, int64_t scratc
   return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
 }
 
+bool cache_map(const __nv_bfloat16* ptr, const TensorView& v, int S, int Hkv, int B, CUtensorMap* map) {
+  const cuuint64_t dims[5] = {HEAD_DIM, cuuint64_t(S), 1, cuuint64_t(Hkv), cuuint64_t(B)};
+  const int64_t row = S > 1 ? v.ss : HEAD_DIM, head = Hkv > 1 ? v.sh : HEAD_DIM, batch = B > 1 ? v.sb : HEAD_DIM;
+  if (row <= 0 || head <= 0 || batch <= 0) return false;
+  const cuuint64_t strides[4] = {cuuint64_t(row) * 2, cuuint64_t(row) * 2, cuuint64_t(head) * 2, cuuint64_t(batch) * 2};
+  const cuuint32_t box[5] = {64, TILE_N, 1, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+  return encode_map(map, ptr, 5, dims, strides, box, ones);
+}
+
+template <bool PAIR>
+int launch_tree_umma(const TreeParams& t, int B, const ServingState& st, int64_t scratch_bytes, int64_t* scratch_needed, cudaStream_t stream) {
+  TreeUmmaParams p;
+  p.t = t;
+  p.B = B;
+  p.t.row_groups = ceil_div(t.n * (t.H / t.Hkv), UMMA_ROWS<PAIR>);
+  const int64_t tiles = int64_t(B) * t.Hkv * p.t.row_groups * ceil_div(t.S, TILE_N);       // at most
+  const int64_t parts = (tiles + UMMA_MIN_TILES - 1) / UMMA_MIN_TILES;
+  const int64_t rows = int64_t(B) * t.n * t.H;
+  if (tiles / B > 0x7fffffffLL || rows > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
+  const int grid = parts < st.sm_count ? int(parts) : st.sm_count;
+  *scratch_needed = grid * 2 * UMMA_PARTIAL<PAIR> * int64_t(sizeof(float));
+  if (!t.scratch || scratch_bytes < *scratch_needed) return INTRA_NEED_SCRATCH;
+  p.use_tma = cache_map(t.k, t.ks, t.S, t.Hkv, B, &p.maps[0]) && cache_map(t.v, t.vs, t.S, t.Hkv, B, &p.maps[1]);
+  p.status = st.status_word;
+  tree_umma_kernel<PAIR><<<grid, UMMA_THREADS, UMMA_SMEM_BYTES<PAIR>, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) {
+    tree_umma_merge_kernel<PAIR><<<unsigned((rows + UMMA_MERGE_ROWS - 1) / UMMA_MERGE_ROWS), 32 * UMMA_MERGE_ROWS, 0, stream>>>(p, grid);
+    e = cudaGetLastError();
+  }
+  return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
+}
+
 }  // namespace
+
+cudaError_t intra::serving_status_word(int** word) {
+  void* ptr = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&ptr, g_serving_status);
+  *word = static_cast<int*>(ptr);
+  return e;
+}
 
 extern "C" {
 
@@ -141,6 +192,8 @@ int intra_b200_tree_attn(const void* q, const void* k, const void* v, const int*
   p.S = S; p.H = H; p.Hkv = Hkv; p.n = n;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  if (!mask && n * (H / Hkv) > 128) return launch_tree_umma<true>(p, B, *st, scratch_bytes, scratch_needed, stream);
+  if (!mask && n * (H / Hkv) > 32) return launch_tree_umma<false>(p, B, *st, scratch_bytes, scratch_needed, stream);
   if (n * (H / Hkv) <= 16) return launch_tree_mma<1>(p, B, *st, scratch_bytes, scratch_needed, stream);
   return launch_tree_mma<2>(p, B, *st, scratch_bytes, scratch_needed, stream);
 }

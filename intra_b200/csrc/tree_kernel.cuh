@@ -69,7 +69,7 @@ __device__ __forceinline__ int tree_context(const TreeParams& p, int b) {
 // thread arrives. A parent that is not an earlier token ends the walk. Pointer doubling: six rounds for 64 tokens.
 __device__ __forceinline__ void tree_ancestors(const TreeParams& p, int b, int tid, unsigned long long* anc, int8_t* up) {
   if (p.all_own || p.parents == nullptr) {
-    if (tid < p.n) anc[tid] = p.all_own ? ~0ull : (2ull << tid) - 1ull;
+    if (tid < p.n) anc[tid] = (2ull << (p.all_own ? p.n - 1 : tid)) - 1ull;
     __syncthreads();
     return;
   }

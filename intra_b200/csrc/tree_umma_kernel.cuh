@@ -1,0 +1,644 @@
+// Attention of drafted tokens over a cache (tree_kernel.cuh) for more rows than a warp's registers hold: the products on
+// tcgen05 with 128 rows a tile, K and V tiles of 128 keys.
+//
+// Up to 256 rows the bound is still reading K and V (64 KB a key tile, 2,800 cycles at an SM's share of the HBM
+// bandwidth; the products of 256 rows take 2,048). So the work is dealt by key tiles, whatever sequence they belong to: all
+// tiles of all units - a unit is a KV head of a sequence, with up to ROWS rows - stand in one list, CTA c takes
+// the c-th part of it. A unit that no CTA holds as a whole leaves partial results (the sum, its maximum and
+// weight) that tree_umma_merge_kernel joins.
+//
+// Two streams of softmax work run side by side, so that the tensor cores have one's products while the other is at its
+// exponentials:
+//   PAIR (more than 128 rows): the streams are two tiles of 128 rows that read the same K and V tiles. Tensor memory:
+//     one score buffer that a stream hands back as soon as it has copied its scores out, P0 and P1 in bf16, O0, O1.
+//   otherwise: the streams are the even and the odd key tiles of the same rows. There is room for P as two bf16 numbers
+//     (16 significant bits) over each stream's own scores; O0 and O1 are joined at the end of a unit.
+//
+// Warp roles (512 threads): warps 0-3 and 4-7 softmax sets of the streams, a thread owning a row, which also write
+// the results; 8-11 request the tiles: TMA where a tile's rows are all keys of the sequence and the cache's strides
+// allow, else 16-byte copies in which rows past its last key become zeros; 12 issues QK^T (and, but for PAIR, PV), 13 PV.
+//
+// Barriers, all waits bounded (2 s; see attn_kernel.cuh for what a CTA does that gives up):
+//   full[r], free[r]   ring of tile buffers, in the order K0 K1 V0 K2 V1 .. over the CTA's tiles
+//   q_full, q_free     per unit: the query rows are there / their last QK^T has completed
+//   s_full[s]          scores of stream s are there (and all products before them are complete)
+//   s_taken[s]         PAIR: set s has copied its scores of a tile
+//   p_full[s], pv_done[s]   set s has stored its probabilities / PV_s has completed
+//   o_done[s]          the last PV_s of a unit has completed
+//   o_free[s]          set s has read O (of both streams, but for PAIR) of a unit
+//   ml_ready[s][u & 1] not PAIR: set s has published its rows' maxima and sums of unit u
+// Each completes again only after its waiters have seen the completion before. A wait for "the phase before the first"
+// (parity 1 of a fresh barrier) returns at once.
+#pragma once
+#include <cuda.h>
+
+#include "softmax.cuh"
+#include "tree_kernel.cuh"
+
+namespace intra {
+
+constexpr int UMMA_THREADS = 512;
+constexpr int UMMA_SM_REGS = 184, UMMA_LOAD_REGS = 64, UMMA_ISSUE_REGS = 80;
+static_assert(256 * UMMA_SM_REGS + 128 * (UMMA_LOAD_REGS + UMMA_ISSUE_REGS) <= 65536,
+              "register budgets exceed what the CTA was launched with: setmaxnreg.inc would never return");
+template <bool PAIR> constexpr int UMMA_ROWS = PAIR ? 2 * TILE_M : TILE_M;       // rows of a unit
+constexpr int UMMA_RING = 5;                     // tile buffers
+template <bool PAIR> constexpr int UMMA_SMEM_BYTES = (UMMA_RING + (PAIR ? 2 : 1)) * TILE_BYTES + 1024;
+// Partial results: a CTA leaves at most two, of the unit its part begins in and of the one it ends in. Each is the rows'
+// sums, then their maxima (log2 units) and weights.
+template <bool PAIR> constexpr int64_t UMMA_PARTIAL = int64_t(UMMA_ROWS<PAIR>) * (HEAD_DIM + 2);
+// A CTA's part is at least this many key tiles: a shorter one costs more in its ends and its merge than it spreads.
+constexpr int UMMA_MIN_TILES = 2;
+
+struct TreeUmmaParams {
+  TreeParams t;                // row_groups: units per KV head
+  CUtensorMap maps[2];         // K, V: (128, S, 1, Hkv, B)
+  int use_tma;
+  int B;
+  int* status;
+};
+
+struct TreePiece {             // what a CTA does of one unit
+  int b, hk, rg;               // sequence, KV head, row group
+  int first, count;            // key tiles
+  int of;                      // key tiles of the whole unit
+  int ctx, n_keys;
+};
+__device__ __forceinline__ int tree_tiles(const TreeParams& p, int b) { return (tree_context(p, b) + p.n + TILE_N - 1) / TILE_N; }
+
+// The list of all units' key tiles, and a CTA's part [next, end) of it as a cursor that every role moves by itself.
+struct TreeWalk {
+  int64_t per, next, end;      // length of a part; places in the list
+  int64_t b_start;             // place of sequence b's first tile
+  int b, b_tiles;              // b_tiles: of one unit
+  // Called by whole warps; all lanes get the same.
+  __device__ __forceinline__ TreeWalk(const TreeParams& p, int B, int cta, int grid) {
+    const int lane = threadIdx.x & 31, units = p.Hkv * p.row_groups;
+    int64_t total = 0;
+    for (int s = lane; s < B; s += 32) total += tree_tiles(p, s);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    total *= units;
+    per = (total + grid - 1) / grid;
+    per = per < UMMA_MIN_TILES ? UMMA_MIN_TILES : per;
+    next = per * cta;
+    end = next + per < total ? next + per : total;
+    b = b_tiles = 0;
+    b_start = 0;
+    if (next >= end) return;
+    for (int s0 = 0; s0 < B; s0 += 32) {                           // the sequence that holds `next`
+      const int64_t mine = s0 + lane < B ? int64_t(tree_tiles(p, s0 + lane)) * units : 0;
+      int64_t upto = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += y;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, b_start + upto > next);
+      if (past) {
+        b = s0 + __ffs(past) - 1;
+        b_start += __shfl_sync(0xffffffffu, upto - mine, __ffs(past) - 1);
+        break;
+      }
+      b_start += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    b_tiles = tree_tiles(p, b);
+  }
+  __device__ __forceinline__ bool piece(const TreeParams& p, TreePiece& x) {
+    if (next >= end) return false;
+    const int units = p.Hkv * p.row_groups;
+    if (next - b_start >= int64_t(b_tiles) * units) {
+      b_start += int64_t(b_tiles) * units;
+      b_tiles = tree_tiles(p, ++b);
+    }
+    const int local = int(next - b_start), unit = local / b_tiles;
+    x.b = b;
+    x.hk = unit / p.row_groups;
+    x.rg = unit - x.hk * p.row_groups;
+    x.of = b_tiles;
+    x.first = local - unit * b_tiles;
+    x.count = int(end - next < b_tiles - x.first ? end - next : b_tiles - x.first);
+    x.ctx = tree_context(p, b);
+    x.n_keys = x.ctx + p.n;
+    next += x.count;
+    return true;
+  }
+};
+
+// tree_ancestors for one warp: the tokens' own keys that `token` sees, as bits. A lane holds tokens lane and lane + 32.
+__device__ __forceinline__ unsigned long long tree_own_keys(const TreeParams& p, int b, int token) {
+  if (p.all_own) return (2ull << (p.n - 1)) - 1ull;
+  if (p.parents == nullptr) return (2ull << token) - 1ull;
+  const int lane = threadIdx.x & 31;
+  unsigned long long anc[2];
+  int up[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int i = lane + 32 * c, parent = i < p.n ? p.parents[b * p.parents_sb + i] : -1;
+    up[c] = parent >= 0 && parent < i ? parent : -1;
+    anc[c] = 1ull << i;
+  }
+  auto of_token = [](const unsigned long long (&x)[2], int i) {
+    const unsigned long long a = __shfl_sync(0xffffffffu, x[0], i & 31), c = __shfl_sync(0xffffffffu, x[1], i & 31);
+    return i & 32 ? c : a;
+  };
+  for (int reach = 1; reach < p.n; reach *= 2) {
+    unsigned long long more[2];
+    int next[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int i = up[c] < 0 ? 0 : up[c];
+      const int a = __shfl_sync(0xffffffffu, up[0], i & 31), d = __shfl_sync(0xffffffffu, up[1], i & 31);
+      const unsigned long long x = of_token(anc, i);
+      more[c] = up[c] < 0 ? 0ull : x;
+      next[c] = up[c] < 0 ? -1 : i & 32 ? d : a;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) { anc[c] |= more[c]; up[c] = next[c]; }
+  }
+  return of_token(anc, token);
+}
+
+// Where a row's result goes: bf16 into the output where its unit is whole, else fp32.
+struct TreeRowOut {
+  __nv_bfloat16* out;
+  float* part;                 // null: whole
+};
+
+// COLS columns from `col` on of one row of a piece, key by key, for rows whose sums are not finite: an infinite or NaN value row
+// makes every row's sum NaN, also those of tokens that do not see it (zero times infinity). m and l are the row's.
+template <int COLS>
+__device__ __noinline__ void tree_exact_row(const TreeParams& p, const TreePiece& pc, unsigned long long own, int token, int head, int col,
+                                            float m, float l, const TreeRowOut& dst) {
+  float acc[COLS];
+  for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+  const __nv_bfloat16* const q = p.q + pc.b * p.q_sb + head * p.q_sh + token * p.q_sn;
+  const int last = min((pc.first + pc.count) * TILE_N, pc.n_keys);
+  for (int key = pc.first * TILE_N; key < last; ++key) {
+    if (key >= pc.ctx && !((own >> (key - pc.ctx)) & 1ull)) continue;
+    const __nv_bfloat16* const k = p.k + pc.b * p.ks.sb + pc.hk * p.ks.sh + key * p.ks.ss;
+    const __nv_bfloat16* const v = p.v + pc.b * p.vs.sb + pc.hk * p.vs.sh + key * p.vs.ss + col;
+    float s = 0.f;
+    for (int c = 0; c < HEAD_DIM; ++c) s += __bfloat162float(q[c]) * __bfloat162float(k[c]);
+    const float prob = ptx::ex2(s * p.scale_log2 - m);
+    for (int c = 0; c < COLS; ++c) acc[c] += prob * __bfloat162float(v[c]);
+  }
+  for (int c = 0; c < COLS; ++c) {
+    if (dst.part != nullptr) dst.part[col + c] = acc[c];
+    else dst.out[col + c] = __float2bfloat16(l == 0.f ? 0.f : acc[c] / l);
+  }
+}
+
+template <bool PAIR>
+__global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid_constant__ TreeUmmaParams p) {
+  constexpr int RING = UMMA_RING, ROWS = UMMA_ROWS<PAIR>, COLS = PAIR ? HEAD_DIM : HEAD_DIM / 2;
+  enum : int {
+    FULL = 0, FREE = FULL + RING, Q_FULL = FREE + RING, Q_FREE, S_FULL, S_TAKEN = S_FULL + 2, P_FULL = S_TAKEN + 2,
+    PV_DONE = P_FULL + 2, O_DONE = PV_DONE + 2, O_FREE = O_DONE + 2, ML_READY = O_FREE + 2, DRAIN = ML_READY + 4, N_BARS = DRAIN + 2
+  };
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bars[N_BARS];
+  __shared__ uint32_t tmem_base_smem;
+  __shared__ int abort_flag;
+  __shared__ float2 row_ml[2][PAIR ? 1 : 2][PAIR ? 1 : TILE_M];     // [unit parity][stream][row]
+  const TreeParams& t = p.t;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t q_smem = smem_base, ring_smem = smem_base + (PAIR ? 2 : 1) * TILE_BYTES;
+  const uint32_t bar0 = ptx::smem_u32(bars);
+  auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
+  const int rep = t.H / t.Hkv, all_rows = t.n * rep;
+
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < N_BARS; ++i) {
+      int n = 1;
+      if (i < FREE || i == Q_FULL) n = 128;
+      if ((i >= S_TAKEN && i < PV_DONE) || (i >= O_FREE && i < DRAIN)) n = 4;
+      ptx::mbar_init(&bars[i], n);
+    }
+    ptx::fence_mbar_init();
+  }
+  if (warp == 0) {
+    ptx::tmem_alloc(&tmem_base_smem, 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = tmem_base_smem;
+  volatile int* abort_p = &abort_flag;
+  bool ok = true;
+#define TREE_WAIT(index, parity, code) ptx::mbar_wait_at(bar(index), (parity) & 1, abort_p, code)
+  TreeWalk walk(t, p.B, blockIdx.x, gridDim.x);
+  TreePiece pc;
+  // Ring requests of tile j, counted over the CTA: its K, and its V behind the next tile's K.
+  auto k_request = [](uint32_t j) { return j == 0 ? 0u : 2 * j - 1; };
+  auto v_request = [](uint32_t j) { return 2 * j + 2; };
+
+  if (warp < 8) {
+    // ================================ softmax sets, results =======================================
+    ptx::setmaxnreg_inc<UMMA_SM_REGS>();
+    const int sx = warp >> 2, row = tid & 127;
+    const uint32_t lane_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t s_addr = lane_addr + (PAIR ? 0 : sx * 128);
+    const uint32_t p_addr = PAIR ? lane_addr + 128 + sx * 64 : s_addr;
+    const uint32_t o_addr = lane_addr + 256 + sx * 128;
+    uint32_t kt = 0, unit = 0, done[2] = {0, 0};          // tiles of this stream, units, units in which a stream had tiles
+    while (walk.piece(t, pc)) {
+      const int r = pc.rg * ROWS + (PAIR ? sx * TILE_M : 0) + row;
+      const bool valid = r < all_rows, busy = __any_sync(0xffffffffu, valid);
+      const int token = min(r, all_rows - 1) / rep, head = pc.hk * rep + min(r, all_rows - 1) - token * rep;
+      const unsigned long long own = (pc.first + pc.count) * TILE_N > pc.ctx ? tree_own_keys(t, pc.b, token) : 0ull;
+      float m_run = -CUDART_INF_F, l_run = 0.f;
+      const int n_mine = PAIR ? pc.count : (pc.count + 1 - sx) / 2;
+#pragma unroll 1
+      for (int i = 0; i < n_mine; ++i, ++kt) {
+        const int key0 = (pc.first + (PAIR ? i : 2 * i + sx)) * TILE_N;
+        ok = TREE_WAIT(S_FULL + sx, kt, 11 + sx);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        if (!busy) {                                      // no row of this warp exists: its results are never read
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR) ptx::mbar_arrive_at(bar(S_TAKEN + sx));
+            ptx::mbar_arrive_at(bar(P_FULL + sx));
+          }
+          continue;
+        }
+        float s[TILE_N];
+        uint32_t* const su = reinterpret_cast<uint32_t*>(s);
+        float tile_max;
+        auto chunk_max = [&](int c) { return sm::row_max(*reinterpret_cast<const float(*)[32]>(&s[32 * c])); };
+        if (key0 + TILE_N <= pc.ctx) {                    // every token sees the whole tile
+          ptx::tmem_ld32(s_addr, su);
+          ptx::tmem_wait_ld();
+          ptx::tmem_ld32(s_addr + 32, su + 32);
+          tile_max = chunk_max(0);
+          ptx::tmem_wait_ld();
+          ptx::tmem_ld32(s_addr + 64, su + 64);
+          tile_max = fmaxf(tile_max, chunk_max(1));
+          ptx::tmem_wait_ld();
+          ptx::tmem_ld32(s_addr + 96, su + 96);
+          tile_max = fmaxf(tile_max, chunk_max(2));
+          ptx::tmem_wait_ld();
+          if (PAIR) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_at(bar(S_TAKEN + sx));
+          }
+          tile_max = fmaxf(tile_max, chunk_max(3));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) ptx::tmem_ld32(s_addr + 32 * c, su + 32 * c);
+          ptx::tmem_wait_ld();
+          if (PAIR) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_at(bar(S_TAKEN + sx));
+          }
+          tile_max = -CUDART_INF_F;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int at = key0 + 32 * c - pc.ctx;        // place of the chunk's first key among the tokens' own
+            const uint32_t seen = at >= 0 ? (at < 64 ? uint32_t(own >> at) : 0u) : at <= -32 ? ~0u : uint32_t(own << -at) | ((1u << -at) - 1u);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[32 * c + e] = (seen >> e) & 1u ? s[32 * c + e] : -CUDART_INF_F;
+            tile_max = fmaxf(tile_max, chunk_max(c));
+          }
+        }
+        const float m_new = fmaxf(m_run, tile_max);
+        // the maximum moves only when the scores outgrow it by 2^8; until then probabilities are merely scaled
+        const bool grow = (m_new - m_run) * t.scale_log2 > RESCALE_THRESHOLD;
+        float alpha = 1.f;
+        if (grow) {
+          alpha = ptx::ex2((m_run - m_new) * t.scale_log2);
+          l_run *= alpha;
+          m_run = m_new;
+        }
+        // The stream's PV before this one reads P and writes O. Where P stands over the scores, it has completed before
+        // they came (one thread issues both, in order); else it is waited for.
+        if (PAIR) {
+          ok = TREE_WAIT(PV_DONE + sx, kt - 1, 13 + sx);
+          if (!ok) break;
+          ptx::tc_fence_after();
+        }
+        if (i > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+          for (int c = 0; c < HEAD_DIM / 16; ++c) {
+            uint32_t o[16];
+            ptx::tmem_ld16(o_addr + c * 16, o);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            ptx::tmem_st16(o_addr + c * 16, o);
+          }
+        }
+        const float base = m_run == -CUDART_INF_F ? 0.f : m_run * t.scale_log2;
+        sm::f2 sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+          if (PAIR) {
+            sm::exp_chunk<sm::EX2_FMA_PAIRS_NONE>(s, c * 32, t.scale_log2, base, pk, sum);
+            ptx::tmem_st16(p_addr + c * 16, pk);
+          } else {
+            uint32_t lo[16];
+            const sm::f2 scale2 = sm::pack2(t.scale_log2, t.scale_log2), nbase2 = sm::pack2(-base, -base);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float x0, x1;
+              sm::unpack2(sm::fma2(sm::pack2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), scale2, nbase2), x0, x1);
+              const float p0 = ptx::ex2(x0), p1 = ptx::ex2(x1);
+              sum[e & 3] = sm::add2(sum[e & 3], sm::pack2(p0, p1));
+              split_bf16(p0, p1, pk[e], lo[e]);
+            }
+            ptx::tmem_st16(p_addr + c * 16, pk);
+            ptx::tmem_st16(p_addr + 64 + c * 16, lo);
+          }
+        }
+        l_run += sm::sum4(sum);
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_at(bar(P_FULL + sx));
+      }
+      if (!ok) break;
+
+      // ---- results ----------------------------------------------------------------------------------------
+      const int n_other = PAIR ? 0 : (pc.count + sx) / 2;                 // tiles of the other stream
+      float m = m_run == -CUDART_INF_F ? -CUDART_INF_F : m_run * t.scale_log2, l = l_run;
+      float w_mine = 1.f, w_other = 0.f;
+      if (!PAIR) {                                        // the two streams' sums are of the same rows
+        float2(*const ml)[PAIR ? 1 : TILE_M] = row_ml[unit & 1];
+        ml[sx][PAIR ? 0 : row] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_at(bar(ML_READY + 2 * sx + (unit & 1)));
+        ok = TREE_WAIT(ML_READY + 2 * (sx ^ 1) + (unit & 1), unit >> 1, 45 + sx);
+        if (!ok) break;
+        const float2 other = ml[sx ^ 1][PAIR ? 0 : row];
+        const float m_all = fmaxf(m, other.x);
+        w_mine = n_mine > 0 ? merge_weight(m, m_all) : 0.f;
+        w_other = n_other > 0 ? merge_weight(other.x, m_all) : 0.f;
+        l = w_mine * l + w_other * other.y;
+        m = m_all;
+      }
+      if (n_mine > 0) ok = TREE_WAIT(O_DONE + sx, done[sx], 41);
+      if (ok && n_other > 0) ok = TREE_WAIT(O_DONE + (sx ^ 1), done[sx ^ 1], 42);
+      if (!ok) break;
+      done[sx] += n_mine > 0;
+      done[sx ^ 1] += n_other > 0;
+      ptx::tc_fence_after();
+      const int col = PAIR ? 0 : sx * COLS;               // !PAIR: set s takes half s of the columns, of both streams
+      auto chunk = [&](int c, float (&o)[32]) {           // sums of 32 columns, called by whole warps
+        uint32_t y[32];
+        if constexpr (PAIR) {
+          ptx::tmem_ld32(o_addr + c, y);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(y[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if ((x == sx ? n_mine : n_other) > 0) {
+              const float w = x == sx ? w_mine : w_other;
+              ptx::tmem_ld32(lane_addr + 256 + x * 128 + col + c, y);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] += w * __uint_as_float(y[e]);
+            }
+          }
+        }
+      };
+      bool finite = true;
+      if (busy) {
+        TreeRowOut dst = {t.o + ((int64_t(pc.b) * t.n + token) * t.H + head) * HEAD_DIM, nullptr};
+        if (pc.count != pc.of) {
+          float* const part = t.scratch + (int64_t(blockIdx.x) * 2 + (pc.first == 0 ? 1 : 0)) * UMMA_PARTIAL<PAIR>;
+          const int at = r - pc.rg * ROWS;
+          dst.part = part + int64_t(at) * HEAD_DIM;
+          if (valid && col == 0) reinterpret_cast<float2*>(part + int64_t(ROWS) * HEAD_DIM)[at] = make_float2(m, l);
+        }
+        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+#pragma unroll 1
+        for (int c = 0; c < COLS; c += 32) {
+          float o[32];
+          chunk(c, o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) finite = finite && fabsf(o[e]) < CUDART_INF_F;
+          if (!valid) continue;
+          if (dst.part != nullptr) {
+            float4* const d = reinterpret_cast<float4*>(dst.part + col + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          } else {
+            uint4* const d = reinterpret_cast<uint4*>(dst.out + col + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              d[e] = make_uint4(ptx::pack_bf16(o[8 * e] * inv, o[8 * e + 1] * inv), ptx::pack_bf16(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                ptx::pack_bf16(o[8 * e + 4] * inv, o[8 * e + 5] * inv), ptx::pack_bf16(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+          }
+        }
+        if (valid && !finite) tree_exact_row<COLS>(t, pc, own, token, head, col, m, l, dst);       // over what was just written
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_at(bar(O_FREE + sx));              // the next unit's first PV may overwrite O
+      ++unit;
+    }
+  } else if (warp < 12) {
+    // ================================ requests of the tiles ========================================
+    ptx::setmaxnreg_dec<UMMA_LOAD_REGS>();
+    const int lt = tid - 256;                             // 0 .. 127; in copies: row lt >> 4 of every 8, piece lt & 15
+    auto request = [&](uint32_t req, int operand, const TreePiece& x, int tile) {
+      const uint32_t slot = req % RING, dst = ring_smem + slot * TILE_BYTES;
+      if (!(ok = TREE_WAIT(FREE + slot, req / RING - 1, 21 + operand))) return;
+      const int key0 = tile * TILE_N;
+      if (p.use_tma && (key0 + TILE_N <= x.n_keys || x.n_keys == t.S)) {  // rows past the cache's end come as zeros
+        if (lt == 0) {
+          ptx::mbar_expect_tx_at(bar(FULL + slot), TILE_BYTES);
+          ptx::tma_load_5d_at(dst, &p.maps[operand], bar(FULL + slot), 0, key0, 0, x.hk, x.b);
+          ptx::tma_load_5d_at(dst + HALF_BYTES, &p.maps[operand], bar(FULL + slot), 64, key0, 0, x.hk, x.b);
+        } else {
+          ptx::mbar_arrive_at(bar(FULL + slot));
+        }
+        return;
+      }
+      const TensorView& st = operand ? t.vs : t.ks;
+      const __nv_bfloat16* const src = (operand ? t.v : t.k) + x.b * st.sb + x.hk * st.sh + (lt & 15) * 8;
+#pragma unroll 4
+      for (int c = 0; c < TILE_N / 8; ++c) {
+        const int row = c * 8 + (lt >> 4);
+        const bool there = key0 + row < x.n_keys;
+        ptx::cp_async_16(dst + tile_offset(row, lt & 15), there ? src + (key0 + row) * st.ss : src, there ? 16u : 0u);
+      }
+      ptx::cp_async_mbar_arrive_noinc(&bars[FULL + slot]);
+    };
+    uint32_t j = 0, unit = 0;
+    TreePiece before;                                     // of the tile whose V is requested next
+    int v_tile = -1;
+    if (lt < 2) ptx::prefetch_tensormap(&p.maps[lt]);
+    while (ok && walk.piece(t, pc)) {
+      for (int i = 0; i < pc.count && ok; ++i, ++j) {
+        request(k_request(j), 0, pc, pc.first + i);
+        if (ok && i == 0) {
+          ok = TREE_WAIT(Q_FREE, unit - 1, 23);
+          if (!ok) break;
+#pragma unroll 4
+          for (int c = 0; c < ROWS / 8; ++c) {
+            const int at = c * 8 + (lt >> 4), r = pc.rg * ROWS + at, token = r / rep;
+            const __nv_bfloat16* const src = t.q + pc.b * t.q_sb + (pc.hk * rep + r - token * rep) * t.q_sh + token * t.q_sn + (lt & 15) * 8;
+            ptx::cp_async_16(q_smem + (at >> 7) * TILE_BYTES + tile_offset(at & 127, lt & 15), r < all_rows ? src : t.q, r < all_rows ? 16u : 0u);
+          }
+          ptx::cp_async_mbar_arrive_noinc(&bars[Q_FULL]);
+        }
+        if (ok && v_tile >= 0) request(v_request(j - 1), 1, before, v_tile);
+        before = pc;
+        v_tile = pc.first + i;
+      }
+      ++unit;
+    }
+    if (ok && v_tile >= 0) request(v_request(j - 1), 1, before, v_tile);
+    ptx::cp_async_commit();
+    ptx::cp_async_wait<0>();
+  } else {
+    ptx::setmaxnreg_dec<UMMA_ISSUE_REGS>();
+    // ================================ MMA issue ====================================================
+    const uint64_t q_desc = tile_desc_kmajor(q_smem), k_desc = tile_desc_kmajor(ring_smem), v_desc = tile_desc_mnmajor(ring_smem);
+    constexpr uint64_t STEP = TILE_BYTES >> 4;             // descriptor distance between buffers
+    uint32_t j = 0, unit = 0, kt[2] = {0, 0};              // tiles of the CTA before this unit, units, tiles per stream
+    // Scores of tile j for stream sx; `last` reads K last, `final` the unit's queries.
+    auto qk = [&](uint32_t tile, int sx, bool first_of_unit, bool last, bool final) {
+      const uint32_t req = k_request(tile), slot = req % RING;
+      ok = (!first_of_unit || TREE_WAIT(Q_FULL, unit, 31)) && TREE_WAIT(FULL + slot, req / RING, 32);
+      if (PAIR && ok) ok = TREE_WAIT(S_TAKEN + (sx ^ 1), sx ? tile : tile - 1, 33);      // the other set has copied its scores out
+      if (!ok) return;
+      ptx::tc_fence_after();
+      if (ptx::elect_one()) {
+        ptx::fence_proxy_async_smem();                    // tiles may have come by plain copies
+        issue_qk_loop(q_desc + (PAIR ? sx : 0) * STEP, k_desc + slot * STEP, tmem + (PAIR ? 0 : sx * 128));
+        ptx::mma_commit_at(bar(S_FULL + sx));
+        if (last) ptx::mma_commit_at(bar(FREE + slot));
+        if (final) ptx::mma_commit_at(bar(Q_FREE));
+      }
+      __syncwarp();
+    };
+    auto pv = [&](uint32_t tile, int sx, bool first_of_stream, bool last, bool final) {
+      const uint32_t req = v_request(tile), slot = req % RING;
+      ok = TREE_WAIT(FULL + slot, req / RING, 40);
+      if (ok && first_of_stream) ok = TREE_WAIT(O_FREE + sx, unit - 1, 37) && (PAIR || TREE_WAIT(O_FREE + (sx ^ 1), unit - 1, 38));
+      if (ok) ok = TREE_WAIT(P_FULL + sx, kt[sx], 35);
+      if (!ok) return;
+      ++kt[sx];
+      ptx::tc_fence_after();
+      if (ptx::elect_one()) {
+        ptx::fence_proxy_async_smem();
+        const uint32_t p_cols = PAIR ? tmem + 128 + sx * 64 : tmem + sx * 128;
+        issue_pv_loop(p_cols, v_desc + slot * STEP, tmem + 256 + sx * 128, first_of_stream ? 0 : 1);
+        if (!PAIR) issue_pv_loop(p_cols + 64, v_desc + slot * STEP, tmem + 256 + sx * 128, 1);
+        if (PAIR) ptx::mma_commit_at(bar(PV_DONE + sx));
+        if (last) ptx::mma_commit_at(bar(FREE + slot));
+        if (final) ptx::mma_commit_at(bar(O_DONE + sx));
+      }
+      __syncwarp();
+    };
+    if (warp == 12 || (PAIR && warp == 13)) {
+      while (ok && walk.piece(t, pc)) {
+        const int count = pc.count;
+        if (PAIR) {
+#pragma unroll 1
+          for (int i = 0; i < count && ok; ++i)
+#pragma unroll 1
+            for (int sx = 0; sx < 2 && ok; ++sx) {
+              if (warp == 12) qk(j + i, sx, i == 0 && sx == 0, sx == 1, sx == 1 && i == count - 1);
+              else pv(j + i, sx, i == 0, sx == 1, i == count - 1);
+            }
+        } else {
+#pragma unroll 1
+          for (int i = -2; i < count && ok; ++i) {         // PV of tile i, then QK^T of tile i + 2 into the scores it has read
+            if (i >= 0) pv(j + i, i & 1, i < 2, true, i + 2 >= count);
+            if (ok && i + 2 < count) qk(j + i + 2, i & 1, i == -2, true, i + 3 == count);
+          }
+        }
+        j += count;
+        ++unit;
+      }
+      if (!ok) {                                           // let MMAs in flight finish before TMEM is freed
+        const int drain = DRAIN + (warp - 12);
+        if (ptx::elect_one()) ptx::mma_commit_at(bar(drain));
+        __syncwarp();
+        int dummy = 0;
+        ptx::mbar_wait(&bars[drain], 0, &dummy, 100);
+      }
+    }
+  }
+#undef TREE_WAIT
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+  if (tid == 0 && abort_flag != 0) {
+    ptx::drain_copies(bars, FREE);                         // tiles that were requested before the give-up
+    atomicCAS(p.status, 0, STATUS_WAIT_BASE + abort_flag);
+  }
+}
+
+// Joins the partial results of units that several CTAs had a part of. A warp per row: lane = 4 dims.
+constexpr int UMMA_MERGE_ROWS = 8;
+template <bool PAIR>
+__global__ void __launch_bounds__(32 * UMMA_MERGE_ROWS) tree_umma_merge_kernel(const __grid_constant__ TreeUmmaParams p, int grid) {
+  const TreeParams& t = p.t;
+  const int lane = threadIdx.x & 31, rep = t.H / t.Hkv;
+  const int64_t out_row = int64_t(blockIdx.x) * UMMA_MERGE_ROWS + (threadIdx.x >> 5);      // (b, hk, row of the KV head)
+  const int all_rows = t.n * rep;
+  const int hk_b = int(out_row / all_rows), row = int(out_row - int64_t(hk_b) * all_rows);
+  const int b = hk_b / t.Hkv, hk = hk_b - b * t.Hkv;
+  if (b >= p.B) return;
+  const int rg = row / UMMA_ROWS<PAIR>, at = row - rg * UMMA_ROWS<PAIR>;
+  int64_t total = 0, start = 0;                           // tiles of all units, and before this one
+  const int units = t.Hkv * t.row_groups;
+  for (int s = lane; s < p.B; s += 32) {
+    const int64_t n = int64_t(tree_tiles(t, s)) * units;
+    total += n;
+    start += s < b ? n : 0;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, d);
+    start += __shfl_xor_sync(0xffffffffu, start, d);
+  }
+  int64_t per = (total + grid - 1) / grid;
+  per = per < UMMA_MIN_TILES ? UMMA_MIN_TILES : per;
+  const int tiles = tree_tiles(t, b);
+  start += int64_t(hk * t.row_groups + rg) * tiles;
+  const int c0 = int(start / per), c1 = int((start + tiles - 1) / per);
+  if (c0 == c1) return;                                   // one CTA held the unit and wrote its rows
+  auto slot = [&](int c) { return t.scratch + (int64_t(c) * 2 + (c == c0 ? 1 : 0)) * UMMA_PARTIAL<PAIR>; };
+  auto ml = [&](int c) { return reinterpret_cast<const float2*>(slot(c) + int64_t(UMMA_ROWS<PAIR>) * HEAD_DIM)[at]; };
+  float m_all = -CUDART_INF_F;
+  for (int c = c0 + lane; c <= c1; c += 32) m_all = fmaxf(m_all, ml(c).x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, d));
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l_all = 0.f;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const float2 x = ml(c);
+    const float f = merge_weight(x.x, m_all);
+    const float4 o = reinterpret_cast<const float4*>(slot(c) + int64_t(at) * HEAD_DIM)[lane];
+    acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
+    l_all += f * x.y;
+  }
+  const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+  const int token = row / rep, head = hk * rep + row - token * rep;
+  uint2* const dst = reinterpret_cast<uint2*>(t.o + ((int64_t(b) * t.n + token) * t.H + head) * HEAD_DIM) + lane;
+  *dst = make_uint2(ptx::pack_bf16(acc.x * inv, acc.y * inv), ptx::pack_bf16(acc.z * inv, acc.w * inv));
+}
+
+}  // namespace intra
