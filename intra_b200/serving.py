@@ -26,6 +26,7 @@ from .interface import _byte_span, _c_strides, _raise, _raw_stream
 
 MAX_TOKENS = 64             # nodes of a tree: ancestors are kept as 64 bits
 _PROB_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_SCALE = 128 ** -0.5
 
 
 def _no_grad(*tensors):
@@ -40,53 +41,71 @@ def _rows_usable(x):
 
 
 def _attention_inputs(q, k, v):
-    """Checks of q (B, H, n, 128) and a cache k, v (B, Hkv, S, 128); tensors whose rows are not 16-byte aligned are copied."""
-    for x in (q, k, v):
-        if not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() != 4 or x.shape[-1] != 128:
-            raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
-    _no_grad(q, k, v)
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"incompatible shapes q={tuple(q.shape)} k={tuple(k.shape)} v={tuple(v.shape)}")
-    if k.device != q.device or v.device != q.device:
+    """q (B, H, n, 128) and a cache k, v (B, Hkv, S, 128) as the kernels can read them (tensors whose rows are not 16-byte
+    aligned are copied), their strides {batch, token, head} for the C ABI, and their device. Raises for others."""
+    bf16, dev, qn, kn = torch.bfloat16, q.device, q.shape, k.shape
+    if not (q.is_cuda and q.dtype is bf16 and k.dtype is bf16 and v.dtype is bf16 and len(qn) == 4 and len(kn) == 4
+            and qn[3] == 128 and kn[3] == 128):
+        raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        raise RuntimeError("INTRA kernels are forward-only; call them under torch.no_grad()")
+    if kn != v.shape or kn[0] != qn[0] or kn[1] == 0 or qn[1] == 0 or qn[1] % kn[1]:
+        raise ValueError(f"incompatible shapes q={tuple(qn)} k={tuple(kn)} v={tuple(v.shape)}")
+    if k.device != dev or v.device != dev:
         raise ValueError("q, k, v must be on the same device")
-    return [x if _rows_usable(x) else x.contiguous() for x in (q, k, v)]
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if (qs[3] != 1 or ks[3] != 1 or vs[3] != 1 or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15
+            or (qs[0] | qs[1] | qs[2] | ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & 7):
+        q, k, v = (x if _rows_usable(x) else x.contiguous() for x in (q, k, v))
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+    return (q, k, v, _c_strides(qs[0], qs[2], qs[1]), _c_strides(ks[0], ks[2], ks[1]), _c_strides(vs[0], vs[2], vs[1]), dev)
 
 
-def _integers(x, name, shapes, device):
-    """An int32 tensor of one of `shapes` on `device`, unit stride in the last dimension."""
+def _integers(x, name, shape, device, shared=None):
+    """An int32 tensor of `shape`, or of shape `shared` that all sequences share, unit stride in the last dimension, and its
+    address and batch stride."""
     if x is None:
-        return None
-    if x.dtype != torch.int32 or tuple(x.shape) not in shapes or x.device != device:
-        raise ValueError(f"{name} must be int32 of shape {' or '.join(map(str, shapes))} on {device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+        return None, None, 0
+    n = x.shape
+    if x.dtype is not torch.int32 or (n != shape and n != shared) or x.device != device:
+        raise ValueError(f"{name} must be int32 of shape {shape}{f' or {shared}' if shared else ''} on {device}, "
+                         f"got {x.dtype} {tuple(n)} on {x.device}")
+    if x.stride(-1) != 1:
+        x = x.contiguous()
+    return x, x.data_ptr(), x.stride(0) if len(n) == 2 else 0
 
 
 def _mask(mask, B, n, S, device):
-    """(tensor, strides {batch, token, key}) of a boolean mask (B or 1, 1, n or 1, >= S)."""
-    if (mask.dtype != torch.bool or mask.dim() != 4 or mask.device != device or mask.shape[0] not in (1, B)
-            or mask.shape[2] not in (1, n) or mask.shape[3] < S or (mask.shape[1] != 1 and mask.stride(1) != 0)):
+    """Strides {batch, token, key} of a boolean mask (B or 1, 1, n or 1, >= S)."""
+    m = mask.shape
+    if (mask.dtype is not torch.bool or len(m) != 4 or mask.device != device or (m[0] != B and m[0] != 1)
+            or (m[2] != n and m[2] != 1) or m[3] < S or (m[1] != 1 and mask.stride(1) != 0)):
         raise ValueError(f"mask must be bool (batch or 1, 1, tokens or 1, at least {S}) on {device}, the same for every head")
     st = mask.stride()
-    return _c_strides(st[0] if mask.shape[0] > 1 else 0, st[2] if mask.shape[2] > 1 else 0, st[3])
-
-
-def _bsh(x):
-    """Strides {batch, token, head} of a (B, heads, tokens, 128) tensor."""
-    s = x.stride()
-    return _c_strides(s[0], s[2], s[1])
+    return st[0] if m[0] > 1 else 0, st[2] if m[2] > 1 else 0, st[3]
 
 
 def _ptr(x):
     return None if x is None else x.data_ptr()
 
 
-def _with_scratch(call, device):
+# Bytes of scratch a call wants, by its sizes: asking the library costs as much as a third of a short call.
+_SCRATCH = {}
+_SCRATCH_MAX = 1024
+
+
+def _with_scratch(key, call, device):
     """Runs call(scratch pointer, its bytes, where the bytes wanted are stored) with a buffer as large as it asks for."""
+    nbytes = _SCRATCH.get(key, 0)
     need = ctypes.c_int64(0)
-    rc = call(None, 0, need)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    rc = call(_ptr(scratch), nbytes, need)
     if rc == _loader.NEED_SCRATCH:
-        scratch = torch.empty(need.value, dtype=torch.uint8, device=device)
-        rc = call(scratch.data_ptr(), need.value, need)
+        if len(_SCRATCH) >= _SCRATCH_MAX:
+            _SCRATCH.clear()
+        nbytes = _SCRATCH[key] = need.value
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        rc = call(scratch.data_ptr(), nbytes, need)
     if rc != 0:
         _raise(rc)
 
@@ -97,35 +116,33 @@ def tree_attn(q, k, v, parents=None, lengths=None, mask=None, softmax_scale=None
     q (B, H, n, 128), 1 <= n <= 64; k, v (B, Hkv, S, 128), H a multiple of Hkv. The tokens' own keys are rows lengths[b] ..
     lengths[b] + n - 1; `lengths` (B,) int32 on the GPU, None: the cache's last n rows. (Values that leave the tokens no room
     in the cache are brought into 0 .. S - n; they cannot be refused without a synchronisation.) Token i sees all keys
-    before those, its ancestors and itself: parents (n,) or (B, n) int32, parents[i] the earlier token that token i follows, negative for
-    none; None: token i follows token i - 1. `mask`, bool (B or 1, 1, n or 1, >= S), hides further keys. Returns (B, n, H, 128)."""
+    before those, its ancestors and itself: parents (n,) or (B, n) int32, parents[i] the earlier token that token i follows,
+    negative for none; None: token i follows token i - 1. `mask`, bool (B or 1, 1, n or 1, >= S), hides further keys.
+    Returns (B, n, H, 128); a token that sees nothing gets zeros."""
     return _tree(q, k, v, parents, lengths, mask, softmax_scale, False)
 
 
 def _tree(q, k, v, parents, lengths, mask, softmax_scale, all_own):
     """tree_attn; with `all_own` the tokens see all their own keys, so that the mask decides alone."""
-    q, k, v = _attention_inputs(q, k, v)
+    q, k, v, qs, ks, vs, dev = _attention_inputs(q, k, v)
     B, H, n, D = q.shape
-    Hkv, S = k.shape[1:3]
+    _, Hkv, S, _ = k.shape
     if not 1 <= n <= MAX_TOKENS or n > S:
         raise ValueError(f"expected 1 to {MAX_TOKENS} tokens whose keys are in the cache, got {n} and a cache of {S} rows")
-    dev = q.device
-    parents = _integers(parents, "parents", ((n,), (B, n)), dev)
-    lengths = _integers(lengths, "lengths", ((B,),), dev)
-    m_strides = None if mask is None else _mask(mask, B, n, S, dev)
-    out = torch.empty((B, n, H, D), dtype=q.dtype, device=dev)
+    parents, up, up_stride = _integers(parents, "parents", (B, n), dev, (n,))
+    lengths, used, _ = _integers(lengths, "lengths", (B,), dev)
+    ms = None if mask is None else _c_strides(*_mask(mask, B, n, S, dev))
+    out = q.new_empty((B, n, H, D))
     if B == 0:
         return out
-    scale = 0.08838834764831845 if softmax_scale is None else float(softmax_scale)
-    up = parents.stride(0) if parents is not None and parents.dim() == 2 else 0
-    qs, ks, vs, stream = _bsh(q), _bsh(k), _bsh(v), _raw_stream(dev.index)
+    index, scale = dev.index, _SCALE if softmax_scale is None else float(softmax_scale)
+    stream = _raw_stream(index)
 
     def call(scratch, nbytes, need):
-        return lib.intra_b200_tree_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(parents), _ptr(lengths), _ptr(mask),
-                                        out.data_ptr(), scratch, nbytes, need, B, S, H, Hkv, n, qs, ks, vs, up, all_own, m_strides, scale,
-                                        dev.index, stream)
+        return lib.intra_b200_tree_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), up, used, _ptr(mask), out.data_ptr(), scratch,
+                                        nbytes, need, B, S, H, Hkv, n, qs, ks, vs, up_stride, all_own, ms, scale, index, stream)
 
-    _with_scratch(call, dev)
+    _with_scratch((n, B, S, H, Hkv, ms is None, index), call, dev)
     return out
 
 
@@ -135,45 +152,47 @@ def decode_attn_accumulate(q, k, v, weights, lengths=None, mask=None, softmax_sc
     sees rows 0 .. lengths[b], its own being the last of them; `lengths` (B,) int32, None: all S. (Values outside 0 ..
     S - 1 are brought into that range.) `mask`, bool (B or 1, 1, 1, >= S), hides further keys. Weights of keys the
     token does not see stay as they are. Returns (B, 1, H, 128)."""
-    q, k, v = _attention_inputs(q, k, v)
+    q, k, v, qs, ks, vs, dev = _attention_inputs(q, k, v)
     B, H, n, D = q.shape
-    Hkv, S = k.shape[1:3]
+    _, Hkv, S, _ = k.shape
     if n != 1 or S == 0:
         raise ValueError(f"expected one token per sequence and a cache that holds it, got {n} and {S} rows")
-    dev = q.device
-    if (not weights.is_cuda or weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[:2] != k.shape[:2]
-            or weights.shape[2] < S or weights.device != dev):
+    wn, ws = weights.shape, weights.stride()
+    if weights.dtype is not torch.float32 or len(wn) != 3 or wn[0] != B or wn[1] != Hkv or wn[2] < S or weights.device != dev:
         raise ValueError(f"weights must be float32 (batch, KV heads, at least {S}) on {dev}")
     _no_grad(weights)
-    _distinct_rows(weights, "weights")
-    lengths = _integers(lengths, "lengths", ((B,),), dev)
-    m_strides = None if mask is None else _mask(mask, B, 1, S, dev)
-    out = torch.empty((B, 1, H, D), dtype=q.dtype, device=dev)
+    if not (ws[2] == 1 and ws[1] >= wn[2] and ws[0] >= ws[1] * Hkv):     # else look closer
+        _distinct_rows(weights, "weights")
+    lengths, used, _ = _integers(lengths, "lengths", (B,), dev)
+    ms = None
+    if mask is not None:
+        ms = _mask(mask, B, 1, S, dev)
+        ms = _c_strides(ms[0], ms[2], 0)
+    out = q.new_empty((B, 1, H, D))
     if B == 0:
         return out
-    if mask is not None:
-        m_strides = _c_strides(m_strides[0], m_strides[2], 0)
-    scale = 0.08838834764831845 if softmax_scale is None else float(softmax_scale)
-    qs, ks, vs, stream, ws = _bsh(q), _bsh(k), _bsh(v), _raw_stream(dev.index), weights.stride()
+    index, scale = dev.index, _SCALE if softmax_scale is None else float(softmax_scale)
+    stream = _raw_stream(index)
 
     def call(scratch, nbytes, need):
-        return lib.intra_b200_decode_accumulate(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), _ptr(lengths), out.data_ptr(),
-                                                weights.data_ptr(), scratch, nbytes, need, B, S, H, Hkv, qs, ks, vs, m_strides,
-                                                ws[0], ws[1], scale, dev.index, stream)
+        return lib.intra_b200_decode_accumulate(q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), used, out.data_ptr(),
+                                                weights.data_ptr(), scratch, nbytes, need, B, S, H, Hkv, qs, ks, vs, ms,
+                                                ws[0], ws[1], scale, index, stream)
 
-    _with_scratch(call, dev)
+    _with_scratch((0, B, S, H, Hkv, index), call, dev)
     return out
 
 
 def _distinct_rows(x, name):
     """A tensor that is written needs unit stride in its last dimension and rows that do not share memory."""
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    shape, strides = x.shape, x.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name} needs unit stride in the last dimension")
-    reach = x.shape[-1]
-    for size, stride in sorted(((n, s) for n, s in zip(x.shape[:-1], x.stride()[:-1]) if n > 1), key=lambda d: d[1]):
+    reach = shape[-1]
+    for stride, size in sorted((s, n) for n, s in zip(shape[:-1], strides[:-1]) if n > 1):
         if stride < reach:
             raise ValueError(f"{name} has rows that share memory")
-        reach = stride * (size - 1) + reach
+        reach += stride * (size - 1)
 
 
 def verify_drafts(tokens, target_probs, draft_probs, uniform, parents=None):
@@ -181,46 +200,58 @@ def verify_drafts(tokens, target_probs, draft_probs, uniform, parents=None):
 
     tokens (B, n) int64 or int32, 1 <= n <= 64: node 0 is the token sampled last, nodes 1 .. n - 1 are drafts. target_probs
     (B, n, V): the target's distribution behind each node; draft_probs (B, n or n - 1, V), of the same type (float32,
-    bfloat16 or float16): the distribution the children of each node were drawn from, None for drafts that were not drawn (each counts
-    as certain). uniform (B, n) float32 in [0, 1): entry i decides node i, entry 0 draws the last token. parents (n,) or
-    (B, n) int32: the node each follows, an earlier one; None: a chain.
+    bfloat16 or float16): the distribution the children of each node were drawn from, None for drafts that were not drawn
+    (each counts as certain). uniform (B, n) float32 in [0, 1): entry i decides node i, entry 0 draws the last token. parents
+    (n,) or (B, n) int32: the node each follows, an earlier one; None: a chain.
 
-    From node 0 on, the children x of the current node are tried in index order: accepted iff uniform * q(x) * Z < R(x), with R the
-    target's distribution and Z = 1 at first; a rejection replaces R by max(R / Z - q, 0) and Z by its sum (unless that is
+    From node 0 on, the children x of the current node are tried in index order: accepted iff uniform * q(x) * Z < R(x), with R
+    the target's distribution and Z = 1 at first; a rejection replaces R by max(R - Z q, 0) and Z by its sum (unless that is
     zero). When none is left the last token is drawn from R: the smallest t with R(0) + .. + R(t) > uniform * sum R. Sums
     and comparisons are in 64 bits.
 
     Returns accepted (B,) int32, the number m of accepted drafts; path (B, n) int32, the nodes from 0 on, then -1; and tokens
     (B, n) int64: the m accepted ones, the drawn one, then -1. Drafts outside the vocabulary are rejected."""
-    if target_probs.dim() != 3 or target_probs.dtype not in _PROB_TYPES or not target_probs.is_cuda:
+    pn, kind = target_probs.shape, _PROB_TYPES.get(target_probs.dtype)
+    if len(pn) != 3 or kind is None or not target_probs.is_cuda:
         raise ValueError("target_probs must be a CUDA float32, bfloat16 or float16 tensor (batch, nodes, vocabulary)")
-    B, n, V = target_probs.shape
+    B, n, V = pn
     dev = target_probs.device
     _no_grad(target_probs, draft_probs, uniform)
     if not 1 <= n <= MAX_TOKENS or V == 0:
         raise ValueError(f"expected 1 to {MAX_TOKENS} nodes and a vocabulary, got {n} and {V}")
-    if tokens.dtype not in (torch.int64, torch.int32) or tokens.shape != (B, n) or tokens.device != dev:
+    wide = tokens.dtype is torch.int64
+    if not (wide or tokens.dtype is torch.int32) or tokens.shape != (B, n) or tokens.device != dev:
         raise ValueError(f"tokens must be int64 or int32 ({B}, {n}) on {dev}")
-    if uniform.dtype != torch.float32 or uniform.shape != (B, n) or uniform.device != dev:
+    if uniform.dtype is not torch.float32 or uniform.shape != (B, n) or uniform.device != dev:
         raise ValueError(f"uniform must be float32 ({B}, {n}) on {dev}")
-    if draft_probs is not None and (draft_probs.dtype != target_probs.dtype or draft_probs.dim() != 3 or draft_probs.shape[0] != B
-                                    or draft_probs.shape[1] not in (n - 1, n) or draft_probs.shape[2] != V or draft_probs.device != dev):
-        raise ValueError(f"draft_probs must be {target_probs.dtype} ({B}, {n - 1} or {n}, {V}) on {dev}")
-    parents = _integers(parents, "parents", ((n,), (B, n)), dev)
+    if draft_probs is not None:
+        dn = draft_probs.shape
+        if (draft_probs.dtype is not target_probs.dtype or len(dn) != 3 or dn[0] != B or (dn[1] != n and dn[1] != n - 1) or dn[2] != V
+                or draft_probs.device != dev):
+            raise ValueError(f"draft_probs must be {target_probs.dtype} ({B}, {n - 1} or {n}, {V}) on {dev}")
+        if dn[1] == 0:                                       # no drafts
+            draft_probs = None
+    parents, up, up_stride = _integers(parents, "parents", (B, n), dev, (n,))
     accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    path = torch.empty((B, n), dtype=torch.int32, device=dev)
+    path = accepted.new_empty((B, n))
     out = torch.empty((B, n), dtype=torch.int64, device=dev)
     if B == 0:
         return accepted, path, out
-    target_probs, tokens, uniform = (x if x.stride(-1) == 1 else x.contiguous() for x in (target_probs, tokens, uniform))
-    if draft_probs is not None and (draft_probs.numel() == 0 or draft_probs.stride(-1) != 1):
-        draft_probs = None if draft_probs.numel() == 0 else draft_probs.contiguous()
-    up = parents.stride(0) if parents is not None and parents.dim() == 2 else 0
-    rc = lib.intra_b200_verify_drafts(tokens.data_ptr(), tokens.dtype == torch.int64, target_probs.data_ptr(), _ptr(draft_probs),
-                                      _PROB_TYPES[target_probs.dtype], uniform.data_ptr(), _ptr(parents), accepted.data_ptr(),
-                                      path.data_ptr(), out.data_ptr(), B, n, V, _c_strides(*target_probs.stride()),
-                                      None if draft_probs is None else _c_strides(*draft_probs.stride()), tokens.stride(0),
-                                      uniform.stride(0), up, dev.index, _raw_stream(dev.index))
+    if target_probs.stride(2) != 1:
+        target_probs = target_probs.contiguous()
+    if tokens.stride(1) != 1:
+        tokens = tokens.contiguous()
+    if uniform.stride(1) != 1:
+        uniform = uniform.contiguous()
+    ds = None
+    if draft_probs is not None:
+        if draft_probs.stride(2) != 1:
+            draft_probs = draft_probs.contiguous()
+        ds = _c_strides(*draft_probs.stride())
+    rc = lib.intra_b200_verify_drafts(tokens.data_ptr(), wide, target_probs.data_ptr(), _ptr(draft_probs), kind, uniform.data_ptr(),
+                                      up, accepted.data_ptr(), path.data_ptr(), out.data_ptr(), B, n, V,
+                                      _c_strides(*target_probs.stride()), ds, tokens.stride(0), uniform.stride(0), up_stride,
+                                      dev.index, _raw_stream(dev.index))
     if rc != 0:
         _raise(rc)
     return accepted, path, out
@@ -260,41 +291,50 @@ def _overlapping(tensors):
 
 def keep_drafts(caches, lengths, path):
     """Moves the cache rows of accepted tokens together, in place: in each of `caches` (a tensor or a sequence of them, K and V of
-    all layers, (B, Hkv, S, 128) bfloat16, all of one shape) row lengths[b] + path[b, i] becomes row lengths[b] + i, for every i with path[b, i] >= 0. lengths (B,) int32: rows before the
-    tokens' own, as in `tree_attn`; path (B, n) int32, n <= 64, as `verify_drafts` returns it. Entries outside 0 .. n - 1 move
-    nothing, and neither does a sequence whose lengths[b] is not in 0 .. S - n. Other rows stay as they are."""
+    all layers, (B, Hkv, S, 128) bfloat16, all of one shape) row lengths[b] + path[b, i] becomes row lengths[b] + i, for every i
+    with path[b, i] >= 0. lengths (B,) int32: rows before the tokens' own, as in `tree_attn`; path (B, n) int32, n <= 64, as
+    `verify_drafts` returns it. Entries outside 0 .. n - 1 move nothing, and neither does a sequence whose lengths[b] is not in
+    0 .. S - n. Other rows stay as they are. The caches must not share memory."""
     caches = [caches] if isinstance(caches, torch.Tensor) else list(caches)
     if not caches:
         return
-    first = caches[0]
-    dev = first.device
-    for x in caches:
-        if not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() != 4 or x.shape[-1] != 128:
-            raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
-        if x.shape != first.shape or x.device != dev:
-            raise ValueError("caches must agree in shape and device")
-        if not _rows_usable(x):
-            raise ValueError("caches need unit stride in the last dimension and 16-byte aligned rows")
-        _distinct_rows(x, "a cache")
-    _no_grad(*caches)
-    B, Hkv, S, _ = first.shape
-    if path.dim() != 2 or not 1 <= path.shape[1] <= min(MAX_TOKENS, S):
+    first, count = caches[0], len(caches)
+    dev, shape = first.device, first.shape
+    # what all of them have in common is looked at once
+    if not first.is_cuda or {x.dtype for x in caches} != {torch.bfloat16} or len(shape) != 4 or shape[3] != 128:
+        raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
+    if any([x.shape != shape for x in caches]) or {x.get_device() for x in caches} != {dev.index}:
+        raise ValueError("caches must agree in shape and device")
+    if torch.is_grad_enabled() and any([x.requires_grad for x in caches]):
+        raise RuntimeError("INTRA kernels are forward-only; call them under torch.no_grad()")
+    pointers, strides = [x.data_ptr() for x in caches], [x.stride() for x in caches]
+    layouts = {}
+    for s, x in zip(strides, caches):
+        if s not in layouts:
+            if not _rows_usable(x):
+                raise ValueError("caches need unit stride in the last dimension and 16-byte aligned rows")
+            _distinct_rows(x, "a cache")
+            layouts[s] = [s[d] if shape[d] > 1 else 8 for d in (0, 2, 1)]
+    if any([p & 15 for p in pointers]):
+        raise ValueError("caches need unit stride in the last dimension and 16-byte aligned rows")
+    B, Hkv, S, _ = shape
+    if len(path.shape) != 2 or not 1 <= path.shape[1] <= min(MAX_TOKENS, S):
         raise ValueError(f"path must be (batch, n) with n from 1 to {min(MAX_TOKENS, S)}")
-    path = _integers(path, "path", ((B, path.shape[1]),), dev)
-    lengths = _integers(lengths, "lengths", ((B,),), dev)
+    n = path.shape[1]
+    path, nodes, path_stride = _integers(path, "path", (B, n), dev)
+    lengths, used, _ = _integers(lengths, "lengths", (B,), dev)
     if lengths is None:
         raise ValueError("lengths is needed")
-    if len(caches) > 1 and _overlapping(caches):
-        raise ValueError("caches must not overlap")
     if B == 0 or Hkv == 0:
         return
-    pointers = (ctypes.c_void_p * len(caches))(*[x.data_ptr() for x in caches])
-    strides = (ctypes.c_int64 * (3 * len(caches)))()
-    for i, x in enumerate(caches):
-        s = x.stride()
-        strides[3 * i:3 * i + 3] = [s[d] if x.shape[d] > 1 else 8 for d in (0, 2, 1)]
-    rc = lib.intra_b200_keep_drafts(pointers, strides, len(caches), lengths.data_ptr(), path.data_ptr(), path.stride(0), B, S, Hkv,
-                                    path.shape[1], dev.index, _raw_stream(dev.index))
+    if count > 1:
+        span = _byte_span(first)[1] - pointers[0]
+        order = sorted(pointers)
+        if (len(layouts) > 1 or any([b - a < span for a, b in zip(order, order[1:])])) and _overlapping(caches):
+            raise ValueError("caches must not share memory")
+    c_strides = (ctypes.c_int64 * (3 * count))(*[st for s in strides for st in layouts[s]])
+    rc = lib.intra_b200_keep_drafts((ctypes.c_void_p * count)(*pointers), c_strides, count, used, nodes, path_stride, B, S, Hkv, n,
+                                    dev.index, _raw_stream(dev.index))
     if rc != 0:
         _raise(rc)
 
@@ -308,33 +348,33 @@ def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
     Returns (k, v, weights, kept): the kept rows, their weights and their old places (B, Hkv, keep) int32. Behind a sequence's
     last row come zeros, and -1 in `kept`; lengths are min(lengths, keep) from then on. `out` = (k, v, weights) writes into the
     caller's tensors of at least `keep` rows, whose rows from `keep` on stay as they are; they must not overlap the inputs."""
-    for x in (k, v):
-        if not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() != 4 or x.shape[-1] != 128:
-            raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
+    kn, dev, bf16 = k.shape, k.device, torch.bfloat16
+    if not k.is_cuda or k.dtype is not bf16 or v.dtype is not bf16 or len(kn) != 4 or kn[3] != 128:
+        raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
     _no_grad(k, v, weights)
-    B, Hkv, S, D = k.shape
-    dev = k.device
-    if v.shape != k.shape or v.device != dev or S == 0:
-        raise ValueError(f"incompatible shapes k={tuple(k.shape)} v={tuple(v.shape)}")
-    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[:2] != k.shape[:2] or weights.shape[2] < S or weights.device != dev:
+    B, Hkv, S, D = kn
+    if v.shape != kn or v.device != dev or S == 0:
+        raise ValueError(f"incompatible shapes k={tuple(kn)} v={tuple(v.shape)}")
+    wn = weights.shape
+    if weights.dtype is not torch.float32 or len(wn) != 3 or wn[0] != B or wn[1] != Hkv or wn[2] < S or weights.device != dev:
         raise ValueError(f"weights must be float32 (batch, KV heads, at least {S}) on {dev}")
     keep, recent = int(keep), int(recent)
     if not 1 <= keep or not 0 <= recent <= keep:
         raise ValueError(f"expected keep >= 1 and recent from 0 to keep, got {keep} and {recent}")
-    lengths = _integers(lengths, "lengths", ((B,),), dev)
-    k, v = (x if _rows_usable(x) else x.contiguous() for x in (k, v))
-    weights = weights if weights.stride(-1) == 1 else weights.contiguous()
+    lengths, used, _ = _integers(lengths, "lengths", (B,), dev)
+    k, v = k if _rows_usable(k) else k.contiguous(), v if _rows_usable(v) else v.contiguous()
+    if weights.stride(2) != 1:
+        weights = weights.contiguous()
     if out is None:
-        k2, v2 = (torch.empty((B, Hkv, keep, D), dtype=k.dtype, device=dev) for _ in range(2))
-        w2 = torch.empty((B, Hkv, keep), dtype=torch.float32, device=dev)
+        k2, v2, w2 = k.new_empty((B, Hkv, keep, D)), k.new_empty((B, Hkv, keep, D)), weights.new_empty((B, Hkv, keep))
     else:
         k2, v2, w2 = out
         for x in (k2, v2):
-            if x.dtype != k.dtype or x.dim() != 4 or x.shape[:2] != k.shape[:2] or x.shape[2] < keep or x.shape[3] != D or x.device != dev:
+            if x.dtype is not bf16 or x.dim() != 4 or x.shape[:2] != kn[:2] or x.shape[2] < keep or x.shape[3] != D or x.device != dev:
                 raise ValueError(f"out needs bfloat16 ({B}, {Hkv}, at least {keep}, 128) for k and v on {dev}")
             if not _rows_usable(x):
                 raise ValueError("out needs unit stride in the last dimension and 16-byte aligned rows")
-        if w2.dtype != torch.float32 or w2.dim() != 3 or w2.shape[:2] != k.shape[:2] or w2.shape[2] < keep or w2.device != dev:
+        if w2.dtype is not torch.float32 or w2.dim() != 3 or w2.shape[:2] != kn[:2] or w2.shape[2] < keep or w2.device != dev:
             raise ValueError(f"out needs float32 ({B}, {Hkv}, at least {keep}) for the weights on {dev}")
         _no_grad(k2, v2, w2)
         for x in (k2, v2, w2):
@@ -342,17 +382,21 @@ def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
         if _overlapping((k2, v2, w2)) or any(_overlapping((x, y)) for x in (k2, v2, w2) for y in (k, v, weights)):
             raise ValueError("out must not overlap the cache: rows are still read while it is written")
     kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
-    if B == 0 or Hkv == 0:
-        return k2[:, :, :keep], v2[:, :, :keep], w2[:, :, :keep], kept
-    rc = lib.intra_b200_evict(k.data_ptr(), v.data_ptr(), weights.data_ptr(), _ptr(lengths), k2.data_ptr(), v2.data_ptr(),
-                              w2.data_ptr(), kept.data_ptr(), B, S, Hkv, keep, recent, _bsh(k), _bsh(v), _c_strides(*weights.stride()),
-                              _written(k2, (0, 2, 1)), _written(v2, (0, 2, 1)), _written(w2, (0, 1)), dev.index, _raw_stream(dev.index))
-    if rc != 0:
-        _raise(rc)
+    if B > 0 and Hkv > 0:
+        ks, vs, ws = k.stride(), v.stride(), weights.stride()
+        rc = lib.intra_b200_evict(k.data_ptr(), v.data_ptr(), weights.data_ptr(), used, k2.data_ptr(), v2.data_ptr(),
+                                  w2.data_ptr(), kept.data_ptr(), B, S, Hkv, keep, recent, _c_strides(ks[0], ks[2], ks[1]),
+                                  _c_strides(vs[0], vs[2], vs[1]), _c_strides(*ws), _written(k2, (0, 2, 1)), _written(v2, (0, 2, 1)),
+                                  _written(w2, (0, 1)), dev.index, _raw_stream(dev.index))
+        if rc != 0:
+            _raise(rc)
+    if out is None:
+        return k2, v2, w2, kept
     return k2[:, :, :keep], v2[:, :, :keep], w2[:, :, :keep], kept
 
 
 def _written(x, order):
     """Strides of a tensor that is written, those of dimensions of one entry made positive."""
-    s = [x.stride(d) if x.shape[d] > 1 else 8 for d in order]
+    n, st = x.shape, x.stride()
+    s = [st[d] if n[d] > 1 else 8 for d in order]
     return _c_strides(s[0], s[1], s[2] if len(s) > 2 else 0)
