@@ -121,7 +121,7 @@ int intra_b200_tree_attn(const void* q, const void* k, const void* v, const int*
  * token sampled last, parents as above. target[b][i] is the target's distribution over V tokens behind node i, draft[b][i]
  * the one its children were drawn from (n or n - 1 rows), both of type `prob_type`; draft NULL: drafts are certain. Child c of
  * the current node, in index order, is accepted iff uniform[b][c] * q(x) * Z < R(x), R and Z being p and 1; a rejection turns
- * R into max(R / Z - q, 0) and Z into its sum, where that is not zero. At the end one token is drawn from R: the
+ * R into max(R - Z q, 0) and Z into its sum, where that is not zero. At the end one token is drawn from R: the
  * smallest t with R(0) + .. + R(t) > uniform[b][0] * sum R. Sums in 64 bits. Outputs, contiguous: accepted[b], the number
  * of accepted drafts m; path[b] = 0 and the accepted nodes, then -1; out_tokens[b]: the accepted tokens, the drawn one
  * at place m, then -1. Drafts outside 0 .. V - 1 are rejected. Strides in elements {batch, node}; unit stride over V. */

@@ -4,9 +4,9 @@
 // index order, with token x, is accepted iff u_c q(x) Z < R(x); R is what is left of the current node's target row p and Z
 // its weight, R = p and Z = 1 to begin with. A rejection takes the drafts' distribution out,
 //
-//   R <- max(R / Z - q, 0),  Z <- sum R          (both stay where nothing would be left),
+//   R <- max(R - Z q, 0),  Z <- sum R            (both stay where nothing would be left),
 //
-// so that tokens come out distributed as p whatever q is. When no child is accepted the walk ends, and one more token
+// so that tokens come out distributed as p whatever q is (R / Z is the target's distribution given the rejections). When no child is accepted the walk ends, and one more token
 // is drawn from R: the smallest t with R(0) + .. + R(t) > u_0 sum R. Drafts without a distribution count as
 // certain: q is one at their token. All of it in 64 bits: an error of 2^-24 in a running sum over 10^5 tokens decides
 // the token in one draw of a hundred, 2^-53 in none.
@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const __grid_con
   __shared__ long long tok[VERIFY_MAX_TOKENS];
   __shared__ int parent[VERIFY_MAX_TOKENS], node[VERIFY_MAX_TOKENS];
   __shared__ double px[VERIFY_MAX_TOKENS], qx[VERIFY_MAX_TOKENS], ux[VERIFY_MAX_TOKENS];
-  __shared__ double weight[VERIFY_MAX_TOKENS];                     // Z before each rejection at the current node ...
+  __shared__ double weight[VERIFY_MAX_TOKENS];                     // Z at each rejection at the current node ...
   __shared__ long long gone[VERIFY_MAX_TOKENS];                    // ... and the token it rejected
   __shared__ double warp_sum[VERIFY_WARPS], scan_sum[VERIFY_WARPS];
   __shared__ double cta_sum[2];                                    // of the last two passes, read by the cluster
@@ -91,13 +91,10 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const __grid_con
   double Z = 1.0, total = 0.0;
   const T* p_row = target;
   const T* q_row = draft;
-  // What is left of token t's probability p0 after `count` rejections at the current node, q0 being its draft probability.
+  // What is left of the probability p0 of token t after `count` rejections at the current node, q0 being its draft probability.
   auto left = [&](double p0, double q0, long long t, int count) {
     double r = p0;
-    for (int c = 0; c < count; ++c) {
-      const double q = draft != nullptr ? q0 : t == gone[c] ? 1.0 : 0.0;
-      r = fmax((c == 0 ? r : r / weight[c]) - q, 0.0);
-    }
+    for (int c = 0; c < count; ++c) r = fmax(fma(-weight[c], draft != nullptr ? q0 : t == gone[c] ? 1.0 : 0.0, r), 0.0);
     return r;
   };
   auto left_at = [&](int t, int count) {
@@ -106,8 +103,35 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const __grid_con
   // Sum of what is left over the whole row: the same number in every thread of the cluster.
   auto row_sum = [&](int count) {
     double sum = 0.0;
-#pragma unroll 8
-    for (int t = begin + lane; t < end; t += 32) sum += left_at(t, count);
+    constexpr int AT_ONCE = 8;                                     // tokens of a lane whose loads are under way together
+    int t = begin + lane;
+    for (; t + 32 * (AT_ONCE - 1) < end; t += 32 * AT_ONCE) {
+      T pt[AT_ONCE], qt[AT_ONCE];
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) pt[e] = p_row[t + 32 * e];
+      const bool drawn = draft != nullptr && count > 0;
+      if (drawn) {
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; ++e) qt[e] = q_row[t + 32 * e];
+      }
+      double r[AT_ONCE];
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) r[e] = as_double(pt[e]);
+      for (int c = 0; c < count; ++c) {
+        const double w = -weight[c];
+        if (drawn) {
+#pragma unroll
+          for (int e = 0; e < AT_ONCE; ++e) r[e] = fmax(fma(w, as_double(qt[e]), r[e]), 0.0);
+        } else {
+          const int x = gone[c] >= 0 && gone[c] < V ? int(gone[c]) : -1;
+#pragma unroll
+          for (int e = 0; e < AT_ONCE; ++e) r[e] = t + 32 * e == x ? fmax(w + r[e], 0.0) : r[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) sum += r[e];
+    }
+    for (; t < end; t += 32) sum += left_at(t, count);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) warp_sum[warp] = sum;
