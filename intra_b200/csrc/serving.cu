@@ -125,10 +125,12 @@ int launch_tree_umma(const TreeParams& t, int B, const ServingState& st, int64_t
   p.t = t;
   p.B = B;
   p.t.row_groups = ceil_div(t.n * (t.H / t.Hkv), UMMA_ROWS<PAIR>);
+  p.by_rep = fast_div(t.H / t.Hkv);
   const int64_t tiles = int64_t(B) * t.Hkv * p.t.row_groups * ceil_div(t.S, TILE_N);       // at most
   const int64_t parts = (tiles + UMMA_MIN_TILES - 1) / UMMA_MIN_TILES;
   const int64_t rows = int64_t(B) * t.n * t.H;
-  if (tiles / B > 0x7fffffffLL || rows > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
+  const int64_t merge_ctas = int64_t(B) * t.Hkv * p.t.row_groups * UMMA_MERGE_CTAS<PAIR>;
+  if (tiles + st.sm_count > 0x7fffffffLL || rows > 0x7fffffffLL || merge_ctas > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
   const int grid = parts < st.sm_count ? int(parts) : st.sm_count;
   *scratch_needed = grid * 2 * UMMA_PARTIAL<PAIR> * int64_t(sizeof(float));
   if (!t.scratch || scratch_bytes < *scratch_needed) return INTRA_NEED_SCRATCH;
@@ -137,8 +139,16 @@ int launch_tree_umma(const TreeParams& t, int B, const ServingState& st, int64_t
   tree_umma_kernel<PAIR><<<grid, UMMA_THREADS, UMMA_SMEM_BYTES<PAIR>, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) {
-    tree_umma_merge_kernel<PAIR><<<unsigned((rows + UMMA_MERGE_ROWS - 1) / UMMA_MERGE_ROWS), 32 * UMMA_MERGE_ROWS, 0, stream>>>(p, grid);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(unsigned(merge_ctas));
+    cfg.blockDim = dim3(32 * UMMA_MERGE_WARPS);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, tree_umma_merge_kernel<PAIR>, p, uint32_t(grid));
   }
   return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
 }

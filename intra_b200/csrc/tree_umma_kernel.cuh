@@ -16,7 +16,9 @@
 //
 // Warp roles (512 threads): warps 0-3 and 4-7 softmax sets of the streams, a thread owning a row, which also write
 // the results; 8-11 request the tiles: TMA where a tile's rows are all keys of the sequence and the cache's strides
-// allow, else 16-byte copies in which rows past its last key become zeros; 12 issues QK^T (and, but for PAIR, PV), 13 PV.
+// allow, else 16-byte copies in which rows past its last key become zeros; 12 issues QK^T (and, but for PAIR, PV), 13 PV;
+// 14 and 15 bring the query rows of the units after the first, whose rows the softmax sets fetch. Whoever writes operands by plain copies fences them for the tensor cores' proxy before it
+// reports them.
 //
 // Barriers, all waits bounded (2 s; see attn_kernel.cuh for what a CTA does that gives up):
 //   full[r], free[r]   ring of tile buffers, in the order K0 K1 V0 K2 V1 .. over the CTA's tiles
@@ -45,13 +47,14 @@ template <bool PAIR> constexpr int UMMA_ROWS = PAIR ? 2 * TILE_M : TILE_M;      
 constexpr int UMMA_RING = 5;                     // tile buffers
 template <bool PAIR> constexpr int UMMA_SMEM_BYTES = (UMMA_RING + (PAIR ? 2 : 1)) * TILE_BYTES + 1024;
 // Partial results: a CTA leaves at most two, of the unit its part begins in and of the one it ends in. Each is the rows'
-// sums, then their maxima (log2 units) and weights.
+// sums, [column][row] so that 32 rows' stores of a column lie together, then their maxima (log2 units) and weights.
 template <bool PAIR> constexpr int64_t UMMA_PARTIAL = int64_t(UMMA_ROWS<PAIR>) * (HEAD_DIM + 2);
 // A CTA's part is at least this many key tiles: a shorter one costs more in its ends and its merge than it spreads.
 constexpr int UMMA_MIN_TILES = 2;
 
 struct TreeUmmaParams {
   TreeParams t;                // row_groups: units per KV head
+  FastDiv by_rep;              // query heads per KV head
   CUtensorMap maps[2];         // K, V: (128, S, 1, Hkv, B)
   int use_tma;
   int B;
@@ -66,32 +69,36 @@ struct TreePiece {             // what a CTA does of one unit
 };
 __device__ __forceinline__ int tree_tiles(const TreeParams& p, int b) { return (tree_context(p, b) + p.n + TILE_N - 1) / TILE_N; }
 
-// The list of all units' key tiles, and a CTA's part [next, end) of it as a cursor that every role moves by itself.
+// The list of all units' key tiles (at most 2^31 - 1), and a CTA's part [next, end) of it as a cursor that every role
+// moves by itself.
 struct TreeWalk {
-  int64_t per, next, end;      // length of a part; places in the list
-  int64_t b_start;             // place of sequence b's first tile
+  uint32_t per, next, end;     // length of a part; places in the list
+  uint32_t b_start;            // place of sequence b's first tile
   int b, b_tiles;              // b_tiles: of one unit
   // Called by whole warps; all lanes get the same.
-  __device__ __forceinline__ TreeWalk(const TreeParams& p, int B, int cta, int grid) {
+  __device__ __forceinline__ TreeWalk(const TreeParams& p, int B, uint32_t cta, uint32_t grid) {
     const int lane = threadIdx.x & 31, units = p.Hkv * p.row_groups;
-    int64_t total = 0;
-    for (int s = lane; s < B; s += 32) total += tree_tiles(p, s);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    uint32_t total = 0;
+    if (p.lengths == nullptr) {
+      total = uint32_t(B) * uint32_t(tree_tiles(p, 0));
+    } else {
+      for (int s = lane; s < B; s += 32) total += tree_tiles(p, s);
+      total = __reduce_add_sync(0xffffffffu, total);
+    }
     total *= units;
     per = (total + grid - 1) / grid;
     per = per < UMMA_MIN_TILES ? UMMA_MIN_TILES : per;
-    next = per * cta;
-    end = next + per < total ? next + per : total;
+    next = per * cta < total ? per * cta : total;
+    end = total - next > per ? next + per : total;
     b = b_tiles = 0;
     b_start = 0;
     if (next >= end) return;
     for (int s0 = 0; s0 < B; s0 += 32) {                           // the sequence that holds `next`
-      const int64_t mine = s0 + lane < B ? int64_t(tree_tiles(p, s0 + lane)) * units : 0;
-      int64_t upto = mine;
+      const uint32_t mine = s0 + lane < B ? uint32_t(tree_tiles(p, s0 + lane)) * units : 0u;
+      uint32_t upto = mine;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, upto, d);
+        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += y;
       }
       const uint32_t past = __ballot_sync(0xffffffffu, b_start + upto > next);
@@ -106,18 +113,18 @@ struct TreeWalk {
   }
   __device__ __forceinline__ bool piece(const TreeParams& p, TreePiece& x) {
     if (next >= end) return false;
-    const int units = p.Hkv * p.row_groups;
-    if (next - b_start >= int64_t(b_tiles) * units) {
-      b_start += int64_t(b_tiles) * units;
+    const uint32_t units = p.Hkv * p.row_groups;
+    if (next - b_start >= uint32_t(b_tiles) * units) {
+      b_start += uint32_t(b_tiles) * units;
       b_tiles = tree_tiles(p, ++b);
     }
-    const int local = int(next - b_start), unit = local / b_tiles;
+    const uint32_t local = next - b_start, unit = local / uint32_t(b_tiles);
     x.b = b;
-    x.hk = unit / p.row_groups;
+    x.hk = p.row_groups == 1 ? unit : unit / p.row_groups;
     x.rg = unit - x.hk * p.row_groups;
     x.of = b_tiles;
     x.first = local - unit * b_tiles;
-    x.count = int(end - next < b_tiles - x.first ? end - next : b_tiles - x.first);
+    x.count = min(int(end - next), b_tiles - x.first);
     x.ctx = tree_context(p, b);
     x.n_keys = x.ctx + p.n;
     next += x.count;
@@ -163,6 +170,7 @@ __device__ __forceinline__ unsigned long long tree_own_keys(const TreeParams& p,
 struct TreeRowOut {
   __nv_bfloat16* out;
   float* part;                 // null: whole
+  int part_step;               // floats between columns
 };
 
 // COLS columns from `col` on of one row of a piece, key by key, for rows whose sums are not finite: an infinite or NaN value row
@@ -184,7 +192,7 @@ __device__ __noinline__ void tree_exact_row(const TreeParams& p, const TreePiece
     for (int c = 0; c < COLS; ++c) acc[c] += prob * __bfloat162float(v[c]);
   }
   for (int c = 0; c < COLS; ++c) {
-    if (dst.part != nullptr) dst.part[col + c] = acc[c];
+    if (dst.part != nullptr) dst.part[(col + c) * dst.part_step] = acc[c];
     else dst.out[col + c] = __float2bfloat16(l == 0.f ? 0.f : acc[c] / l);
   }
 }
@@ -213,7 +221,8 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
     abort_flag = 0;
     for (int i = 0; i < N_BARS; ++i) {
       int n = 1;
-      if (i < FREE || i == Q_FULL) n = 128;
+      if (i < FREE) n = 128;
+      if (i == Q_FULL) n = 8;
       if ((i >= S_TAKEN && i < PV_DONE) || (i >= O_FREE && i < DRAIN)) n = 4;
       ptx::mbar_init(&bars[i], n);
     }
@@ -223,6 +232,23 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
     ptx::tmem_alloc(&tmem_base_smem, 512);
     ptx::tmem_relinquish();
   }
+  if (warp == 8 && lane < 2) ptx::prefetch_tensormap(&p.maps[lane]);
+  cudaTriggerProgrammaticLaunchCompletion();             // the merge may be set up; it waits for this kernel's end by itself
+  TreeWalk walk(t, p.B, blockIdx.x, gridDim.x);
+  TreePiece pc;
+  // Copies rows `first`, first + step, .. of a unit's queries, 16 threads a row; rows past the last become zeros.
+  auto copy_queries = [&](const TreePiece& x, int first, int step) {
+#pragma unroll 4
+    for (int at = first; at < ROWS; at += step) {
+      const int r = x.rg * ROWS + at, token = fdiv(r, p.by_rep);
+      const __nv_bfloat16* const src = t.q + x.b * t.q_sb + (x.hk * rep + r - token * rep) * t.q_sh + token * t.q_sn + (lane & 15) * 8;
+      ptx::cp_async_16(q_smem + (at >> 7) * TILE_BYTES + tile_offset(at & 127, lane & 15), r < all_rows ? src : t.q, r < all_rows ? 16u : 0u);
+    }
+    ptx::cp_async_commit();
+    ptx::cp_async_wait<0>();
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+  };
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
@@ -230,8 +256,6 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
   volatile int* abort_p = &abort_flag;
   bool ok = true;
 #define TREE_WAIT(index, parity, code) ptx::mbar_wait_at(bar(index), (parity) & 1, abort_p, code)
-  TreeWalk walk(t, p.B, blockIdx.x, gridDim.x);
-  TreePiece pc;
   // Ring requests of tile j, counted over the CTA: its K, and its V behind the next tile's K.
   auto k_request = [](uint32_t j) { return j == 0 ? 0u : 2 * j - 1; };
   auto v_request = [](uint32_t j) { return 2 * j + 2; };
@@ -246,9 +270,13 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
     const uint32_t o_addr = lane_addr + 256 + sx * 128;
     uint32_t kt = 0, unit = 0, done[2] = {0, 0};          // tiles of this stream, units, units in which a stream had tiles
     while (walk.piece(t, pc)) {
+      if (unit == 0) {                                    // the first unit's queries: nobody else has as many hands free
+        copy_queries(pc, 2 * warp + (lane >> 4), 16);
+        if (lane == 0) ptx::mbar_arrive_at(bar(Q_FULL));
+      }
       const int r = pc.rg * ROWS + (PAIR ? sx * TILE_M : 0) + row;
       const bool valid = r < all_rows, busy = __any_sync(0xffffffffu, valid);
-      const int token = min(r, all_rows - 1) / rep, head = pc.hk * rep + min(r, all_rows - 1) - token * rep;
+      const int token = fdiv(min(r, all_rows - 1), p.by_rep), head = pc.hk * rep + min(r, all_rows - 1) - token * rep;
       const unsigned long long own = (pc.first + pc.count) * TILE_N > pc.ctx ? tree_own_keys(t, pc.b, token) : 0ull;
       float m_run = -CUDART_INF_F, l_run = 0.f;
       const int n_mine = PAIR ? pc.count : (pc.count + 1 - sx) / 2;
@@ -259,12 +287,16 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
         if (!ok) break;
         ptx::tc_fence_after();
         if (!busy) {                                      // no row of this warp exists: its results are never read
+          if (PAIR) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_at(bar(S_TAKEN + sx));
+            ok = TREE_WAIT(PV_DONE + sx, kt - 1, 13 + sx);                // P is reported once a PV, as by warps with rows
+            if (!ok) break;
+          }
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            if (PAIR) ptx::mbar_arrive_at(bar(S_TAKEN + sx));
-            ptx::mbar_arrive_at(bar(P_FULL + sx));
-          }
+          if (lane == 0) ptx::mbar_arrive_at(bar(P_FULL + sx));
           continue;
         }
         float s[TILE_N];
@@ -415,11 +447,11 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
       };
       bool finite = true;
       if (busy) {
-        TreeRowOut dst = {t.o + ((int64_t(pc.b) * t.n + token) * t.H + head) * HEAD_DIM, nullptr};
+        TreeRowOut dst = {t.o + ((int64_t(pc.b) * t.n + token) * t.H + head) * HEAD_DIM, nullptr, ROWS};
         if (pc.count != pc.of) {
           float* const part = t.scratch + (int64_t(blockIdx.x) * 2 + (pc.first == 0 ? 1 : 0)) * UMMA_PARTIAL<PAIR>;
           const int at = r - pc.rg * ROWS;
-          dst.part = part + int64_t(at) * HEAD_DIM;
+          dst.part = part + at;
           if (valid && col == 0) reinterpret_cast<float2*>(part + int64_t(ROWS) * HEAD_DIM)[at] = make_float2(m, l);
         }
         const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
@@ -431,9 +463,8 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
           for (int e = 0; e < 32; ++e) finite = finite && fabsf(o[e]) < CUDART_INF_F;
           if (!valid) continue;
           if (dst.part != nullptr) {
-            float4* const d = reinterpret_cast<float4*>(dst.part + col + c);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 32; ++e) dst.part[(col + c + e) * ROWS] = o[e];
           } else {
             uint4* const d = reinterpret_cast<uint4*>(dst.out + col + c);
 #pragma unroll
@@ -453,11 +484,18 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
     // ================================ requests of the tiles ========================================
     ptx::setmaxnreg_dec<UMMA_LOAD_REGS>();
     const int lt = tid - 256;                             // 0 .. 127; in copies: row lt >> 4 of every 8, piece lt & 15
+    int copied = -1;                                      // buffer whose copies this thread has issued and not reported
+    auto report = [&] {
+      ptx::fence_proxy_async_smem();
+      ptx::mbar_arrive_at(bar(FULL + copied));
+      copied = -1;
+    };
     auto request = [&](uint32_t req, int operand, const TreePiece& x, int tile) {
       const uint32_t slot = req % RING, dst = ring_smem + slot * TILE_BYTES;
       if (!(ok = TREE_WAIT(FREE + slot, req / RING - 1, 21 + operand))) return;
       const int key0 = tile * TILE_N;
       if (p.use_tma && (key0 + TILE_N <= x.n_keys || x.n_keys == t.S)) {  // rows past the cache's end come as zeros
+        if (copied >= 0) { ptx::cp_async_wait<0>(); report(); }
         if (lt == 0) {
           ptx::mbar_expect_tx_at(bar(FULL + slot), TILE_BYTES);
           ptx::tma_load_5d_at(dst, &p.maps[operand], bar(FULL + slot), 0, key0, 0, x.hk, x.b);
@@ -475,35 +513,25 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
         const bool there = key0 + row < x.n_keys;
         ptx::cp_async_16(dst + tile_offset(row, lt & 15), there ? src + (key0 + row) * st.ss : src, there ? 16u : 0u);
       }
-      ptx::cp_async_mbar_arrive_noinc(&bars[FULL + slot]);
+      ptx::cp_async_commit();
+      // A tile is reported when the next one's copies are under way; nothing that the next buffer waits for needs it.
+      if (copied >= 0) { ptx::cp_async_wait<1>(); report(); }
+      copied = int(slot);
     };
-    uint32_t j = 0, unit = 0;
+    uint32_t j = 0;
     TreePiece before;                                     // of the tile whose V is requested next
     int v_tile = -1;
-    if (lt < 2) ptx::prefetch_tensormap(&p.maps[lt]);
     while (ok && walk.piece(t, pc)) {
       for (int i = 0; i < pc.count && ok; ++i, ++j) {
         request(k_request(j), 0, pc, pc.first + i);
-        if (ok && i == 0) {
-          ok = TREE_WAIT(Q_FREE, unit - 1, 23);
-          if (!ok) break;
-#pragma unroll 4
-          for (int c = 0; c < ROWS / 8; ++c) {
-            const int at = c * 8 + (lt >> 4), r = pc.rg * ROWS + at, token = r / rep;
-            const __nv_bfloat16* const src = t.q + pc.b * t.q_sb + (pc.hk * rep + r - token * rep) * t.q_sh + token * t.q_sn + (lt & 15) * 8;
-            ptx::cp_async_16(q_smem + (at >> 7) * TILE_BYTES + tile_offset(at & 127, lt & 15), r < all_rows ? src : t.q, r < all_rows ? 16u : 0u);
-          }
-          ptx::cp_async_mbar_arrive_noinc(&bars[Q_FULL]);
-        }
         if (ok && v_tile >= 0) request(v_request(j - 1), 1, before, v_tile);
         before = pc;
         v_tile = pc.first + i;
       }
-      ++unit;
     }
     if (ok && v_tile >= 0) request(v_request(j - 1), 1, before, v_tile);
-    ptx::cp_async_commit();
     ptx::cp_async_wait<0>();
+    if (copied >= 0) report();
   } else {
     ptx::setmaxnreg_dec<UMMA_ISSUE_REGS>();
     // ================================ MMA issue ====================================================
@@ -518,7 +546,6 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
       if (!ok) return;
       ptx::tc_fence_after();
       if (ptx::elect_one()) {
-        ptx::fence_proxy_async_smem();                    // tiles may have come by plain copies
         issue_qk_loop(q_desc + (PAIR ? sx : 0) * STEP, k_desc + slot * STEP, tmem + (PAIR ? 0 : sx * 128));
         ptx::mma_commit_at(bar(S_FULL + sx));
         if (last) ptx::mma_commit_at(bar(FREE + slot));
@@ -535,7 +562,6 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
       ++kt[sx];
       ptx::tc_fence_after();
       if (ptx::elect_one()) {
-        ptx::fence_proxy_async_smem();
         const uint32_t p_cols = PAIR ? tmem + 128 + sx * 64 : tmem + sx * 128;
         issue_pv_loop(p_cols, v_desc + slot * STEP, tmem + 256 + sx * 128, first_of_stream ? 0 : 1);
         if (!PAIR) issue_pv_loop(p_cols + 64, v_desc + slot * STEP, tmem + 256 + sx * 128, 1);
@@ -573,6 +599,17 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
         int dummy = 0;
         ptx::mbar_wait(&bars[drain], 0, &dummy, 100);
       }
+    } else if (warp >= 14) {
+      // ================================ query rows ==================================================
+      while (ok && walk.piece(t, pc)) {
+        if (unit > 0) {
+          ok = TREE_WAIT(Q_FREE, unit - 1, 23);
+          if (!ok) break;
+          copy_queries(pc, 2 * (warp - 14) + (lane >> 4), 4);
+          if (lane < 4) ptx::mbar_arrive_at(bar(Q_FULL));
+        }
+        ++unit;
+      }
     }
   }
 #undef TREE_WAIT
@@ -589,56 +626,78 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
   }
 }
 
-// Joins the partial results of units that several CTAs had a part of. A warp per row: lane = 4 dims.
-constexpr int UMMA_MERGE_ROWS = 8;
+// Joins the partial results of units that several CTAs had a part of. A thread has UMMA_MERGE_COLS columns of a row, a
+// warp 32 rows. Loads of rows that do not exist stay inside the buffer and are not used.
+constexpr int UMMA_MERGE_COLS = 4, UMMA_MERGE_WARPS = 4;
+constexpr int UMMA_MERGE_SPLIT = HEAD_DIM / (UMMA_MERGE_COLS * UMMA_MERGE_WARPS);       // CTAs per 32 rows
+template <bool PAIR> constexpr int UMMA_MERGE_CTAS = UMMA_ROWS<PAIR> / 32 * UMMA_MERGE_SPLIT;      // per unit
 template <bool PAIR>
-__global__ void __launch_bounds__(32 * UMMA_MERGE_ROWS) tree_umma_merge_kernel(const __grid_constant__ TreeUmmaParams p, int grid) {
+__global__ void __launch_bounds__(32 * UMMA_MERGE_WARPS) tree_umma_merge_kernel(const __grid_constant__ TreeUmmaParams p, uint32_t grid) {
+  constexpr int ROWS = UMMA_ROWS<PAIR>;
   const TreeParams& t = p.t;
   const int lane = threadIdx.x & 31, rep = t.H / t.Hkv;
-  const int64_t out_row = int64_t(blockIdx.x) * UMMA_MERGE_ROWS + (threadIdx.x >> 5);      // (b, hk, row of the KV head)
-  const int all_rows = t.n * rep;
-  const int hk_b = int(out_row / all_rows), row = int(out_row - int64_t(hk_b) * all_rows);
-  const int b = hk_b / t.Hkv, hk = hk_b - b * t.Hkv;
-  if (b >= p.B) return;
-  const int rg = row / UMMA_ROWS<PAIR>, at = row - rg * UMMA_ROWS<PAIR>;
-  int64_t total = 0, start = 0;                           // tiles of all units, and before this one
-  const int units = t.Hkv * t.row_groups;
+  const int unit = blockIdx.x / UMMA_MERGE_CTAS<PAIR>, block = blockIdx.x - unit * UMMA_MERGE_CTAS<PAIR>;
+  const int units = t.Hkv * t.row_groups, b = unit / units, in_b = unit - b * units;
+  const int hk = in_b / t.row_groups, rg = in_b - hk * t.row_groups;
+  const int at = block / UMMA_MERGE_SPLIT * 32 + lane, row = rg * ROWS + at;
+  const int col = (block % UMMA_MERGE_SPLIT * UMMA_MERGE_WARPS + (threadIdx.x >> 5)) * UMMA_MERGE_COLS;
+  if (row - lane >= t.n * rep) return;                    // no such rows
+  uint32_t total = 0, start = 0;                          // tiles of all units, and before this one
   for (int s = lane; s < p.B; s += 32) {
-    const int64_t n = int64_t(tree_tiles(t, s)) * units;
+    const uint32_t n = uint32_t(tree_tiles(t, s)) * units;
     total += n;
-    start += s < b ? n : 0;
+    start += s < b ? n : 0u;
   }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, d);
-    start += __shfl_xor_sync(0xffffffffu, start, d);
-  }
-  int64_t per = (total + grid - 1) / grid;
+  total = __reduce_add_sync(0xffffffffu, total);
+  start = __reduce_add_sync(0xffffffffu, start);
+  uint32_t per = (total + grid - 1) / grid;
   per = per < UMMA_MIN_TILES ? UMMA_MIN_TILES : per;
   const int tiles = tree_tiles(t, b);
-  start += int64_t(hk * t.row_groups + rg) * tiles;
+  start += uint32_t(in_b) * tiles;
   const int c0 = int(start / per), c1 = int((start + tiles - 1) / per);
+  cudaGridDependencySynchronize();                        // everything before this ran beside the main kernel's end
   if (c0 == c1) return;                                   // one CTA held the unit and wrote its rows
-  auto slot = [&](int c) { return t.scratch + (int64_t(c) * 2 + (c == c0 ? 1 : 0)) * UMMA_PARTIAL<PAIR>; };
-  auto ml = [&](int c) { return reinterpret_cast<const float2*>(slot(c) + int64_t(UMMA_ROWS<PAIR>) * HEAD_DIM)[at]; };
-  float m_all = -CUDART_INF_F;
-  for (int c = c0 + lane; c <= c1; c += 32) m_all = fmaxf(m_all, ml(c).x);
+  // The part in the CTA the unit begins in is that CTA's second slot, in the others the first.
+  const float* const first = t.scratch + (int64_t(c0) * 2 + 1) * UMMA_PARTIAL<PAIR>;
+  auto slot = [&](int i) { return first + (i == 0 ? 0 : (int64_t(i) * 2 - 1) * UMMA_PARTIAL<PAIR>); };
+  auto ml = [&](int i) { return reinterpret_cast<const float2*>(slot(i) + ROWS * HEAD_DIM)[at]; };
+  const int parts = c1 - c0 + 1;
+  float acc[UMMA_MERGE_COLS];
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, d));
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l_all = 0.f;
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const float2 x = ml(c);
-    const float f = merge_weight(x.x, m_all);
-    const float4 o = reinterpret_cast<const float4*>(slot(c) + int64_t(at) * HEAD_DIM)[lane];
-    acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
-    l_all += f * x.y;
+  for (int e = 0; e < UMMA_MERGE_COLS; ++e) acc[e] = 0.f;
+  float m_all = -CUDART_INF_F, l_all = 0.f;
+  constexpr int AT_ONCE = 8;                              // parts whose loads are under way together
+  for (int i0 = 0; i0 < parts; i0 += AT_ONCE) {           // running maximum over batches of parts
+    float2 x[AT_ONCE];
+    float o[AT_ONCE][UMMA_MERGE_COLS];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int c = min(i0 + i, parts - 1);
+      x[i] = ml(c);
+#pragma unroll
+      for (int e = 0; e < UMMA_MERGE_COLS; ++e) o[i][e] = slot(c)[(col + e) * ROWS + at];
+    }
+    float m_new = m_all;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) m_new = fmaxf(m_new, x[i].x);
+    const float alpha = merge_weight(m_all, m_new);
+    l_all *= alpha;
+#pragma unroll
+    for (int e = 0; e < UMMA_MERGE_COLS; ++e) acc[e] *= alpha;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const float f = i0 + i < parts ? merge_weight(x[i].x, m_new) : 0.f;
+      l_all += i0 + i < parts ? f * x[i].y : 0.f;
+#pragma unroll
+      for (int e = 0; e < UMMA_MERGE_COLS; ++e) acc[e] += i0 + i < parts ? f * o[i][e] : 0.f;
+    }
+    m_all = m_new;
   }
+  if (row >= t.n * rep) return;
   const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
-  const int token = row / rep, head = hk * rep + row - token * rep;
-  uint2* const dst = reinterpret_cast<uint2*>(t.o + ((int64_t(b) * t.n + token) * t.H + head) * HEAD_DIM) + lane;
-  *dst = make_uint2(ptx::pack_bf16(acc.x * inv, acc.y * inv), ptx::pack_bf16(acc.z * inv, acc.w * inv));
+  const int token = fdiv(row, p.by_rep), head = hk * rep + row - token * rep;
+  *reinterpret_cast<uint2*>(t.o + ((int64_t(b) * t.n + token) * t.H + head) * HEAD_DIM + col) =
+      make_uint2(ptx::pack_bf16(acc[0] * inv, acc[1] * inv), ptx::pack_bf16(acc[2] * inv, acc[3] * inv));
 }
 
 }  // namespace intra

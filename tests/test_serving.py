@@ -102,7 +102,12 @@ TREES = [
     (2, 9, 1, 7, 500, "bhsd", "random", True, "strided"), (1, 64, 2, 3, 130, "bhsd", "random", True, "padding"),
     (1, 4, 1, 9, 40000, "sliced", "random", False, None), (16, 32, 8, 8, 2100, "bhsd", None, False, "padding"),
     (70, 4, 1, 3, 90, "bhsd", "random", True, None), (1, 40, 1, 64, 333, "bhsd", "random", True, "random"),
-    (2, 32, 8, 20, 16400, "bhsd", "random", True, "padding")]
+    (2, 32, 8, 20, 16400, "bhsd", "random", True, "padding"),
+    # more than 256 rows per KV head, of which the last tile has none; CTAs that hold many whole units, or parts of two
+    (1, 5, 1, 64, 900, "bhsd", "random", True, None), (2, 12, 4, 60, 1500, "bshd", "random", True, None), (50, 8, 2, 20, 420, "bhsd", "random", True, None),
+    (60, 8, 1, 40, 140, "bhsd", "random", True, None), (130, 8, 2, 33, 400, "sliced", "chain", True, None),
+    # caches that tensor maps do not describe
+    (3, 8, 2, 30, 1000, "batch1", "random", True, None), (3, 8, 2, 64, 1300, "batch1", None, False, None)]
 
 
 def _tree_case(B, H, Hkv, n, S, layout, kind, with_lengths, mask_kind, seed=0):
