@@ -40,8 +40,10 @@ void init_serving(int device) {
   e = cudaDeviceGetAttribute(&st.sm_count, cudaDevAttrMultiProcessorCount, device);
   if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<1>, tree_smem_bytes<1>(TREE_MASK_TOKENS));
   if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<2>, tree_smem_bytes<2>(TREE_MASK_TOKENS));
-  if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<false>, UMMA_SMEM_BYTES<false>);
-  if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<true>, UMMA_SMEM_BYTES<true>);
+  if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<false, false>, UMMA_SMEM_BYTES<false>);
+  if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<false, true>, UMMA_SMEM_BYTES<false>);
+  if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<true, false>, UMMA_SMEM_BYTES<true>);
+  if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<true, true>, UMMA_SMEM_BYTES<true>);
   void* word = nullptr;
   if (e == cudaSuccess) e = cudaGetSymbolAddress(&word, g_serving_status);
   st.status_word = static_cast<int*>(word);
@@ -74,6 +76,23 @@ cudaError_t launch_cluster(K kernel, int64_t clusters, int cluster, int threads,
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// Launch of a kernel that may be set up while the kernel before it in the stream still runs, and that waits for that one's
+// end (cudaGridDependencySynchronize) before it touches memory.
+template <typename K, typename... P>
+cudaError_t launch_early(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, const P&... p) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p...);
 }
 
 // How a cache of S keys is dealt out: CTAs per cluster and clusters per unit (a KV head's rows that one pass takes). As
@@ -119,6 +138,7 @@ bool cache_map(const __nv_bfloat16* ptr, const TensorView& v, int S, int Hkv, in
   return encode_map(map, ptr, 5, dims, strides, box, ones);
 }
 
+constexpr int UMMA_FROM_ROWS = 16;
 template <bool PAIR>
 int launch_tree_umma(const TreeParams& t, int B, const ServingState& st, int64_t scratch_bytes, int64_t* scratch_needed, cudaStream_t stream) {
   TreeUmmaParams p;
@@ -129,27 +149,34 @@ int launch_tree_umma(const TreeParams& t, int B, const ServingState& st, int64_t
   const int64_t tiles = int64_t(B) * t.Hkv * p.t.row_groups * ceil_div(t.S, TILE_N);       // at most
   const int64_t parts = (tiles + UMMA_MIN_TILES - 1) / UMMA_MIN_TILES;
   const int64_t rows = int64_t(B) * t.n * t.H;
+  const int64_t places = tiles + int64_t(B) * t.Hkv * p.t.row_groups * 3;      // and their ends
   const int64_t merge_ctas = int64_t(B) * t.Hkv * p.t.row_groups * UMMA_MERGE_CTAS<PAIR>;
-  if (tiles + st.sm_count > 0x7fffffffLL || rows > 0x7fffffffLL || merge_ctas > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
+  if (places + st.sm_count > 0x7fffffffLL || rows > 0x7fffffffLL || merge_ctas > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
   const int grid = parts < st.sm_count ? int(parts) : st.sm_count;
+  p.t.pair = PAIR;
   *scratch_needed = grid * 2 * UMMA_PARTIAL<PAIR> * int64_t(sizeof(float));
+  if (t.mask) {                   // behind the partial results: the mask's bits, those of any token, the tiles
+    char* const at = reinterpret_cast<char*>(t.scratch) + *scratch_needed;
+    p.t.bits_tokens = t.mask_sn ? t.n : 1;
+    p.t.bits_words = ceil_div(t.S, TILE_N) * (TILE_N / 32);
+    p.t.live_words = ceil_div(ceil_div(t.S, TILE_N), 64);
+    const int64_t row = int64_t(p.t.bits_words) * 4;
+    p.t.bits = reinterpret_cast<uint32_t*>(at);
+    p.t.any = reinterpret_cast<uint32_t*>(at + row * B * p.t.bits_tokens);
+    p.t.live = reinterpret_cast<uint8_t*>(at + row * B * (p.t.bits_tokens + 1));
+    *scratch_needed += row * B * (p.t.bits_tokens + 1) + int64_t(p.t.live_words) * 8 * B;
+    if (B > 65535) return INTRA_ERR_UNSUPPORTED;                   // grid.y of the bits
+  }
   if (!t.scratch || scratch_bytes < *scratch_needed) return INTRA_NEED_SCRATCH;
   p.use_tma = cache_map(t.k, t.ks, t.S, t.Hkv, B, &p.maps[0]) && cache_map(t.v, t.vs, t.S, t.Hkv, B, &p.maps[1]);
   p.status = st.status_word;
-  tree_umma_kernel<PAIR><<<grid, UMMA_THREADS, UMMA_SMEM_BYTES<PAIR>, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(unsigned(merge_ctas));
-    cfg.blockDim = dim3(32 * UMMA_MERGE_WARPS);
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, tree_umma_merge_kernel<PAIR>, p, uint32_t(grid));
-  }
+  cudaError_t e = cudaSuccess;
+  if (t.mask) e = launch_early(tree_mask_kernel, dim3(unsigned(ceil_div(p.t.bits_words, 32)), unsigned(B)), 32 * TREE_MASK_ROWS, 0, stream, p.t);
+  if (e == cudaSuccess)
+    e = t.mask ? launch_early(tree_umma_kernel<PAIR, true>, dim3(unsigned(grid)), UMMA_THREADS, UMMA_SMEM_BYTES<PAIR>, stream, p)
+               : launch_early(tree_umma_kernel<PAIR, false>, dim3(unsigned(grid)), UMMA_THREADS, UMMA_SMEM_BYTES<PAIR>, stream, p);
+  if (e == cudaSuccess)
+    e = launch_early(tree_umma_merge_kernel<PAIR>, dim3(unsigned(merge_ctas)), 32 * UMMA_MERGE_WARPS, 0, stream, p, uint32_t(grid));
   return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
 }
 
@@ -202,8 +229,8 @@ int intra_b200_tree_attn(const void* q, const void* k, const void* v, const int*
   p.S = S; p.H = H; p.Hkv = Hkv; p.n = n;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  if (!mask && n * (H / Hkv) > 128) return launch_tree_umma<true>(p, B, *st, scratch_bytes, scratch_needed, stream);
-  if (!mask && n * (H / Hkv) > 32) return launch_tree_umma<false>(p, B, *st, scratch_bytes, scratch_needed, stream);
+  if (n * (H / Hkv) > 128) return launch_tree_umma<true>(p, B, *st, scratch_bytes, scratch_needed, stream);
+  if (n * (H / Hkv) > UMMA_FROM_ROWS) return launch_tree_umma<false>(p, B, *st, scratch_bytes, scratch_needed, stream);
   if (n * (H / Hkv) <= 16) return launch_tree_mma<1>(p, B, *st, scratch_bytes, scratch_needed, stream);
   return launch_tree_mma<2>(p, B, *st, scratch_bytes, scratch_needed, stream);
 }

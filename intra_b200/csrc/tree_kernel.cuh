@@ -44,6 +44,13 @@ struct TreeParams {
   int all_own;                 // tokens see all n own keys: the mask decides alone
   int64_t mask_sb, mask_sn, mask_ss;
   int mask_vec;                // 16 mask bytes of a key block can be loaded at once
+  // tree_umma_kernel.cuh: the mask as bits, a word for 32 keys ([sequence][token or 1][word]), the same of the keys any token
+  // sees, and a bit for each key tile that holds such keys ([sequence][64-bit word]); null: no mask
+  const uint32_t* bits;
+  const uint32_t* any;
+  const uint8_t* live;
+  int bits_tokens, bits_words, live_words;
+  int pair;                    // units of 256 rows
   int S, H, Hkv, n;
   int row_groups;              // passes over the keys, each for up to 16 * MT rows
   int cluster, n_clusters;

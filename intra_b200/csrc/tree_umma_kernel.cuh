@@ -16,7 +16,7 @@
 //
 // Warp roles (512 threads): warps 0-3 and 4-7 softmax sets of the streams, a thread owning a row, which also write
 // the results; 8-11 request the tiles: TMA where a tile's rows are all keys of the sequence and the cache's strides
-// allow, else 16-byte copies in which rows past its last key become zeros; 12 issues QK^T (and, but for PAIR, PV), 13 PV;
+// allow, else 16-byte copies in which rows past its last key, and rows no token sees, become zeros; 12 issues QK^T (and, but for PAIR, PV), 13 PV;
 // 14 and 15 bring the query rows of the units after the first, whose rows the softmax sets fetch. Whoever writes operands by plain copies fences them for the tensor cores' proxy before it
 // reports them.
 //
@@ -65,36 +65,82 @@ struct TreePiece {             // what a CTA does of one unit
   int b, hk, rg;               // sequence, KV head, row group
   int first, count;            // key tiles
   int of;                      // key tiles of the whole unit
+  int starts;                  // the piece begins with the unit
   int ctx, n_keys;
 };
-__device__ __forceinline__ int tree_tiles(const TreeParams& p, int b) { return (tree_context(p, b) + p.n + TILE_N - 1) / TILE_N; }
-
-// The list of all units' key tiles (at most 2^31 - 1), and a CTA's part [next, end) of it as a cursor that every role
-// moves by itself.
-struct TreeWalk {
-  uint32_t per, next, end;     // length of a part; places in the list
-  uint32_t b_start;            // place of sequence b's first tile
-  int b, b_tiles;              // b_tiles: of one unit
-  // Called by whole warps; all lanes get the same.
-  __device__ __forceinline__ TreeWalk(const TreeParams& p, int B, uint32_t cta, uint32_t grid) {
-    const int lane = threadIdx.x & 31, units = p.Hkv * p.row_groups;
-    uint32_t total = 0;
-    if (p.lengths == nullptr) {
-      total = uint32_t(B) * uint32_t(tree_tiles(p, 0));
-    } else {
-      for (int s = lane; s < B; s += 32) total += tree_tiles(p, s);
-      total = __reduce_add_sync(0xffffffffu, total);
+// Key tiles of a sequence; with a mask from the first to the last of which any token sees a key (one, where there is none).
+__device__ __forceinline__ int tree_tiles(const TreeParams& p, int b, int* first = nullptr) {
+  const int all = (tree_context(p, b) + p.n + TILE_N - 1) / TILE_N;
+  int lo = 0, hi = all;
+  if (p.live != nullptr) {
+    const unsigned long long* const live = reinterpret_cast<const unsigned long long*>(p.live) + int64_t(b) * p.live_words;
+    lo = all;
+    hi = 0;
+    for (int i = 0; i * 64 < all; ++i) {
+      const int left = all - i * 64;
+      const unsigned long long x = live[i] & (left >= 64 ? ~0ull : (1ull << left) - 1ull);
+      if (x) {
+        lo = min(lo, i * 64 + __ffsll(x) - 1);
+        hi = i * 64 + 64 - __clzll(x);
+      }
     }
-    total *= units;
+    if (hi == 0) { lo = 0; hi = 1; }
+  }
+  if (first) *first = lo;
+  return hi - lo;
+}
+
+// The list of all units' key tiles. A unit counts for `cost` places more than it has tiles, in front of them: what the end
+// of one unit and the start of the next cost the CTA that has both (parts of a few tiles would only be spread unevenly by
+// it). Measured with 0 / 1 / 3 places: 64 tokens over 65536 keys (PAIR) 73.1 / 71.9 / 70.6 us, 26 tokens over 8 sequences of
+// 4096 to 8192 keys 59.8 / 59.2 / 67.8. At most 2^31 - 1 places.
+struct TreeList {
+  uint32_t units, cost, per, total;      // units per sequence; places of a CTA's part, of all
+  // Called by whole warps; all lanes get the same. `before`: tiles and units of sequences before `b`.
+  __device__ __forceinline__ TreeList(const TreeParams& p, int B, uint32_t grid, int b = 0, uint32_t* before = nullptr) {
+    units = p.Hkv * p.row_groups;
+    uint32_t tiles = 0, front = 0;
+    if (p.lengths == nullptr && p.live == nullptr) {               // all sequences alike
+      tiles = uint32_t(B) * uint32_t(tree_tiles(p, 0));
+      front = uint32_t(b) * uint32_t(tree_tiles(p, 0));
+    } else {
+      for (int s = threadIdx.x & 31; s < B; s += 32) {
+        const uint32_t n = tree_tiles(p, s);
+        tiles += n;
+        front += s < b ? n : 0u;
+      }
+      tiles = __reduce_add_sync(0xffffffffu, tiles);
+      front = __reduce_add_sync(0xffffffffu, front);
+    }
+    const uint32_t share = tiles * units / grid;
+    cost = share < 8 ? 0 : p.pair && share >= 16 ? 3 : 1;
+    total = (tiles + cost * B) * units;
     per = (total + grid - 1) / grid;
     per = per < UMMA_MIN_TILES ? UMMA_MIN_TILES : per;
-    next = per * cta < total ? per * cta : total;
-    end = total - next > per ? next + per : total;
-    b = b_tiles = 0;
+    if (before) *before = (front + cost * b) * units;
+  }
+};
+
+// A CTA's part [next, end) of the list as a cursor that every warp moves by itself. Cursor and piece stand in shared memory:
+// as registers they would make the softmax warps, which hold a row's 128 scores, spill.
+struct TreeWalk {
+  uint32_t next, end;
+  uint32_t b_start;            // place of sequence b's first unit
+  uint32_t units, cost;
+  int b, b_tiles, b_first;     // of one unit: its tiles, the first of them
+  // Called by whole warps; all lanes get the same.
+  __device__ __forceinline__ void start(const TreeParams& p, int B, uint32_t cta, uint32_t grid) {
+    const int lane = threadIdx.x & 31;
+    const TreeList list(p, B, grid);
+    units = list.units;
+    cost = list.cost;
+    next = list.per * cta < list.total ? list.per * cta : list.total;
+    end = list.total - next > list.per ? next + list.per : list.total;
+    b = b_tiles = b_first = 0;
     b_start = 0;
     if (next >= end) return;
     for (int s0 = 0; s0 < B; s0 += 32) {                           // the sequence that holds `next`
-      const uint32_t mine = s0 + lane < B ? uint32_t(tree_tiles(p, s0 + lane)) * units : 0u;
+      const uint32_t mine = s0 + lane < B ? (uint32_t(tree_tiles(p, s0 + lane)) + cost) * units : 0u;
       uint32_t upto = mine;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
@@ -109,28 +155,42 @@ struct TreeWalk {
       }
       b_start += __shfl_sync(0xffffffffu, upto, 31);
     }
-    b_tiles = tree_tiles(p, b);
+    b_tiles = tree_tiles(p, b, &b_first);
   }
-  __device__ __forceinline__ bool piece(const TreeParams& p, TreePiece& x) {
-    if (next >= end) return false;
-    const uint32_t units = p.Hkv * p.row_groups;
-    if (next - b_start >= uint32_t(b_tiles) * units) {
-      b_start += uint32_t(b_tiles) * units;
-      b_tiles = tree_tiles(p, ++b);
+  __device__ __forceinline__ void piece(const TreeParams& p, TreePiece& x) {
+    x.count = 0;
+    while (next < end) {
+      uint32_t places = b_tiles + cost;
+      if (next - b_start >= places * units) {
+        b_start += places * units;
+        b_tiles = tree_tiles(p, ++b, &b_first);
+        places = b_tiles + cost;
+      }
+      const uint32_t local = next - b_start, unit = local / places, at = local - unit * places;
+      const uint32_t take = min(end - next, places - at);
+      next += take;
+      const int first = max(int(at) - int(cost), 0), last = int(at + take) - int(cost);
+      if (last <= first) continue;                                 // of this unit only places without tiles
+      x.b = b;
+      x.hk = p.row_groups == 1 ? unit : unit / p.row_groups;
+      x.rg = unit - x.hk * p.row_groups;
+      x.of = b_tiles;
+      x.first = b_first + first;
+      x.count = last - first;
+      x.starts = first == 0;
+      x.ctx = tree_context(p, b);
+      x.n_keys = x.ctx + p.n;
+      return;
     }
-    const uint32_t local = next - b_start, unit = local / uint32_t(b_tiles);
-    x.b = b;
-    x.hk = p.row_groups == 1 ? unit : unit / p.row_groups;
-    x.rg = unit - x.hk * p.row_groups;
-    x.of = b_tiles;
-    x.first = local - unit * b_tiles;
-    x.count = min(int(end - next), b_tiles - x.first);
-    x.ctx = tree_context(p, b);
-    x.n_keys = x.ctx + p.n;
-    next += x.count;
-    return true;
   }
 };
+// The warp's next piece of its CTA's part; false: there is none.
+__device__ __forceinline__ bool tree_next(const TreeParams& p, TreeWalk& walk, TreePiece& x) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) walk.piece(p, x);
+  __syncwarp();
+  return x.count > 0;
+}
 
 // tree_ancestors for one warp: the tokens' own keys that `token` sees, as bits. A lane holds tokens lane and lane + 32.
 __device__ __forceinline__ unsigned long long tree_own_keys(const TreeParams& p, int b, int token) {
@@ -166,6 +226,11 @@ __device__ __forceinline__ unsigned long long tree_own_keys(const TreeParams& p,
   return of_token(anc, token);
 }
 
+// The mask of a token as bits, a word for 32 keys.
+__device__ __forceinline__ const uint32_t* tree_bits(const TreeParams& p, int b, int token) {
+  return p.bits + (int64_t(b) * p.bits_tokens + (p.bits_tokens == 1 ? 0 : token)) * p.bits_words;
+}
+
 // Where a row's result goes: bf16 into the output where its unit is whole, else fp32.
 struct TreeRowOut {
   __nv_bfloat16* out;
@@ -184,6 +249,7 @@ __device__ __noinline__ void tree_exact_row(const TreeParams& p, const TreePiece
   const int last = min((pc.first + pc.count) * TILE_N, pc.n_keys);
   for (int key = pc.first * TILE_N; key < last; ++key) {
     if (key >= pc.ctx && !((own >> (key - pc.ctx)) & 1ull)) continue;
+    if (p.bits != nullptr && !((tree_bits(p, pc.b, token)[key >> 5] >> (key & 31)) & 1u)) continue;
     const __nv_bfloat16* const k = p.k + pc.b * p.ks.sb + pc.hk * p.ks.sh + key * p.ks.ss;
     const __nv_bfloat16* const v = p.v + pc.b * p.vs.sb + pc.hk * p.vs.sh + key * p.vs.ss + col;
     float s = 0.f;
@@ -197,7 +263,7 @@ __device__ __noinline__ void tree_exact_row(const TreeParams& p, const TreePiece
   }
 }
 
-template <bool PAIR>
+template <bool PAIR, bool MASK>
 __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid_constant__ TreeUmmaParams p) {
   constexpr int RING = UMMA_RING, ROWS = UMMA_ROWS<PAIR>, COLS = PAIR ? HEAD_DIM : HEAD_DIM / 2;
   enum : int {
@@ -208,6 +274,8 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
   __shared__ uint64_t bars[N_BARS];
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
+  __shared__ TreeWalk walks[UMMA_THREADS / 32];
+  __shared__ TreePiece pieces[UMMA_THREADS / 32];
   __shared__ float2 row_ml[2][PAIR ? 1 : 2][PAIR ? 1 : TILE_M];     // [unit parity][stream][row]
   const TreeParams& t = p.t;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -233,9 +301,15 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
     ptx::tmem_relinquish();
   }
   if (warp == 8 && lane < 2) ptx::prefetch_tensormap(&p.maps[lane]);
+  cudaGridDependencySynchronize();                       // what is above ran beside the end of the kernel before this one
   cudaTriggerProgrammaticLaunchCompletion();             // the merge may be set up; it waits for this kernel's end by itself
-  TreeWalk walk(t, p.B, blockIdx.x, gridDim.x);
-  TreePiece pc;
+  TreeWalk& walk = walks[warp];
+  const TreePiece& pc = pieces[warp];
+  {
+    TreeWalk w;
+    w.start(t, p.B, blockIdx.x, gridDim.x);
+    if (lane == 0) walk = w;
+  }
   // Copies rows `first`, first + step, .. of a unit's queries, 16 threads a row; rows past the last become zeros.
   auto copy_queries = [&](const TreePiece& x, int first, int step) {
 #pragma unroll 4
@@ -269,7 +343,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
     const uint32_t p_addr = PAIR ? lane_addr + 128 + sx * 64 : s_addr;
     const uint32_t o_addr = lane_addr + 256 + sx * 128;
     uint32_t kt = 0, unit = 0, done[2] = {0, 0};          // tiles of this stream, units, units in which a stream had tiles
-    while (walk.piece(t, pc)) {
+    while (tree_next(t, walk, pieces[warp])) {
       if (unit == 0) {                                    // the first unit's queries: nobody else has as many hands free
         copy_queries(pc, 2 * warp + (lane >> 4), 16);
         if (lane == 0) ptx::mbar_arrive_at(bar(Q_FULL));
@@ -278,11 +352,14 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
       const bool valid = r < all_rows, busy = __any_sync(0xffffffffu, valid);
       const int token = fdiv(min(r, all_rows - 1), p.by_rep), head = pc.hk * rep + min(r, all_rows - 1) - token * rep;
       const unsigned long long own = (pc.first + pc.count) * TILE_N > pc.ctx ? tree_own_keys(t, pc.b, token) : 0ull;
+      const uint32_t* const mask_row = MASK ? tree_bits(t, pc.b, token) : nullptr;
       float m_run = -CUDART_INF_F, l_run = 0.f;
-      const int n_mine = PAIR ? pc.count : (pc.count + 1 - sx) / 2;
+      const int n_mine = PAIR ? pc.count : (pc.count + 1 - sx) / 2, tile0 = pc.first, ctx = pc.ctx;
 #pragma unroll 1
       for (int i = 0; i < n_mine; ++i, ++kt) {
-        const int key0 = (pc.first + (PAIR ? i : 2 * i + sx)) * TILE_N;
+        const int tile = tile0 + (PAIR ? i : 2 * i + sx), key0 = tile * TILE_N;
+        uint4 seen4 = make_uint4(~0u, ~0u, ~0u, ~0u);     // keys of the tile that the mask lets the row's token see
+        if (MASK) seen4 = reinterpret_cast<const uint4*>(mask_row)[tile];
         ok = TREE_WAIT(S_FULL + sx, kt, 11 + sx);
         if (!ok) break;
         ptx::tc_fence_after();
@@ -303,7 +380,8 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
         uint32_t* const su = reinterpret_cast<uint32_t*>(s);
         float tile_max;
         auto chunk_max = [&](int c) { return sm::row_max(*reinterpret_cast<const float(*)[32]>(&s[32 * c])); };
-        if (key0 + TILE_N <= pc.ctx) {                    // every token sees the whole tile
+        // does every token see the whole tile?
+        if (key0 + TILE_N <= ctx && (!MASK || __all_sync(0xffffffffu, (seen4.x & seen4.y & seen4.z & seen4.w) == ~0u))) {
           ptx::tmem_ld32(s_addr, su);
           ptx::tmem_wait_ld();
           ptx::tmem_ld32(s_addr + 32, su + 32);
@@ -333,8 +411,9 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
           tile_max = -CUDART_INF_F;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int at = key0 + 32 * c - pc.ctx;        // place of the chunk's first key among the tokens' own
-            const uint32_t seen = at >= 0 ? (at < 64 ? uint32_t(own >> at) : 0u) : at <= -32 ? ~0u : uint32_t(own << -at) | ((1u << -at) - 1u);
+            const int at = key0 + 32 * c - ctx;        // place of the chunk's first key among the tokens' own
+            const uint32_t mine = at >= 0 ? (at < 64 ? uint32_t(own >> at) : 0u) : at <= -32 ? ~0u : uint32_t(own << -at) | ((1u << -at) - 1u);
+            const uint32_t seen = mine & (c == 0 ? seen4.x : c == 1 ? seen4.y : c == 2 ? seen4.z : seen4.w);
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[32 * c + e] = (seen >> e) & 1u ? s[32 * c + e] : -CUDART_INF_F;
             tile_max = fmaxf(tile_max, chunk_max(c));
@@ -449,7 +528,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
       if (busy) {
         TreeRowOut dst = {t.o + ((int64_t(pc.b) * t.n + token) * t.H + head) * HEAD_DIM, nullptr, ROWS};
         if (pc.count != pc.of) {
-          float* const part = t.scratch + (int64_t(blockIdx.x) * 2 + (pc.first == 0 ? 1 : 0)) * UMMA_PARTIAL<PAIR>;
+          float* const part = t.scratch + (int64_t(blockIdx.x) * 2 + pc.starts) * UMMA_PARTIAL<PAIR>;
           const int at = r - pc.rg * ROWS;
           dst.part = part + at;
           if (valid && col == 0) reinterpret_cast<float2*>(part + int64_t(ROWS) * HEAD_DIM)[at] = make_float2(m, l);
@@ -490,11 +569,14 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
       ptx::mbar_arrive_at(bar(FULL + copied));
       copied = -1;
     };
-    auto request = [&](uint32_t req, int operand, const TreePiece& x, int tile) {
+    // `any`: keys of the tile that some token sees
+    struct Place { int b, hk, n_keys; };
+    auto request = [&](uint32_t req, int operand, const Place& x, int tile, const uint4& any) {
       const uint32_t slot = req % RING, dst = ring_smem + slot * TILE_BYTES;
       if (!(ok = TREE_WAIT(FREE + slot, req / RING - 1, 21 + operand))) return;
       const int key0 = tile * TILE_N;
-      if (p.use_tma && (key0 + TILE_N <= x.n_keys || x.n_keys == t.S)) {  // rows past the cache's end come as zeros
+      const bool all = (any.x & any.y & any.z & any.w) == ~0u;
+      if (p.use_tma && all && (key0 + TILE_N <= x.n_keys || x.n_keys == t.S)) {  // rows past the cache's end come as zeros
         if (copied >= 0) { ptx::cp_async_wait<0>(); report(); }
         if (lt == 0) {
           ptx::mbar_expect_tx_at(bar(FULL + slot), TILE_BYTES);
@@ -510,7 +592,8 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
 #pragma unroll 4
       for (int c = 0; c < TILE_N / 8; ++c) {
         const int row = c * 8 + (lt >> 4);
-        const bool there = key0 + row < x.n_keys;
+        const uint32_t word = c < 4 ? any.x : c < 8 ? any.y : c < 12 ? any.z : any.w;
+        const bool there = key0 + row < x.n_keys && ((word >> (row & 31)) & 1u);
         ptx::cp_async_16(dst + tile_offset(row, lt & 15), there ? src + (key0 + row) * st.ss : src, there ? 16u : 0u);
       }
       ptx::cp_async_commit();
@@ -519,17 +602,23 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
       copied = int(slot);
     };
     uint32_t j = 0;
-    TreePiece before;                                     // of the tile whose V is requested next
+    Place before = {0, 0, 0};                             // of the tile whose V is requested next
+    uint4 v_any = make_uint4(~0u, ~0u, ~0u, ~0u);
     int v_tile = -1;
-    while (ok && walk.piece(t, pc)) {
-      for (int i = 0; i < pc.count && ok; ++i, ++j) {
-        request(k_request(j), 0, pc, pc.first + i);
-        if (ok && v_tile >= 0) request(v_request(j - 1), 1, before, v_tile);
-        before = pc;
-        v_tile = pc.first + i;
+    while (ok && tree_next(t, walk, pieces[warp])) {
+      const Place here = {pc.b, pc.hk, pc.n_keys};
+      const int first = pc.first, count = pc.count;
+      for (int i = 0; i < count && ok; ++i, ++j) {
+        uint4 any = make_uint4(~0u, ~0u, ~0u, ~0u);
+        if (MASK) any = reinterpret_cast<const uint4*>(t.any + int64_t(here.b) * t.bits_words)[first + i];
+        request(k_request(j), 0, here, first + i, any);
+        if (ok && v_tile >= 0) request(v_request(j - 1), 1, before, v_tile, v_any);
+        before = here;
+        v_tile = first + i;
+        if (MASK) v_any = any;
       }
     }
-    if (ok && v_tile >= 0) request(v_request(j - 1), 1, before, v_tile);
+    if (ok && v_tile >= 0) request(v_request(j - 1), 1, before, v_tile, v_any);
     ptx::cp_async_wait<0>();
     if (copied >= 0) report();
   } else {
@@ -572,7 +661,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
       __syncwarp();
     };
     if (warp == 12 || (PAIR && warp == 13)) {
-      while (ok && walk.piece(t, pc)) {
+      while (ok && tree_next(t, walk, pieces[warp])) {
         const int count = pc.count;
         if (PAIR) {
 #pragma unroll 1
@@ -601,7 +690,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
       }
     } else if (warp >= 14) {
       // ================================ query rows ==================================================
-      while (ok && walk.piece(t, pc)) {
+      while (ok && tree_next(t, walk, pieces[warp])) {
         if (unit > 0) {
           ok = TREE_WAIT(Q_FREE, unit - 1, 23);
           if (!ok) break;
@@ -626,6 +715,47 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
   }
 }
 
+// A boolean mask as bits: per token a word for 32 keys, the same of the keys any token sees, and which tiles hold such keys (a
+// byte for eight). CTA: 32 words of one sequence, eight tokens at a time; the words are padded to whole tiles with zeros.
+constexpr int TREE_MASK_ROWS = 8;
+__global__ void __launch_bounds__(32 * TREE_MASK_ROWS) tree_mask_kernel(const __grid_constant__ TreeParams p) {
+  __shared__ uint32_t part[TREE_MASK_ROWS][32];
+  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5, b = blockIdx.y;
+  const int word = blockIdx.x * 32 + lane, key0 = word * 32;
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
+  uint32_t any = 0;
+  if (word < p.bits_words) {
+    for (int i = y; i < p.bits_tokens; i += TREE_MASK_ROWS) {
+      const uint8_t* const m = p.mask + b * p.mask_sb + i * p.mask_sn + key0 * p.mask_ss;
+      uint32_t bits = 0;
+      if (p.mask_vec && key0 + 32 <= p.S) {
+        const uint4 w[2] = {reinterpret_cast<const uint4*>(m)[0], reinterpret_cast<const uint4*>(m)[1]};
+        const uint32_t ws[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+        for (int c = 0; c < 8; ++c) bits |= ((__vminu4(ws[c], 0x01010101u) * 0x10204080u) >> 28) << (4 * c);      // a byte's 0 or not, four at a time
+      } else {
+        for (int c = 0; c < 32 && key0 + c < p.S; ++c) bits |= m[c * p.mask_ss] != 0 ? 1u << c : 0u;
+      }
+      const_cast<uint32_t*>(p.bits)[(int64_t(b) * p.bits_tokens + i) * p.bits_words + word] = bits;
+      any |= bits;
+    }
+  }
+  part[y][lane] = any;
+  __syncthreads();
+  if (y != 0) return;
+#pragma unroll
+  for (int i = 1; i < TREE_MASK_ROWS; ++i) any |= part[i][lane];
+  if (word < p.bits_words) const_cast<uint32_t*>(p.any)[int64_t(b) * p.bits_words + word] = any;
+  const uint32_t words = __ballot_sync(0xffffffffu, any != 0u);
+  if (lane == 0) {
+    uint32_t tiles = 0;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) tiles |= (words >> (4 * c)) & 15u ? 1u << c : 0u;
+    const_cast<uint8_t*>(p.live)[int64_t(b) * p.live_words * 8 + blockIdx.x] = uint8_t(tiles);
+  }
+}
+
 // Joins the partial results of units that several CTAs had a part of. A thread has UMMA_MERGE_COLS columns of a row, a
 // warp 32 rows. Loads of rows that do not exist stay inside the buffer and are not used.
 constexpr int UMMA_MERGE_COLS = 4, UMMA_MERGE_WARPS = 4;
@@ -642,19 +772,11 @@ __global__ void __launch_bounds__(32 * UMMA_MERGE_WARPS) tree_umma_merge_kernel(
   const int at = block / UMMA_MERGE_SPLIT * 32 + lane, row = rg * ROWS + at;
   const int col = (block % UMMA_MERGE_SPLIT * UMMA_MERGE_WARPS + (threadIdx.x >> 5)) * UMMA_MERGE_COLS;
   if (row - lane >= t.n * rep) return;                    // no such rows
-  uint32_t total = 0, start = 0;                          // tiles of all units, and before this one
-  for (int s = lane; s < p.B; s += 32) {
-    const uint32_t n = uint32_t(tree_tiles(t, s)) * units;
-    total += n;
-    start += s < b ? n : 0u;
-  }
-  total = __reduce_add_sync(0xffffffffu, total);
-  start = __reduce_add_sync(0xffffffffu, start);
-  uint32_t per = (total + grid - 1) / grid;
-  per = per < UMMA_MIN_TILES ? UMMA_MIN_TILES : per;
+  uint32_t start;
+  const TreeList list(t, p.B, grid, b, &start);
   const int tiles = tree_tiles(t, b);
-  start += uint32_t(in_b) * tiles;
-  const int c0 = int(start / per), c1 = int((start + tiles - 1) / per);
+  start += uint32_t(in_b) * (tiles + list.cost) + list.cost;       // place of the unit's first tile
+  const int c0 = int(start / list.per), c1 = int((start + tiles - 1) / list.per);
   cudaGridDependencySynchronize();                        // everything before this ran beside the main kernel's end
   if (c0 == c1) return;                                   // one CTA held the unit and wrote its rows
   // The part in the CTA the unit begins in is that CTA's second slot, in the others the first.
