@@ -47,10 +47,12 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_rows_kernel(const __grid_co
 }
 
 // ---- eviction -----------------------------------------------------------------------------------------------
-constexpr int EVICT_THREADS = 1024;
+constexpr int EVICT_THREADS = 512;
 constexpr int EVICT_WARPS = EVICT_THREADS / 32;
 constexpr int EVICT_MAX_CLUSTER = 8;
 constexpr int EVICT_SMEM_KEYS = 48 * 1024;       // order keys one CTA holds in shared memory; longer parts are read again
+constexpr int EVICT_DIGITS = 3;                  // of 11, 11 and 10 bits: the first one tells weights of one power of two apart
+constexpr int EVICT_BINS = 2048;
 
 struct EvictParams {
   const __nv_bfloat16* k;      // (B, S, Hkv, 128) by strides
@@ -64,11 +66,10 @@ struct EvictParams {
   TensorView ks, vs, k2s, v2s;
   int64_t weights_sb, weights_sh, weights2_sb, weights2_sh;
   int S, Hkv, keep, recent;
-  int cluster, part;           // CTAs per (batch, head), keys per CTA
-  int in_smem;                 // a CTA's part fits EVICT_SMEM_KEYS
+  int cluster;                 // CTAs per (batch, head)
 };
 
-// Weights as unsigned numbers of the same order; both zeros are equal, NaN is above everything.
+// Weights as unsigned numbers of the same order; both zeros are equal, NaN is above everything. Never zero, which pads.
 __device__ __forceinline__ uint32_t order_key(float w) {
   if (w != w) return 0xffffffffu;
   const uint32_t bits = __float_as_uint(w + 0.f);
@@ -77,12 +78,15 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 
 // Picks the rows of one (batch, head) that stay: the last `recent` in use and the heaviest of the others, ties to the
 // lowest row, `keep` in all. A cluster holds the weights, a contiguous part per CTA, a contiguous part of that per
-// warp. The weight of the last row that stays is found digit by digit, eight bits at a time, from histograms that are
-// summed over the cluster; then one pass numbers the rows that stay.
-__global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(const __grid_constant__ EvictParams p) {
+// warp. The weight of the last row that stays is found digit by digit from histograms that are summed over the cluster
+// (one buffer per digit, so that each takes one barrier); then one pass numbers the rows that stay. What bounds it is
+// the chain of these steps. 16 x 8 heads of 1600 to 16384 keys: 44 us with digits of 8 bits, warps that add up equal
+// digits first (match) and 1024 threads, 14 us so.
+template <bool IN_SMEM>
+__global__ void __launch_bounds__(EVICT_THREADS, 2) evict_select_kernel(const __grid_constant__ EvictParams p) {
   namespace cg = cooperative_groups;
-  extern __shared__ uint32_t evict_keys[];
-  __shared__ int hist[256], total[256];
+  extern __shared__ __align__(16) uint32_t evict_keys[];
+  __shared__ int hist[EVICT_DIGITS][EVICT_BINS];
   __shared__ int warp_above[EVICT_WARPS], warp_ties[EVICT_WARPS];
   __shared__ int cta_above, cta_ties;
   __shared__ int digit_s, need_s;
@@ -90,6 +94,9 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(const __gri
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x % p.cluster, u = blockIdx.x / p.cluster;
   const int hk = u % p.Hkv, b = u / p.Hkv;
+  for (int i = tid; i < EVICT_DIGITS * EVICT_BINS; i += EVICT_THREADS) hist[0][i] = 0;
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
   const int used = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   const float* const w = p.weights + b * p.weights_sb + hk * p.weights_sh;
   int* const kept = p.kept + int64_t(u) * p.keep;
@@ -104,68 +111,103 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(const __gri
   }
   const int old = used - p.recent;                                 // rows that have to earn their place
   int need = p.keep - p.recent;                                    // how many of them stay; less than old
-  const int begin = int(int64_t(rank) * p.part < old ? int64_t(rank) * p.part : old);
-  const int end = min(old - begin, p.part) + begin;
-  if (p.in_smem)
-    for (int i = begin + tid; i < end; i += EVICT_THREADS) evict_keys[i - begin] = order_key(w[i]);
-  auto key_at = [&](int i) { return p.in_smem ? evict_keys[i - begin] : order_key(w[i]); };
+  const int part = ((old + p.cluster - 1) / p.cluster + 3) & ~3;
+  const int begin = int(min(int64_t(rank) * part, int64_t(old))), n = min(part, old - begin);
+  const float* const mine_w = w + begin;
+  const int n4 = (n + 3) >> 2;
+  auto four = [&](int v) {                                         // order keys 4 v .. of this CTA, zeros behind the last
+    if constexpr (IN_SMEM) {
+      return reinterpret_cast<const uint4*>(evict_keys)[v];
+    } else {
+      uint32_t k[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) k[e] = 4 * v + e < n ? order_key(mine_w[4 * v + e]) : 0u;
+      return make_uint4(k[0], k[1], k[2], k[3]);
+    }
+  };
+  __syncthreads();
+  if (IN_SMEM) {                                                   // the first digit on the way
+    constexpr int AT_ONCE = 16;                                    // loads under way together, before any is added up
+    for (int i0 = tid; i0 < n; i0 += AT_ONCE * EVICT_THREADS) {
+      float x[AT_ONCE];
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) x[e] = i0 + e * EVICT_THREADS < n ? mine_w[i0 + e * EVICT_THREADS] : 0.f;
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) {
+        const int i = i0 + e * EVICT_THREADS;
+        if (i >= n) break;
+        const uint32_t key = order_key(x[e]);
+        evict_keys[i] = key;
+        atomicAdd(&hist[0][key >> 21], 1);
+      }
+    }
+    if (tid < 4 * n4 - n) evict_keys[n + tid] = 0u;
+  }
 
   uint32_t prefix = 0, mask = 0;                                   // digits of the last kept row's key found so far
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int i0 = begin + warp * 32; i0 < end; i0 += EVICT_THREADS) {
-      const int i = i0 + lane;
-      const uint32_t key = i < end ? key_at(i) : 0u;
-      const bool in = i < end && (key & mask) == prefix;
-      const uint32_t digit = in ? (key >> shift) & 255u : 256u;
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);  // one addition per digit of a warp
-      if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+#pragma unroll 1
+  for (int d = 0; d < EVICT_DIGITS; ++d) {
+    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
+    const uint32_t digits = d == 2 ? 1023u : 2047u;
+    if (!IN_SMEM || d > 0) {
+#pragma unroll 2
+      for (int v = tid; v < n4; v += EVICT_THREADS) {
+        const uint4 x = four(v);
+        if ((x.x & mask) == prefix && (d > 0 || x.x)) atomicAdd(&hist[d][(x.x >> shift) & digits], 1);
+        if ((x.y & mask) == prefix && (d > 0 || x.y)) atomicAdd(&hist[d][(x.y >> shift) & digits], 1);
+        if ((x.z & mask) == prefix && (d > 0 || x.z)) atomicAdd(&hist[d][(x.z >> shift) & digits], 1);
+        if ((x.w & mask) == prefix && (d > 0 || x.w)) atomicAdd(&hist[d][(x.w >> shift) & digits], 1);
+      }
     }
     cluster.sync();
-    if (tid < 256) {
-      int sum = 0;
-      for (int c = 0; c < p.cluster; ++c) sum += *cluster.map_shared_rank(&hist[tid], c);
-      total[tid] = sum;
+    // The digit at which `need` rows are reached from above: thread t has the bins 2047 - 4 t and the three below.
+    int bins[4] = {0, 0, 0, 0};
+    for (int c = 0; c < p.cluster; ++c) {
+      const int4 x = *reinterpret_cast<const int4*>(cluster.map_shared_rank(&hist[d][EVICT_BINS - 4 - 4 * tid], c));
+      bins[0] += x.w; bins[1] += x.z; bins[2] += x.y; bins[3] += x.x;
+    }
+    const int mine = bins[0] + bins[1] + bins[2] + bins[3];
+    int above = mine;
+#pragma unroll
+    for (int k = 1; k < 32; k *= 2) {
+      const int y = __shfl_up_sync(0xffffffffu, above, k);
+      if (lane >= k) above += y;
+    }
+    if (lane == 31) warp_above[warp] = above;
+    if (tid == 0) { digit_s = int(digits); need_s = 0; }           // nothing to find where no row is needed
+    __syncthreads();
+    above -= mine;
+    for (int k = 0; k < warp; ++k) above += warp_above[k];
+    if (above < need && above + mine >= need) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (above < need && above + bins[k] >= need) { digit_s = EVICT_BINS - 1 - (4 * tid + k); need_s = need - above; }
+        above += bins[k];
+      }
     }
     __syncthreads();
-    if (warp == 0) {                                               // the digit at which `need` rows are reached from above
-      int mine[8], sum = 0;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) sum += mine[c] = total[255 - (lane * 8 + c)];
-      int above = sum;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int y = __shfl_up_sync(0xffffffffu, above, d);
-        if (lane >= d) above += y;
-      }
-      above -= sum;
-      if (above < need && above + sum >= need) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          if (above < need && above + mine[c] >= need) { digit_s = 255 - (lane * 8 + c); need_s = need - above; }
-          above += mine[c];
-        }
-      }
-      if (need == 0 && lane == 0) { digit_s = 255; need_s = 0; }
-    }
-    cluster.sync();                                                // histograms are free again, digit and need are there
     prefix |= uint32_t(digit_s) << shift;
-    mask |= 255u << shift;
+    mask |= digits << shift;
     need = need_s;
     __syncthreads();
   }
   // `need` rows of key `prefix` stay, the lowest ones, and all above it (none, where nothing had to be found)
   const bool none = p.keep == p.recent;
-  const int warp_part = (p.part + EVICT_WARPS - 1) / EVICT_WARPS;
-  const int wb = min(begin + warp * warp_part, end), we = min(wb + warp_part, end);
+  const int warp_part = (n4 + EVICT_WARPS - 1) / EVICT_WARPS;
+  const int wb = min(warp * warp_part, n4), we = min(wb + warp_part, n4);
+  // rows above and ties of four keys, in the halves of a word
+  auto count = [&](const uint4& x) {
+    return (x.x > prefix) + (x.y > prefix) + (x.z > prefix) + (x.w > prefix) +
+           (((x.x == prefix) + (x.y == prefix) + (x.z == prefix) + (x.w == prefix)) << 16);
+  };
   int above = 0, ties = 0;
-  for (int i0 = wb; i0 < we; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t key = i < we ? key_at(i) : 0u;
-    above += __popc(__ballot_sync(0xffffffffu, i < we && !none && key > prefix));
-    ties += __popc(__ballot_sync(0xffffffffu, i < we && !none && key == prefix));
+  for (int v = wb + lane; v < we; v += 32) {
+    const int x = count(four(v));
+    above += x & 0xffff;
+    ties += x >> 16;
   }
+  above = __reduce_add_sync(0xffffffffu, above);
+  ties = __reduce_add_sync(0xffffffffu, ties);
   if (lane == 0) { warp_above[warp] = above; warp_ties[warp] = ties; }
   __syncthreads();
   if (tid == 0) {
@@ -181,20 +223,31 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(const __gri
     ties += *cluster.map_shared_rank(&cta_ties, c);
   }
   for (int c = 0; c < warp; ++c) { above += warp_above[c]; ties += warp_ties[c]; }
-  const uint32_t lower = (1u << lane) - 1u;
-  for (int i0 = wb; i0 < we; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t key = i < we ? key_at(i) : 0u;
-    const bool is_above = i < we && !none && key > prefix, is_tie = i < we && !none && key == prefix;
-    const uint32_t va = __ballot_sync(0xffffffffu, is_above), vt = __ballot_sync(0xffffffffu, is_tie);
-    const int tie = ties + __popc(vt & lower);
-    if (is_above || (is_tie && tie < need)) {
-      const int at = above + __popc(va & lower) + min(tie, need);
-      kept[at] = i;
-      w2[at] = w[i];
+  for (int v0 = wb; v0 < we && !none; v0 += 32) {
+    const uint4 x = v0 + lane < we ? four(v0 + lane) : make_uint4(0u, 0u, 0u, 0u);
+    const int own = count(x);
+    int upto = own;
+#pragma unroll
+    for (int k = 1; k < 32; k *= 2) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, k);
+      if (lane >= k) upto += y;
     }
-    above += __popc(va);
-    ties += __popc(vt);
+    int a = above + ((upto - own) & 0xffff), t = ties + ((upto - own) >> 16);
+    const uint32_t keys[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool is_above = keys[e] > prefix, is_tie = keys[e] == prefix;
+      if (is_above || (is_tie && t < need)) {
+        const int at = a + min(t, need), i = 4 * (v0 + lane) + e;
+        kept[at] = begin + i;
+        w2[at] = mine_w[i];
+      }
+      a += is_above;
+      t += is_tie;
+    }
+    upto = __shfl_sync(0xffffffffu, upto, 31);
+    above += upto & 0xffff;
+    ties += upto >> 16;
   }
   for (int i = rank * EVICT_THREADS + tid; i < p.recent; i += p.cluster * EVICT_THREADS) {
     kept[p.keep - p.recent + i] = old + i;
@@ -218,6 +271,7 @@ __global__ void __launch_bounds__(EVICT_COPY_THREADS) evict_copy_kernel(const __
   uint4* const k2 = reinterpret_cast<uint4*>(p.k2 + b * p.k2s.sb + hk * p.k2s.sh) + piece;
   uint4* const v2 = reinterpret_cast<uint4*>(p.v2 + b * p.v2s.sb + hk * p.v2s.sh) + piece;
   const int* const kept = p.kept + int64_t(u) * p.keep;
+  cudaGridDependencySynchronize();
   uint4 kw[EVICT_ROWS], vw[EVICT_ROWS];
 #pragma unroll
   for (int c = 0; c < EVICT_ROWS; ++c) {

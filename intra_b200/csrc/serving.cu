@@ -47,7 +47,7 @@ void init_serving(int device) {
   void* word = nullptr;
   if (e == cudaSuccess) e = cudaGetSymbolAddress(&word, g_serving_status);
   st.status_word = static_cast<int*>(word);
-  if (e == cudaSuccess) e = opt_in_smem(evict_select_kernel, EVICT_SMEM_KEYS * 4);
+  if (e == cudaSuccess) e = opt_in_smem(evict_select_kernel<true>, EVICT_SMEM_KEYS * 4);
   if (e != cudaSuccess) st.init_status = cuda_fail(e);
 }
 
@@ -64,17 +64,20 @@ TensorView view_of(const int64_t s[3]) { return {s[0], s[1], s[2]}; }
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 template <typename K, typename P>
-cudaError_t launch_cluster(K kernel, int64_t clusters, int cluster, int threads, int smem, cudaStream_t stream, const P& p) {
+cudaError_t launch_cluster(K kernel, int64_t clusters, int cluster, int threads, int smem, cudaStream_t stream, const P& p,
+                           int early = 0) {
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim = {unsigned(cluster), 1, 1};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {unsigned(cluster), 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = early;
   cfg.gridDim = dim3(unsigned(clusters * cluster));
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
@@ -345,14 +348,11 @@ int intra_b200_evict(const void* k, const void* v, const float* weights, const i
   while (c < EVICT_MAX_CLUSTER && units * 2 * c <= 2 * st->sm_count && S >= 2048 * c) c *= 2;
   while (c < EVICT_MAX_CLUSTER && ceil_div(S, c) > EVICT_SMEM_KEYS) c *= 2;
   p.cluster = c;
-  p.part = ceil_div(S, c);
-  p.in_smem = p.part <= EVICT_SMEM_KEYS;
+  const int part = (ceil_div(S, c) + 3) & ~3;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  cudaError_t e = launch_cluster(evict_select_kernel, units, c, EVICT_THREADS, p.in_smem ? p.part * 4 : 0, stream, p);
-  if (e == cudaSuccess) {
-    evict_copy_kernel<<<unsigned(copies), EVICT_COPY_THREADS, 0, stream>>>(p);
-    e = cudaGetLastError();
-  }
+  cudaError_t e = part <= EVICT_SMEM_KEYS ? launch_cluster(evict_select_kernel<true>, units, c, EVICT_THREADS, part * 4, stream, p, 1)
+                                          : launch_cluster(evict_select_kernel<false>, units, c, EVICT_THREADS, 0, stream, p, 1);
+  if (e == cudaSuccess) e = launch_early(evict_copy_kernel, dim3(unsigned(copies)), EVICT_COPY_THREADS, 0, stream, p);
   return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
 }
 
