@@ -76,19 +76,22 @@ __device__ __forceinline__ uint32_t order_key(float w) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+// The weight an order key stands for (minus zero as zero).
+__device__ __forceinline__ float weight_of_key(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+
 // Picks the rows of one (batch, head) that stay: the last `recent` in use and the heaviest of the others, ties to the
 // lowest row, `keep` in all. A cluster holds the weights, a contiguous part per CTA, a contiguous part of that per
 // warp. The weight of the last row that stays is found digit by digit from histograms that are summed over the cluster
 // (one buffer per digit, so that each takes one barrier); then one pass numbers the rows that stay. What bounds it is
 // the chain of these steps. 16 x 8 heads of 1600 to 16384 keys: 44 us with digits of 8 bits, warps that add up equal
-// digits first (match) and 1024 threads, 14 us so.
+// digits first (match) and 1024 threads, 17 us so.
 template <bool IN_SMEM>
 __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_select_kernel(const __grid_constant__ EvictParams p) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint32_t evict_keys[];
   __shared__ int hist[EVICT_DIGITS][EVICT_BINS];
   __shared__ int warp_above[EVICT_WARPS], warp_ties[EVICT_WARPS];
-  __shared__ int cta_above, cta_ties;
+  __shared__ int2 cta_counts;                                      // rows above and ties, read by the cluster
   __shared__ int digit_s, need_s;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -125,6 +128,10 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_select_kernel(const __
       return make_uint4(k[0], k[1], k[2], k[3]);
     }
   };
+  auto sync_all = [&] {
+    if (p.cluster == 1) __syncthreads();
+    else cluster.sync();
+  };
   __syncthreads();
   if (IN_SMEM) {                                                   // the first digit on the way
     constexpr int AT_ONCE = 16;                                    // loads under way together, before any is added up
@@ -159,13 +166,16 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_select_kernel(const __
         if ((x.w & mask) == prefix && (d > 0 || x.w)) atomicAdd(&hist[d][(x.w >> shift) & digits], 1);
       }
     }
-    cluster.sync();
+    sync_all();
     // The digit at which `need` rows are reached from above: thread t has the bins 2047 - 4 t and the three below.
+    int* const my_bins = &hist[d][EVICT_BINS - 4 - 4 * tid];
+    int4 x[EVICT_MAX_CLUSTER];
+#pragma unroll
+    for (int c = 0; c < EVICT_MAX_CLUSTER; ++c)
+      x[c] = c >= p.cluster ? make_int4(0, 0, 0, 0) : p.cluster == 1 ? *reinterpret_cast<const int4*>(my_bins) : *reinterpret_cast<const int4*>(cluster.map_shared_rank(my_bins, c));
     int bins[4] = {0, 0, 0, 0};
-    for (int c = 0; c < p.cluster; ++c) {
-      const int4 x = *reinterpret_cast<const int4*>(cluster.map_shared_rank(&hist[d][EVICT_BINS - 4 - 4 * tid], c));
-      bins[0] += x.w; bins[1] += x.z; bins[2] += x.y; bins[3] += x.x;
-    }
+#pragma unroll
+    for (int c = 0; c < EVICT_MAX_CLUSTER; ++c) { bins[0] += x[c].w; bins[1] += x[c].z; bins[2] += x[c].y; bins[3] += x[c].x; }
     const int mine = bins[0] + bins[1] + bins[2] + bins[3];
     int above = mine;
 #pragma unroll
@@ -210,19 +220,24 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_select_kernel(const __
   ties = __reduce_add_sync(0xffffffffu, ties);
   if (lane == 0) { warp_above[warp] = above; warp_ties[warp] = ties; }
   __syncthreads();
-  if (tid == 0) {
-    int a = 0, t = 0;
-    for (int c = 0; c < EVICT_WARPS; ++c) { a += warp_above[c]; t += warp_ties[c]; }
-    cta_above = a;
-    cta_ties = t;
+  above = lane < warp ? warp_above[lane] : 0;                      // of the warps before this one
+  ties = lane < warp ? warp_ties[lane] : 0;
+  if (p.cluster > 1) {
+    if (warp == 0) {
+      const int a = __reduce_add_sync(0xffffffffu, lane < EVICT_WARPS ? warp_above[lane] : 0);
+      const int t = __reduce_add_sync(0xffffffffu, lane < EVICT_WARPS ? warp_ties[lane] : 0);
+      if (lane == 0) cta_counts = make_int2(a, t);
+    }
+    cluster.sync();
+    if (lane < rank) {                                             // and of the CTAs before
+      const int2 x = *cluster.map_shared_rank(&cta_counts, lane);
+      above += x.x;
+      ties += x.y;
+    }
+    cluster.barrier_arrive();                                      // the last this CTA reads elsewhere
   }
-  cluster.sync();
-  above = ties = 0;
-  for (int c = 0; c < rank; ++c) {
-    above += *cluster.map_shared_rank(&cta_above, c);
-    ties += *cluster.map_shared_rank(&cta_ties, c);
-  }
-  for (int c = 0; c < warp; ++c) { above += warp_above[c]; ties += warp_ties[c]; }
+  above = __reduce_add_sync(0xffffffffu, above);
+  ties = __reduce_add_sync(0xffffffffu, ties);
   for (int v0 = wb; v0 < we && !none; v0 += 32) {
     const uint4 x = v0 + lane < we ? four(v0 + lane) : make_uint4(0u, 0u, 0u, 0u);
     const int own = count(x);
@@ -240,7 +255,7 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_select_kernel(const __
       if (is_above || (is_tie && t < need)) {
         const int at = a + min(t, need), i = 4 * (v0 + lane) + e;
         kept[at] = begin + i;
-        w2[at] = mine_w[i];
+        w2[at] = IN_SMEM ? weight_of_key(keys[e]) : mine_w[i];
       }
       a += is_above;
       t += is_tie;
@@ -253,10 +268,12 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_select_kernel(const __
     kept[p.keep - p.recent + i] = old + i;
     w2[p.keep - p.recent + i] = w[old + i];
   }
-  cluster.sync();                                                  // nobody leaves while its counts are read
+  if (p.cluster > 1) cluster.barrier_wait();                       // nobody leaves while its counts are read
 }
 
 // Rows of K and V into their new places. Sixteen threads a row, EVICT_ROWS rows each; rows that do not exist become zeros.
+// It runs at the copy bandwidth: 128 x 2048 rows 42 us, 6.4 TB/s read and written. (Copied by the selection's CTAs, each
+// the rows it has numbered, beside other units' selection, the whole call took 61 us instead of 59: too few loads under way.)
 constexpr int EVICT_COPY_THREADS = 256;
 constexpr int EVICT_ROWS = 2;
 __global__ void __launch_bounds__(EVICT_COPY_THREADS) evict_copy_kernel(const __grid_constant__ EvictParams p) {

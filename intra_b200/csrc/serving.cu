@@ -345,7 +345,7 @@ int intra_b200_evict(const void* k, const void* v, const float* weights, const i
   p.weights2_sb = weights_out_strides[0]; p.weights2_sh = weights_out_strides[1];
   p.S = S; p.Hkv = Hkv; p.keep = keep; p.recent = recent;
   int c = 1;
-  while (c < EVICT_MAX_CLUSTER && units * 2 * c <= 2 * st->sm_count && S >= 2048 * c) c *= 2;
+  while (c < EVICT_MAX_CLUSTER && units * 2 * c <= 2 * st->sm_count && S > 6144 * c) c *= 2;
   while (c < EVICT_MAX_CLUSTER && ceil_div(S, c) > EVICT_SMEM_KEYS) c *= 2;
   p.cluster = c;
   const int part = (ceil_div(S, c) + 3) & ~3;
