@@ -405,10 +405,8 @@ void init_decode(int device) {
   if (e != cudaSuccess) { st.init_status = cuda_fail(e); return; }
   if (major != 10) { st.init_status = INTRA_ERR_DEVICE; return; }
   e = cudaDeviceGetAttribute(&st.sm_count, cudaDevAttrMultiProcessorCount, device);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) e = opt_in_smem(decode_kernel<false>, DEC_SMEM_BYTES);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_kernel<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) e = opt_in_smem(decode_kernel<true>, DEC_SMEM_BYTES);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = opt_in_smem(decode_kernel, DEC_SMEM_BYTES);
   if (e != cudaSuccess) { st.init_status = cuda_fail(e); return; }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr;
@@ -420,7 +418,7 @@ void init_decode(int device) {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   int placed = 0;
-  if (cudaOccupancyMaxActiveClusters(&placed, decode_kernel<true>, &cfg) == cudaSuccess && placed >= 8) st.max_cluster = 16;
+  if (cudaOccupancyMaxActiveClusters(&placed, decode_kernel, &cfg) == cudaSuccess && placed >= 8) st.max_cluster = 16;
   else cudaGetLastError();        // not an error of the call: the portable size will do
 }
 
@@ -449,46 +447,6 @@ void plan_decode(int64_t units, int S, int sm_count, int max_cluster, int* clust
   *n_clusters = n;
 }
 
-// Plans and launches a decode step whose parameters are filled but for the split. With weights to accumulate the
-// scratch buffer also holds every head's statistics and the scores, in this order behind the clusters' partial results.
-template <bool ACCUMULATE>
-int launch_decode(DecodeParams& p, int B, const DecodeState& st, int64_t scratch_bytes, int64_t* scratch_needed, cudaStream_t stream) {
-  const int64_t units = int64_t(B) * p.Hkv * p.head_groups;
-  plan_decode(units, p.S, st.sm_count, st.max_cluster, &p.cluster, &p.n_clusters);
-  const int64_t clusters = units * p.n_clusters;
-  if (clusters * p.cluster > 0x7fffffffLL || int64_t(B) * p.H > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
-  int64_t floats = p.n_clusters > 1 ? clusters * DEC_PARTIAL : 0;
-  if (ACCUMULATE) {
-    if (int64_t(B) * p.Hkv > 65535) return INTRA_ERR_UNSUPPORTED;      // grid.y of the accumulation
-    p.stats = reinterpret_cast<float2*>(p.scratch + floats);
-    p.scores = p.scratch + floats + 2 * int64_t(B) * p.H;
-    floats += 2 * int64_t(B) * p.H + units * p.S * p.score_heads;
-  }
-  *scratch_needed = floats * int64_t(sizeof(float));
-  if (*scratch_needed > 0 && (!p.scratch || scratch_bytes < *scratch_needed)) return INTRA_NEED_SCRATCH;
-
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim = {unsigned(p.cluster), 1, 1};
-  cfg.gridDim = dim3(unsigned(clusters * p.cluster));
-  cfg.blockDim = dim3(DEC_THREADS);
-  cfg.dynamicSmemBytes = DEC_SMEM_BYTES;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel<ACCUMULATE>, p);
-  if (e == cudaSuccess && p.n_clusters > 1) {
-    decode_merge_kernel<ACCUMULATE><<<unsigned(B) * unsigned(p.H), HEAD_DIM, 0, stream>>>(p);
-    e = cudaGetLastError();
-  }
-  if (ACCUMULATE && e == cudaSuccess) {
-    decode_weights_kernel<<<dim3(ceil_div(p.S, DEC_WEIGHT_THREADS), unsigned(B * p.Hkv)), DEC_WEIGHT_THREADS, 0, stream>>>(p);
-    e = cudaGetLastError();
-  }
-  return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
-}
-
 }  // namespace
 
 extern "C" {
@@ -511,7 +469,7 @@ int intra_b200_decode(const void* q, const void* k, const void* v, const void* m
   std::call_once(st.once, init_decode, device);
   if (st.init_status != INTRA_OK) return st.init_status;
 
-  DecodeParams p = {};
+  DecodeParams p;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.k = static_cast<const __nv_bfloat16*>(k);
   p.v = static_cast<const __nv_bfloat16*>(v);
@@ -526,48 +484,29 @@ int intra_b200_decode(const void* q, const void* k, const void* v, const void* m
   p.S = S; p.H = H; p.Hkv = Hkv;
   p.head_groups = ceil_div(H / Hkv, DEC_HEADS);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  return launch_decode<false>(p, B, st, scratch_bytes, scratch_needed, static_cast<cudaStream_t>(cuda_stream));
-}
+  const int64_t units = int64_t(B) * Hkv * p.head_groups;
+  plan_decode(units, S, st.sm_count, st.max_cluster, &p.cluster, &p.n_clusters);
+  const int64_t clusters = units * p.n_clusters;
+  if (clusters * p.cluster > 0x7fffffffLL || int64_t(B) * H > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
+  *scratch_needed = p.n_clusters > 1 ? clusters * DEC_PARTIAL * int64_t(sizeof(float)) : 0;
+  if (*scratch_needed > 0 && (!scratch || scratch_bytes < *scratch_needed)) return INTRA_NEED_SCRATCH;
 
-int intra_b200_decode_accumulate(const void* q, const void* k, const void* v, const void* mask, const int* lengths, void* out,
-                                 float* weights, void* scratch, int64_t scratch_bytes, int64_t* scratch_needed, int B, int S,
-                                 int H, int Hkv, const int64_t q_strides[3], const int64_t k_strides[3],
-                                 const int64_t v_strides[3], const int64_t mask_strides[2], int64_t weights_batch_stride,
-                                 int64_t weights_head_stride, float softmax_scale, int device, void* cuda_stream) {
-  if (!q || !k || !v || !out || !weights || !scratch_needed || !q_strides || !k_strides || !v_strides || (mask && !mask_strides) ||
-      B <= 0 || S <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || !(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
-    return INTRA_ERR_BAD_ARG;
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(scratch) || !strides_ok(q_strides) ||
-      !strides_ok(k_strides) || !strides_ok(v_strides) || reinterpret_cast<uintptr_t>(weights) % 4 || reinterpret_cast<uintptr_t>(lengths) % 4)
-    return INTRA_ERR_ALIGNMENT;
-  if ((B > 1 && weights_batch_stride <= 0) || (Hkv > 1 && weights_head_stride <= 0)) return INTRA_ERR_BAD_ARG;
-  if (device < 0 || device >= MAX_DEVICES) return INTRA_ERR_BAD_ARG;
-  DeviceGuard guard(device);
-  if (!guard.ok) return cuda_fail(cudaGetLastError());
-  DecodeState& st = g_decode[device];
-  std::call_once(st.once, init_decode, device);
-  if (st.init_status != INTRA_OK) return st.init_status;
-
-  DecodeParams p = {};
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k = static_cast<const __nv_bfloat16*>(k);
-  p.v = static_cast<const __nv_bfloat16*>(v);
-  p.mask = static_cast<const uint8_t*>(mask);
-  p.lengths = lengths;
-  p.o = static_cast<__nv_bfloat16*>(out);
-  p.weights = weights;
-  p.weights_sb = weights_batch_stride; p.weights_sh = weights_head_stride;
-  p.scratch = static_cast<float*>(scratch);
-  p.q_sb = q_strides[0]; p.q_sh = q_strides[2];
-  p.ks = {k_strides[0], k_strides[1], k_strides[2]};
-  p.vs = {v_strides[0], v_strides[1], v_strides[2]};
-  if (mask) { p.mask_sb = mask_strides[0]; p.mask_ss = mask_strides[1]; }
-  p.mask_vec = mask && p.mask_ss == 1 && aligned16(mask) && p.mask_sb % 16 == 0;
-  p.S = S; p.H = H; p.Hkv = Hkv;
-  p.head_groups = ceil_div(H / Hkv, DEC_HEADS);
-  p.score_heads = imin(H / Hkv, DEC_HEADS);
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  return launch_decode<true>(p, B, st, scratch_bytes, scratch_needed, static_cast<cudaStream_t>(cuda_stream));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {unsigned(p.cluster), 1, 1};
+  cfg.gridDim = dim3(unsigned(clusters * p.cluster));
+  cfg.blockDim = dim3(DEC_THREADS);
+  cfg.dynamicSmemBytes = DEC_SMEM_BYTES;
+  cfg.stream = static_cast<cudaStream_t>(cuda_stream);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel, p);
+  if (e == cudaSuccess && p.n_clusters > 1) {
+    decode_merge_kernel<<<unsigned(B) * unsigned(H), HEAD_DIM, 0, cfg.stream>>>(p);
+    e = cudaGetLastError();
+  }
+  return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
 }
 
 int intra_b200_fwd_llm(const void* q, const void* k, const void* v, void* out, int B, int S, int H, int Hkv,

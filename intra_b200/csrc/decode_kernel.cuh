@@ -56,12 +56,6 @@ struct DecodeParams {
   const uint8_t* mask;         // (B, S) by strides, nonzero = visible; null: every key is
   __nv_bfloat16* o;            // (B, H, 128) contiguous
   float* scratch;              // n_clusters > 1: DEC_PARTIAL floats per cluster
-  const int* lengths;          // ACCUMULATE: keys before the token's own per sequence, null: S - 1
-  float* weights;              // ACCUMULATE: (B, Hkv, S) by strides, unit stride over keys
-  int64_t weights_sb, weights_sh;
-  float* scores;               // ACCUMULATE: of every visible key, [unit][key][score_heads], times scale_log2
-  float2* stats;               // ACCUMULATE: (B, H) maximum and inverse sum of each head's probabilities
-  int score_heads;
   int64_t q_sb, q_sh;
   TensorView ks, vs;
   int64_t mask_sb, mask_ss;
@@ -72,10 +66,6 @@ struct DecodeParams {
   float scale_log2;
 };
 
-// Keys a sequence's token sees, before any mask.
-__device__ __forceinline__ int decode_keys(const DecodeParams& p, int b) { return p.lengths ? min(max(p.lengths[b], 0), p.S - 1) + 1 : p.S; }
-
-template <bool ACCUMULATE>
 __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(const __grid_constant__ DecodeParams p) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(1024) uint8_t dec_smem[];            // the rings; at the end the warps' partial results
@@ -101,10 +91,9 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(co
   // ---- this CTA's key blocks: every n_dealt-th one, without those a mask hides entirely ------------------
   const int n_dealt = p.cluster * p.n_clusters;
   const int first_blk = (group % p.n_clusters) * p.cluster + rank;
-  const int n_keys = ACCUMULATE ? decode_keys(p, b) : p.S;
-  const int n_blk = (n_keys + DEC_BLOCK - 1) / DEC_BLOCK;
+  const int n_blk = (p.S + DEC_BLOCK - 1) / DEC_BLOCK;
   int n_live = first_blk < n_blk ? (n_blk - 1 - first_blk) / n_dealt + 1 : 0;
-  auto block_bits = [&](int key0) { return n_keys - key0 >= DEC_BLOCK ? 0xffffu : (1u << (n_keys - key0)) - 1u; };
+  auto block_bits = [&](int key0) { return p.S - key0 >= DEC_BLOCK ? 0xffffu : (1u << (p.S - key0)) - 1u; };
   if (p.mask != nullptr) {
     uint32_t bits = 0;
     int key0 = 0;
@@ -201,13 +190,12 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(co
       mma_m16n8k16(s[1], qf[t][0], 0u, qf[t][1], 0u, r[2], r[3]);
     }
     uint32_t seen;
-    const int key0 = block(e, seen);
+    block(e, seen);
     float x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int key = 2 * j + (i & 1) + 8 * (i >> 1);
       x[i] = (seen >> key) & 1u ? s[i >> 1][i & 1] * p.scale_log2 : -CUDART_INF_F;
-      if (ACCUMULATE && g < n_heads && (seen >> key) & 1u) p.scores[(int64_t(u) * p.S + key0 + key) * p.score_heads + g] = x[i];
     }
     float m_blk = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
     m_blk = fmaxf(m_blk, __shfl_xor_sync(0xffffffffu, m_blk, 1));
@@ -283,7 +271,6 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(co
     }
     if (p.n_clusters == 1) {
       p.o[(int64_t(b) * p.H + h0 + h) * HEAD_DIM + tid] = __float2bfloat16(l_all == 0.f ? 0.f : acc / l_all);
-      if (ACCUMULATE && tid == 0) p.stats[int64_t(b) * p.H + h0 + h] = make_float2(m_all, 1.f / l_all);
     } else {
       float* part = p.scratch + int64_t(group) * DEC_PARTIAL + h * (HEAD_DIM + 2);
       part[tid] = acc;
@@ -294,7 +281,6 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM) decode_kernel(co
 }
 
 // The clusters' partial results of one query head -> output row. One CTA per (batch, head), thread = dim.
-template <bool ACCUMULATE>
 __global__ void __launch_bounds__(HEAD_DIM) decode_merge_kernel(const __grid_constant__ DecodeParams p) {
   const int h = blockIdx.x % p.H, b = blockIdx.x / p.H;
   const int rep = p.H / p.Hkv;
@@ -312,28 +298,6 @@ __global__ void __launch_bounds__(HEAD_DIM) decode_merge_kernel(const __grid_con
     l_all += f * pc[HEAD_DIM + 1];
   }
   p.o[(int64_t(b) * p.H + h) * HEAD_DIM + threadIdx.x] = __float2bfloat16(l_all == 0.f ? 0.f : acc / l_all);
-  if (ACCUMULATE && threadIdx.x == 0) p.stats[blockIdx.x] = make_float2(m_all, 1.f / l_all);
-}
-
-// weights += each visible key's probabilities summed over its KV head's query heads, from the scores and every head's
-// maximum and sum. A thread per key, so the order of the sum is fixed.
-constexpr int DEC_WEIGHT_THREADS = 256;
-__global__ void __launch_bounds__(DEC_WEIGHT_THREADS) decode_weights_kernel(const __grid_constant__ DecodeParams p) {
-  const int hk = blockIdx.y % p.Hkv, b = blockIdx.y / p.Hkv;
-  const int key = blockIdx.x * DEC_WEIGHT_THREADS + threadIdx.x;
-  if (key >= decode_keys(p, b) || (p.mask != nullptr && p.mask[b * p.mask_sb + key * p.mask_ss] == 0)) return;
-  const int rep = p.H / p.Hkv;
-  const float2* const stats = p.stats + int64_t(b) * p.H + hk * rep;
-  float sum = 0.f;
-  for (int hg = 0; hg < p.head_groups; ++hg) {
-    const float* const x = p.scores + ((int64_t(blockIdx.y) * p.head_groups + hg) * p.S + key) * p.score_heads;
-    const int heads = min(rep - hg * DEC_HEADS, DEC_HEADS);
-    for (int h = 0; h < heads; ++h) {
-      const float2 st = stats[hg * DEC_HEADS + h];
-      sum += ptx::ex2(x[h] - st.x) * st.y;
-    }
-  }
-  p.weights[b * p.weights_sb + hk * p.weights_sh + key] += sum;
 }
 
 }  // namespace intra

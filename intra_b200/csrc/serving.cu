@@ -9,7 +9,7 @@
 #include "cache_kernel.cuh"
 #include "host.h"
 #include "tma_encode.h"
-#include "tree_kernel.cuh"
+#include "tree_mma_kernel.cuh"
 #include "tree_umma_kernel.cuh"
 #include "verify_kernel.cuh"
 
@@ -28,8 +28,6 @@ struct ServingState {
 };
 ServingState g_serving[MAX_DEVICES];
 
-constexpr int TREE_MASK_TOKENS = 32 * 2;         // rows of mask bits the largest launch holds
-
 // Runs once per device with that device current. Allocates nothing, so a first call may be captured.
 void init_serving(int device) {
   ServingState& st = g_serving[device];
@@ -38,8 +36,10 @@ void init_serving(int device) {
   if (e != cudaSuccess) { st.init_status = cuda_fail(e); return; }
   if (major != 10) { st.init_status = INTRA_ERR_DEVICE; return; }
   e = cudaDeviceGetAttribute(&st.sm_count, cudaDevAttrMultiProcessorCount, device);
-  if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<1>, tree_smem_bytes<1>(TREE_MASK_TOKENS));
-  if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<2>, tree_smem_bytes<2>(TREE_MASK_TOKENS));
+  if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<false, false>, tree_smem_bytes(TREE_MAX_TOKENS));
+  if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<false, true>, tree_smem_bytes(TREE_MAX_TOKENS));
+  if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<true, false>, tree_smem_bytes(TREE_MAX_TOKENS));
+  if (e == cudaSuccess) e = opt_in_smem(tree_mma_kernel<true, true>, tree_smem_bytes(TREE_MAX_TOKENS));
   if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<false, false>, UMMA_SMEM_BYTES<false>);
   if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<false, true>, UMMA_SMEM_BYTES<false>);
   if (e == cudaSuccess) e = opt_in_smem(tree_umma_kernel<true, false>, UMMA_SMEM_BYTES<true>);
@@ -98,37 +98,34 @@ cudaError_t launch_early(K kernel, dim3 grid, int threads, int smem, cudaStream_
   return cudaLaunchKernelEx(&cfg, kernel, p...);
 }
 
-// How a cache of S keys is dealt out: CTAs per cluster and clusters per unit (a KV head's rows that one pass takes). As
-// many CTAs as are resident at once, two key blocks each at least; more where a CTA would get more blocks than it can list.
-void plan_tree(int64_t units, int S, int sm_count, int* cluster, int* n_clusters) {
-  const int n_blk = (S + TREE_BLOCK - 1) / TREE_BLOCK;
-  const int64_t slots = int64_t(sm_count) * TREE_CTAS_PER_SM;
-  int c = 1;
-  while (c < 8 && units * 2 * c <= slots && n_blk >= 4 * c) c *= 2;
-  while (c < 8 && n_blk > c * TREE_MAX_BLOCKS) c *= 2;
-  int n = ceil_div(n_blk, c * TREE_MAX_BLOCKS);
-  const int64_t fits = slots / (units * c);
-  n = imax(n, imin(n_blk / (16 * c), fits < 4096 ? int(fits) : 4096));
-  *cluster = c;
-  *n_clusters = n;
-}
-
-template <int MT>
-int launch_tree_mma(TreeParams& p, int B, const ServingState& st, int64_t scratch_bytes, int64_t* scratch_needed, cudaStream_t stream) {
-  const int rows = p.n * (p.H / p.Hkv);
-  p.row_groups = ceil_div(rows, 16 * MT);
-  const int64_t units = int64_t(B) * p.Hkv * p.row_groups;
-  plan_tree(units, p.S, st.sm_count, &p.cluster, &p.n_clusters);
-  const int64_t clusters = units * p.n_clusters;
-  if (clusters * p.cluster > 0x7fffffffLL || int64_t(B) * p.n * p.H > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
-  *scratch_needed = p.n_clusters > 1 ? clusters * TREE_PARTIAL<MT> * int64_t(sizeof(float)) : 0;
-  if (*scratch_needed > 0 && (!p.scratch || scratch_bytes < *scratch_needed)) return INTRA_NEED_SCRATCH;
-  const int smem = tree_smem_bytes<MT>(p.mask ? (p.mask_sn ? p.n : 1) : 0);
-  cudaError_t e = launch_cluster(tree_mma_kernel<MT>, clusters, p.cluster, TREE_THREADS, smem, stream, p);
-  if (e == cudaSuccess && p.n_clusters > 1) {
-    tree_merge_kernel<MT><<<unsigned(B) * unsigned(p.n) * unsigned(p.H), HEAD_DIM, 0, stream>>>(p);
-    e = cudaGetLastError();
+// Up to 16 rows per KV head, or any number of one token's whose weights are accumulated.
+template <bool ACCUMULATE>
+int launch_tree_mma(TreeParams p, const ServingState& st, int64_t scratch_bytes, int64_t* scratch_needed, cudaStream_t stream) {
+  const int all_rows = p.n * (p.H / p.Hkv);
+  p.row_groups = ceil_div(all_rows, TREE_ROWS);
+  p.unit_cost = TREE_UNIT_COST;
+  p.min_tiles = TREE_MIN_BLOCKS;
+  const int64_t units = int64_t(p.B) * p.Hkv * p.row_groups, rows = int64_t(p.B) * p.Hkv * all_rows;
+  const int64_t blocks = units * ceil_div(p.S, TREE_BLOCK), places = blocks + units * TREE_UNIT_COST;      // at most
+  const int slots = st.sm_count * TREE_CTAS_PER_SM;
+  if (places + slots * int64_t(TREE_MIN_BLOCKS) > 0x7fffffffLL || rows > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
+  const int64_t parts = (blocks + TREE_MIN_BLOCKS - 1) / TREE_MIN_BLOCKS;
+  const int grid = parts < slots ? int(parts) : slots;
+  int64_t floats = (grid + units) * int64_t(TREE_PARTIAL);
+  if (ACCUMULATE) {
+    if (int64_t(p.B) * p.Hkv > 65535) return INTRA_ERR_UNSUPPORTED;      // grid.y of the accumulation
+    p.score_keys = ceil_div(p.S, TREE_BLOCK) * TREE_BLOCK;
+    p.scores = p.scratch + floats;
+    floats += units * TREE_ROWS * p.score_keys;
   }
+  *scratch_needed = floats * int64_t(sizeof(float));
+  if (!p.scratch || scratch_bytes < *scratch_needed) return INTRA_NEED_SCRATCH;
+  const int smem = tree_smem_bytes(p.mask ? (p.mask_sn ? p.n : 1) : 0);
+  cudaError_t e = all_rows <= TREE_ROWS / 2 ? launch_early(tree_mma_kernel<ACCUMULATE, true>, dim3(unsigned(grid)), TREE_THREADS, smem, stream, p)
+                                            : launch_early(tree_mma_kernel<ACCUMULATE, false>, dim3(unsigned(grid)), TREE_THREADS, smem, stream, p);
+  if (e == cudaSuccess)
+    e = ACCUMULATE ? launch_early(tree_weights_kernel, dim3(unsigned(ceil_div(p.S, TREE_WEIGHT_KEYS)) + 1, unsigned(p.B * p.Hkv)), TREE_WEIGHT_THREADS, 0, stream, p, uint32_t(grid))
+                   : launch_early(tree_merge_kernel, dim3(unsigned((rows + TREE_MERGE_WARPS - 1) / TREE_MERGE_WARPS)), 32 * TREE_MERGE_WARPS, 0, stream, p, uint32_t(grid));
   return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
 }
 
@@ -141,22 +138,22 @@ bool cache_map(const __nv_bfloat16* ptr, const TensorView& v, int S, int Hkv, in
   return encode_map(map, ptr, 5, dims, strides, box, ones);
 }
 
-constexpr int UMMA_FROM_ROWS = 16;
 template <bool PAIR>
-int launch_tree_umma(const TreeParams& t, int B, const ServingState& st, int64_t scratch_bytes, int64_t* scratch_needed, cudaStream_t stream) {
+int launch_tree_umma(const TreeParams& t, const ServingState& st, int64_t scratch_bytes, int64_t* scratch_needed, cudaStream_t stream) {
   TreeUmmaParams p;
   p.t = t;
-  p.B = B;
+  const int B = t.B;
   p.t.row_groups = ceil_div(t.n * (t.H / t.Hkv), UMMA_ROWS<PAIR>);
   p.by_rep = fast_div(t.H / t.Hkv);
   const int64_t tiles = int64_t(B) * t.Hkv * p.t.row_groups * ceil_div(t.S, TILE_N);       // at most
   const int64_t parts = (tiles + UMMA_MIN_TILES - 1) / UMMA_MIN_TILES;
   const int64_t rows = int64_t(B) * t.n * t.H;
-  const int64_t places = tiles + int64_t(B) * t.Hkv * p.t.row_groups * 3;      // and their ends
+  const int64_t places = tiles + int64_t(B) * t.Hkv * p.t.row_groups * UMMA_UNIT_COST<PAIR>;
   const int64_t merge_ctas = int64_t(B) * t.Hkv * p.t.row_groups * UMMA_MERGE_CTAS<PAIR>;
   if (places + st.sm_count > 0x7fffffffLL || rows > 0x7fffffffLL || merge_ctas > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
   const int grid = parts < st.sm_count ? int(parts) : st.sm_count;
-  p.t.pair = PAIR;
+  p.t.unit_cost = UMMA_UNIT_COST<PAIR>;
+  p.t.min_tiles = UMMA_MIN_TILES;
   *scratch_needed = grid * 2 * UMMA_PARTIAL<PAIR> * int64_t(sizeof(float));
   if (t.mask) {                   // behind the partial results: the mask's bits, those of any token, the tiles
     char* const at = reinterpret_cast<char*>(t.scratch) + *scratch_needed;
@@ -229,13 +226,51 @@ int intra_b200_tree_attn(const void* q, const void* k, const void* v, const int*
     p.mask_sb = mask_strides[0]; p.mask_sn = mask_strides[1]; p.mask_ss = mask_strides[2];
     p.mask_vec = p.mask_ss == 1 && aligned16(mask) && ((p.mask_sb | p.mask_sn) & 15) == 0;
   }
-  p.S = S; p.H = H; p.Hkv = Hkv; p.n = n;
+  p.S = S; p.H = H; p.Hkv = Hkv; p.n = n; p.B = B;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  if (n * (H / Hkv) > 128) return launch_tree_umma<true>(p, B, *st, scratch_bytes, scratch_needed, stream);
-  if (n * (H / Hkv) > UMMA_FROM_ROWS) return launch_tree_umma<false>(p, B, *st, scratch_bytes, scratch_needed, stream);
-  if (n * (H / Hkv) <= 16) return launch_tree_mma<1>(p, B, *st, scratch_bytes, scratch_needed, stream);
-  return launch_tree_mma<2>(p, B, *st, scratch_bytes, scratch_needed, stream);
+  if (n * (H / Hkv) > 128) return launch_tree_umma<true>(p, *st, scratch_bytes, scratch_needed, stream);
+  if (n * (H / Hkv) > TREE_ROWS) return launch_tree_umma<false>(p, *st, scratch_bytes, scratch_needed, stream);
+  return launch_tree_mma<false>(p, *st, scratch_bytes, scratch_needed, stream);
+}
+
+int intra_b200_decode_accumulate(const void* q, const void* k, const void* v, const void* mask, const int* lengths, void* out,
+                                 float* weights, void* scratch, int64_t scratch_bytes, int64_t* scratch_needed, int B, int S,
+                                 int H, int Hkv, const int64_t q_strides[3], const int64_t k_strides[3],
+                                 const int64_t v_strides[3], const int64_t mask_strides[2], int64_t weights_batch_stride,
+                                 int64_t weights_head_stride, float softmax_scale, int device, void* cuda_stream) {
+  if (!q || !k || !v || !out || !weights || !scratch_needed || !q_strides || !k_strides || !v_strides || (mask && !mask_strides) ||
+      B <= 0 || S <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || !(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
+    return INTRA_ERR_BAD_ARG;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(scratch) || !rows_aligned(q_strides) ||
+      !rows_aligned(k_strides) || !rows_aligned(v_strides) || !aligned4(weights) || !aligned4(lengths))
+    return INTRA_ERR_ALIGNMENT;
+  if ((B > 1 && weights_batch_stride <= 0) || (Hkv > 1 && weights_head_stride <= 0)) return INTRA_ERR_BAD_ARG;
+  if (device < 0 || device >= MAX_DEVICES) return INTRA_ERR_BAD_ARG;
+  DeviceGuard guard(device);
+  const ServingState* st;
+  const int rc = serving_device(device, guard, &st);
+  if (rc != INTRA_OK) return rc;
+  TreeParams p = {};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.lengths = lengths;
+  p.mask = static_cast<const uint8_t*>(mask);
+  p.o = static_cast<__nv_bfloat16*>(out);
+  p.weights = weights;
+  p.weights_sb = weights_batch_stride; p.weights_sh = weights_head_stride;
+  p.scratch = static_cast<float*>(scratch);
+  p.q_sb = q_strides[0]; p.q_sn = q_strides[1]; p.q_sh = q_strides[2];
+  p.ks = view_of(k_strides);
+  p.vs = view_of(v_strides);
+  if (mask) {
+    p.mask_sb = mask_strides[0]; p.mask_ss = mask_strides[1];
+    p.mask_vec = p.mask_ss == 1 && aligned16(mask) && (p.mask_sb & 15) == 0;
+  }
+  p.S = S; p.H = H; p.Hkv = Hkv; p.n = 1; p.B = B;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  return launch_tree_mma<true>(p, *st, scratch_bytes, scratch_needed, static_cast<cudaStream_t>(cuda_stream));
 }
 
 int intra_b200_verify_drafts(const void* tokens, int tokens_int64, const void* target, const void* draft, int prob_type,

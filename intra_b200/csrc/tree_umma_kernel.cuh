@@ -1,11 +1,8 @@
-// Attention of drafted tokens over a cache (tree_kernel.cuh) for more rows than a warp's registers hold: the products on
-// tcgen05 with 128 rows a tile, K and V tiles of 128 keys.
+// Attention of drafted tokens over a cache for more rows than a warp's registers hold (tree_mma_kernel.cuh has the definition):
+// the products on tcgen05 with 128 rows a tile, K and V tiles of 128 keys.
 //
 // Up to 256 rows the bound is still reading K and V (64 KB a key tile, 2,800 cycles at an SM's share of the HBM
-// bandwidth; the products of 256 rows take 2,048). So the work is dealt by key tiles, whatever sequence they belong to: all
-// tiles of all units - a unit is a KV head of a sequence, with up to ROWS rows - stand in one list, CTA c takes
-// the c-th part of it. A unit that no CTA holds as a whole leaves partial results (the sum, its maximum and
-// weight) that tree_umma_merge_kernel joins.
+// bandwidth; the products of 256 rows take 2,048). The work is dealt by key tiles (tree_list.cuh).
 //
 // Two streams of softmax work run side by side, so that the tensor cores have one's products while the other is at its
 // exponentials:
@@ -35,7 +32,8 @@
 #include <cuda.h>
 
 #include "softmax.cuh"
-#include "tree_kernel.cuh"
+#include "tree_list.cuh"
+#include "warp_mma.cuh"
 
 namespace intra {
 
@@ -51,180 +49,17 @@ template <bool PAIR> constexpr int UMMA_SMEM_BYTES = (UMMA_RING + (PAIR ? 2 : 1)
 template <bool PAIR> constexpr int64_t UMMA_PARTIAL = int64_t(UMMA_ROWS<PAIR>) * (HEAD_DIM + 2);
 // A CTA's part is at least this many key tiles: a shorter one costs more in its ends and its merge than it spreads.
 constexpr int UMMA_MIN_TILES = 2;
+// Places a unit has in front of its tiles. Measured with 0 / 1 / 3: 64 tokens over 65536 keys (PAIR) 73.1 / 71.9 / 70.6 us, 26
+// tokens over 8 sequences of 4096 to 8192 keys 59.8 / 59.2 / 67.8.
+template <bool PAIR> constexpr int UMMA_UNIT_COST = PAIR ? 3 : 1;
 
 struct TreeUmmaParams {
   TreeParams t;                // row_groups: units per KV head
   FastDiv by_rep;              // query heads per KV head
   CUtensorMap maps[2];         // K, V: (128, S, 1, Hkv, B)
   int use_tma;
-  int B;
   int* status;
 };
-
-struct TreePiece {             // what a CTA does of one unit
-  int b, hk, rg;               // sequence, KV head, row group
-  int first, count;            // key tiles
-  int of;                      // key tiles of the whole unit
-  int starts;                  // the piece begins with the unit
-  int ctx, n_keys;
-};
-// Key tiles of a sequence; with a mask from the first to the last of which any token sees a key (one, where there is none).
-__device__ __forceinline__ int tree_tiles(const TreeParams& p, int b, int* first = nullptr) {
-  const int all = (tree_context(p, b) + p.n + TILE_N - 1) / TILE_N;
-  int lo = 0, hi = all;
-  if (p.live != nullptr) {
-    const unsigned long long* const live = reinterpret_cast<const unsigned long long*>(p.live) + int64_t(b) * p.live_words;
-    lo = all;
-    hi = 0;
-    for (int i = 0; i * 64 < all; ++i) {
-      const int left = all - i * 64;
-      const unsigned long long x = live[i] & (left >= 64 ? ~0ull : (1ull << left) - 1ull);
-      if (x) {
-        lo = min(lo, i * 64 + __ffsll(x) - 1);
-        hi = i * 64 + 64 - __clzll(x);
-      }
-    }
-    if (hi == 0) { lo = 0; hi = 1; }
-  }
-  if (first) *first = lo;
-  return hi - lo;
-}
-
-// The list of all units' key tiles. A unit counts for `cost` places more than it has tiles, in front of them: what the end
-// of one unit and the start of the next cost the CTA that has both (parts of a few tiles would only be spread unevenly by
-// it). Measured with 0 / 1 / 3 places: 64 tokens over 65536 keys (PAIR) 73.1 / 71.9 / 70.6 us, 26 tokens over 8 sequences of
-// 4096 to 8192 keys 59.8 / 59.2 / 67.8. At most 2^31 - 1 places.
-struct TreeList {
-  uint32_t units, cost, per, total;      // units per sequence; places of a CTA's part, of all
-  // Called by whole warps; all lanes get the same. `before`: tiles and units of sequences before `b`.
-  __device__ __forceinline__ TreeList(const TreeParams& p, int B, uint32_t grid, int b = 0, uint32_t* before = nullptr) {
-    units = p.Hkv * p.row_groups;
-    uint32_t tiles = 0, front = 0;
-    if (p.lengths == nullptr && p.live == nullptr) {               // all sequences alike
-      tiles = uint32_t(B) * uint32_t(tree_tiles(p, 0));
-      front = uint32_t(b) * uint32_t(tree_tiles(p, 0));
-    } else {
-      for (int s = threadIdx.x & 31; s < B; s += 32) {
-        const uint32_t n = tree_tiles(p, s);
-        tiles += n;
-        front += s < b ? n : 0u;
-      }
-      tiles = __reduce_add_sync(0xffffffffu, tiles);
-      front = __reduce_add_sync(0xffffffffu, front);
-    }
-    const uint32_t share = tiles * units / grid;
-    cost = share < 8 ? 0 : p.pair && share >= 16 ? 3 : 1;
-    total = (tiles + cost * B) * units;
-    per = (total + grid - 1) / grid;
-    per = per < UMMA_MIN_TILES ? UMMA_MIN_TILES : per;
-    if (before) *before = (front + cost * b) * units;
-  }
-};
-
-// A CTA's part [next, end) of the list as a cursor that every warp moves by itself. Cursor and piece stand in shared memory:
-// as registers they would make the softmax warps, which hold a row's 128 scores, spill.
-struct TreeWalk {
-  uint32_t next, end;
-  uint32_t b_start;            // place of sequence b's first unit
-  uint32_t units, cost;
-  int b, b_tiles, b_first;     // of one unit: its tiles, the first of them
-  // Called by whole warps; all lanes get the same.
-  __device__ __forceinline__ void start(const TreeParams& p, int B, uint32_t cta, uint32_t grid) {
-    const int lane = threadIdx.x & 31;
-    const TreeList list(p, B, grid);
-    units = list.units;
-    cost = list.cost;
-    next = list.per * cta < list.total ? list.per * cta : list.total;
-    end = list.total - next > list.per ? next + list.per : list.total;
-    b = b_tiles = b_first = 0;
-    b_start = 0;
-    if (next >= end) return;
-    for (int s0 = 0; s0 < B; s0 += 32) {                           // the sequence that holds `next`
-      const uint32_t mine = s0 + lane < B ? (uint32_t(tree_tiles(p, s0 + lane)) + cost) * units : 0u;
-      uint32_t upto = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += y;
-      }
-      const uint32_t past = __ballot_sync(0xffffffffu, b_start + upto > next);
-      if (past) {
-        b = s0 + __ffs(past) - 1;
-        b_start += __shfl_sync(0xffffffffu, upto - mine, __ffs(past) - 1);
-        break;
-      }
-      b_start += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    b_tiles = tree_tiles(p, b, &b_first);
-  }
-  __device__ __forceinline__ void piece(const TreeParams& p, TreePiece& x) {
-    x.count = 0;
-    while (next < end) {
-      uint32_t places = b_tiles + cost;
-      if (next - b_start >= places * units) {
-        b_start += places * units;
-        b_tiles = tree_tiles(p, ++b, &b_first);
-        places = b_tiles + cost;
-      }
-      const uint32_t local = next - b_start, unit = local / places, at = local - unit * places;
-      const uint32_t take = min(end - next, places - at);
-      next += take;
-      const int first = max(int(at) - int(cost), 0), last = int(at + take) - int(cost);
-      if (last <= first) continue;                                 // of this unit only places without tiles
-      x.b = b;
-      x.hk = p.row_groups == 1 ? unit : unit / p.row_groups;
-      x.rg = unit - x.hk * p.row_groups;
-      x.of = b_tiles;
-      x.first = b_first + first;
-      x.count = last - first;
-      x.starts = first == 0;
-      x.ctx = tree_context(p, b);
-      x.n_keys = x.ctx + p.n;
-      return;
-    }
-  }
-};
-// The warp's next piece of its CTA's part; false: there is none.
-__device__ __forceinline__ bool tree_next(const TreeParams& p, TreeWalk& walk, TreePiece& x) {
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) walk.piece(p, x);
-  __syncwarp();
-  return x.count > 0;
-}
-
-// tree_ancestors for one warp: the tokens' own keys that `token` sees, as bits. A lane holds tokens lane and lane + 32.
-__device__ __forceinline__ unsigned long long tree_own_keys(const TreeParams& p, int b, int token) {
-  if (p.all_own) return (2ull << (p.n - 1)) - 1ull;
-  if (p.parents == nullptr) return (2ull << token) - 1ull;
-  const int lane = threadIdx.x & 31;
-  unsigned long long anc[2];
-  int up[2];
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int i = lane + 32 * c, parent = i < p.n ? p.parents[b * p.parents_sb + i] : -1;
-    up[c] = parent >= 0 && parent < i ? parent : -1;
-    anc[c] = 1ull << i;
-  }
-  auto of_token = [](const unsigned long long (&x)[2], int i) {
-    const unsigned long long a = __shfl_sync(0xffffffffu, x[0], i & 31), c = __shfl_sync(0xffffffffu, x[1], i & 31);
-    return i & 32 ? c : a;
-  };
-  for (int reach = 1; reach < p.n; reach *= 2) {
-    unsigned long long more[2];
-    int next[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int i = up[c] < 0 ? 0 : up[c];
-      const int a = __shfl_sync(0xffffffffu, up[0], i & 31), d = __shfl_sync(0xffffffffu, up[1], i & 31);
-      const unsigned long long x = of_token(anc, i);
-      more[c] = up[c] < 0 ? 0ull : x;
-      next[c] = up[c] < 0 ? -1 : i & 32 ? d : a;
-    }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) { anc[c] |= more[c]; up[c] = next[c]; }
-  }
-  return of_token(anc, token);
-}
 
 // The mask of a token as bits, a word for 32 keys.
 __device__ __forceinline__ const uint32_t* tree_bits(const TreeParams& p, int b, int token) {
@@ -274,7 +109,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
   __shared__ uint64_t bars[N_BARS];
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
-  __shared__ TreeWalk walks[UMMA_THREADS / 32];
+  __shared__ TreeWalk<TILE_N> walks[UMMA_THREADS / 32];
   __shared__ TreePiece pieces[UMMA_THREADS / 32];
   __shared__ float2 row_ml[2][PAIR ? 1 : 2][PAIR ? 1 : TILE_M];     // [unit parity][stream][row]
   const TreeParams& t = p.t;
@@ -303,11 +138,11 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
   if (warp == 8 && lane < 2) ptx::prefetch_tensormap(&p.maps[lane]);
   cudaGridDependencySynchronize();                       // what is above ran beside the end of the kernel before this one
   cudaTriggerProgrammaticLaunchCompletion();             // the merge may be set up; it waits for this kernel's end by itself
-  TreeWalk& walk = walks[warp];
+  TreeWalk<TILE_N>& walk = walks[warp];
   const TreePiece& pc = pieces[warp];
   {
-    TreeWalk w;
-    w.start(t, p.B, blockIdx.x, gridDim.x);
+    TreeWalk<TILE_N> w;
+    w.start(t, t.B, blockIdx.x, gridDim.x);
     if (lane == 0) walk = w;
   }
   // Copies rows `first`, first + step, .. of a unit's queries, 16 threads a row; rows past the last become zeros.
@@ -773,8 +608,8 @@ __global__ void __launch_bounds__(32 * UMMA_MERGE_WARPS) tree_umma_merge_kernel(
   const int col = (block % UMMA_MERGE_SPLIT * UMMA_MERGE_WARPS + (threadIdx.x >> 5)) * UMMA_MERGE_COLS;
   if (row - lane >= t.n * rep) return;                    // no such rows
   uint32_t start;
-  const TreeList list(t, p.B, grid, b, &start);
-  const int tiles = tree_tiles(t, b);
+  const TreeList<TILE_N> list(t, t.B, grid, b, &start);
+  const int tiles = tree_tiles<TILE_N>(t, b);
   start += uint32_t(in_b) * (tiles + list.cost) + list.cost;       // place of the unit's first tile
   const int c0 = int(start / list.per), c1 = int((start + tiles - 1) / list.per);
   cudaGridDependencySynchronize();                        // everything before this ran beside the main kernel's end
