@@ -47,6 +47,9 @@ void init_serving(int device) {
   void* word = nullptr;
   if (e == cudaSuccess) e = cudaGetSymbolAddress(&word, g_serving_status);
   st.status_word = static_cast<int*>(word);
+  if (e == cudaSuccess) e = opt_in_smem(verify_kernel<float>, VERIFY_SMEM_BYTES);
+  if (e == cudaSuccess) e = opt_in_smem(verify_kernel<__nv_bfloat16>, VERIFY_SMEM_BYTES);
+  if (e == cudaSuccess) e = opt_in_smem(verify_kernel<__half>, VERIFY_SMEM_BYTES);
   if (e == cudaSuccess) e = opt_in_smem(evict_select_kernel<true>, EVICT_SMEM_KEYS * 4);
   if (e != cudaSuccess) st.init_status = cuda_fail(e);
 }
@@ -304,9 +307,9 @@ int intra_b200_verify_drafts(const void* tokens, int tokens_int64, const void* t
   p.cluster = c;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   cudaError_t e;
-  if (prob_type == INTRA_PROB_F32) e = launch_cluster(verify_kernel<float>, B, c, VERIFY_THREADS, 0, stream, p);
-  else if (prob_type == INTRA_PROB_BF16) e = launch_cluster(verify_kernel<__nv_bfloat16>, B, c, VERIFY_THREADS, 0, stream, p);
-  else e = launch_cluster(verify_kernel<__half>, B, c, VERIFY_THREADS, 0, stream, p);
+  if (prob_type == INTRA_PROB_F32) e = launch_cluster(verify_kernel<float>, B, c, VERIFY_THREADS, VERIFY_SMEM_BYTES, stream, p);
+  else if (prob_type == INTRA_PROB_BF16) e = launch_cluster(verify_kernel<__nv_bfloat16>, B, c, VERIFY_THREADS, VERIFY_SMEM_BYTES, stream, p);
+  else e = launch_cluster(verify_kernel<__half>, B, c, VERIFY_THREADS, VERIFY_SMEM_BYTES, stream, p);
   return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
 }
 

@@ -15,6 +15,11 @@
 // that. Every CTA walks the tree by itself, from the n probabilities of the drafted tokens, fetched at once; only a
 // rejection or the final draw reads a row: one pass, its sums exchanged through distributed shared memory. R is
 // not stored: it follows from p, q and the weights of the rejections so far.
+//
+// What bounds a pass is how much of the rows is under way: every thread copies 16-byte granules VERIFY_AHEAD ahead into slots of
+// its own in shared memory (its own copies are all it waits for). 32 trees of 26 nodes over 128257 tokens, the slowest of which
+// take 3 to 5 passes one after the other: 46 us with 8 tokens of both rows per thread in registers, of which the arithmetic in 64
+// bits was 8 us; 30 us so.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -22,6 +27,7 @@
 #include <stdint.h>
 
 #include "attn_kernel.cuh"
+#include "ptx.cuh"
 
 namespace intra {
 
@@ -29,6 +35,9 @@ constexpr int VERIFY_MAX_TOKENS = 64;
 constexpr int VERIFY_THREADS = 512;
 constexpr int VERIFY_WARPS = VERIFY_THREADS / 32;
 constexpr int VERIFY_MAX_CLUSTER = 8;
+constexpr int VERIFY_BATCH = 1;                  // granules a thread takes at a time (with 2 the registers do not last: 45 us)
+constexpr int VERIFY_AHEAD = 4;                  // batches of each row a thread has under way
+constexpr int VERIFY_SMEM_BYTES = VERIFY_THREADS * VERIFY_AHEAD * VERIFY_BATCH * 2 * 16;
 
 struct VerifyParams {
   const void* tokens;          // (B, n) by strides, int64 or int32
@@ -49,9 +58,33 @@ template <> __device__ __forceinline__ double as_double(float x) { return x; }
 template <> __device__ __forceinline__ double as_double(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <> __device__ __forceinline__ double as_double(__half x) { return __half2float(x); }
 
+// A probability as a double by its bits: the conversion instruction runs at an eighth of the rate. Denormals of fp32 come out
+// near 2^-127; the 16 terms of a draw that are read again are converted properly.
+__device__ __forceinline__ double widen(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __hiloint2double(int(b ? (b >> 3) + 0x38000000u : 0u), int(b << 29));
+}
+__device__ __forceinline__ float as_float(float x) { return x; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
+// max(x, 0) by the sign bit.
+__device__ __forceinline__ double above_zero(double x) {
+  const int keep = ~(__double2hiint(x) >> 31);
+  return __hiloint2double(__double2hiint(x) & keep, __double2loint(x) & keep);
+}
+
+// The sum over a warp's lanes, the same in all of them.
+__device__ __forceinline__ double warp_total(double x) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const __grid_constant__ VerifyParams p) {
+__global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const __grid_constant__ VerifyParams p) {
   namespace cg = cooperative_groups;
+  constexpr int EACH = 16 / sizeof(T);                             // tokens of a granule
+  extern __shared__ __align__(16) uint4 verify_smem[];
   __shared__ long long tok[VERIFY_MAX_TOKENS];
   __shared__ int parent[VERIFY_MAX_TOKENS], node[VERIFY_MAX_TOKENS];
   __shared__ double px[VERIFY_MAX_TOKENS], qx[VERIFY_MAX_TOKENS], ux[VERIFY_MAX_TOKENS];
@@ -82,10 +115,6 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const __grid_con
   }
   __syncthreads();
 
-  const int part = (V + p.cluster * VERIFY_WARPS - 1) / (p.cluster * VERIFY_WARPS);      // tokens a warp holds
-  const int64_t first = int64_t(rank * VERIFY_WARPS + warp) * part;
-  const int begin = int(first < V ? first : V), end = min(V - begin, part) + begin;
-
   int at = 0, accepted = 0, rejections = 0, passes = 0;
   int summed = -1;                                                 // rejections the sums of the last pass stand for
   double Z = 1.0, total = 0.0;
@@ -100,58 +129,106 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const __grid_con
   auto left_at = [&](int t, int count) {
     return left(as_double(p_row[t]), draft != nullptr && count > 0 ? as_double(q_row[t]) : 0.0, t, count);
   };
+  // The current row's granules, the first of which begins `off` tokens before token 0, and those of a warp.
+  int off = 0, per_warp = 0, granules = 0;
+  const uint32_t slots = ptx::smem_u32(verify_smem) + tid * 16;
+  constexpr uint32_t SLOT = VERIFY_THREADS * 16;
   // Sum of what is left over the whole row: the same number in every thread of the cluster.
   auto row_sum = [&](int count) {
-    double sum = 0.0;
-    constexpr int AT_ONCE = 8;                                     // tokens of a lane whose loads are under way together
-    int t = begin + lane;
-    for (; t + 32 * (AT_ONCE - 1) < end; t += 32 * AT_ONCE) {
-      T pt[AT_ONCE], qt[AT_ONCE];
+    const bool drawn = draft != nullptr && count > 0;
+    off = int(reinterpret_cast<uintptr_t>(p_row) & 15u) / int(sizeof(T));
+    granules = (V + off + EACH - 1) / EACH;
+    per_warp = (granules + p.cluster * VERIFY_WARPS - 1) / (p.cluster * VERIFY_WARPS);
+    const bool together = drawn && int(reinterpret_cast<uintptr_t>(q_row) & 15u) / int(sizeof(T)) == off;      // else q token by token
+    const uint4* const pg = reinterpret_cast<const uint4*>(p_row - off);
+    const uint4* const qg = reinterpret_cast<const uint4*>(together ? q_row - off : p_row - off);
+    const int g_end = min((rank * VERIFY_WARPS + warp + 1) * per_warp, granules);
+    int g = (rank * VERIFY_WARPS + warp) * per_warp + lane;
+    auto fetch = [&](int granule, int slot) {                      // always one commit group, possibly empty
 #pragma unroll
-      for (int e = 0; e < AT_ONCE; ++e) pt[e] = p_row[t + 32 * e];
-      const bool drawn = draft != nullptr && count > 0;
-      if (drawn) {
-#pragma unroll
-        for (int e = 0; e < AT_ONCE; ++e) qt[e] = q_row[t + 32 * e];
-      }
-      double r[AT_ONCE];
-#pragma unroll
-      for (int e = 0; e < AT_ONCE; ++e) r[e] = as_double(pt[e]);
-      for (int c = 0; c < count; ++c) {
-        const double w = -weight[c];
-        if (drawn) {
-#pragma unroll
-          for (int e = 0; e < AT_ONCE; ++e) r[e] = fmax(fma(w, as_double(qt[e]), r[e]), 0.0);
-        } else {
-          const int x = gone[c] >= 0 && gone[c] < V ? int(gone[c]) : -1;
-#pragma unroll
-          for (int e = 0; e < AT_ONCE; ++e) r[e] = t + 32 * e == x ? fmax(w + r[e], 0.0) : r[e];
+      for (int k = 0; k < VERIFY_BATCH; ++k) {
+        if (granule + 32 * k < g_end) {
+          ptx::cp_async_16(slots + ((slot * VERIFY_BATCH + k) * 2) * SLOT, pg + granule + 32 * k, 16u);
+          if (together) ptx::cp_async_16(slots + ((slot * VERIFY_BATCH + k) * 2 + 1) * SLOT, qg + granule + 32 * k, 16u);
         }
       }
+      ptx::cp_async_commit();
+    };
+    constexpr int STEP = 32 * VERIFY_BATCH;
 #pragma unroll
-      for (int e = 0; e < AT_ONCE; ++e) sum += r[e];
+    for (int k = 0; k < VERIFY_AHEAD - 1; ++k) fetch(g + STEP * k, k);
+    double part_sum[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int slot = 0; g < g_end; g += STEP, slot = (slot + 1) % VERIFY_AHEAD) {
+      fetch(g + STEP * (VERIFY_AHEAD - 1), (slot + VERIFY_AHEAD - 1) % VERIFY_AHEAD);
+      ptx::cp_async_wait<VERIFY_AHEAD - 1>();
+      // granule k of the batch: p, and VERIFY_THREADS granules further q
+      const uint4* const mine = verify_smem + slot * VERIFY_BATCH * 2 * VERIFY_THREADS + tid;
+      const int t0 = g * EACH - off;
+      bool here[VERIFY_BATCH];                                     // a granule of this part with tokens of the row only
+#pragma unroll
+      for (int k = 0; k < VERIFY_BATCH; ++k) {
+        const int t = t0 + k * 32 * EACH;
+        here[k] = g + 32 * k < g_end && t >= 0 && t + EACH <= V && (!drawn || together);
+        if (!here[k] && g + 32 * k < g_end)                        // the ends of the row; rows that lie differently in memory
+          for (int e = 0; e < EACH; ++e)
+            if (t + e >= 0 && t + e < V) part_sum[0] += left_at(t + e, count);
+      }
+#pragma unroll
+      for (int e0 = 0; e0 < EACH; e0 += 4) {                       // four tokens of each granule side by side
+        constexpr int N = 4 * VERIFY_BATCH;
+        double r[N];
+        float q[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const uint4* const at = mine + (e >> 2) * 2 * VERIFY_THREADS;
+          r[e] = here[e >> 2] ? widen(as_float(reinterpret_cast<const T*>(at)[e0 + (e & 3)])) : 0.0;
+          q[e] = drawn && here[e >> 2] ? as_float(reinterpret_cast<const T*>(at + VERIFY_THREADS)[e0 + (e & 3)]) : 0.f;
+        }
+        if (drawn && count == 1) {                                 // the first rejection at a node, whose Z is 1
+#pragma unroll
+          for (int e = 0; e < N; ++e) r[e] = above_zero(r[e] - widen(q[e]));
+        } else {
+          for (int c = 0; c < count; ++c) {
+            const double w = -weight[c];
+            if (drawn) {
+#pragma unroll
+              for (int e = 0; e < N; ++e) r[e] = above_zero(fma(w, widen(q[e]), r[e]));
+            } else {
+              const long long x = gone[c] - (t0 + e0);
+#pragma unroll
+              for (int e = 0; e < N; ++e) r[e] = x == (e >> 2) * 32 * EACH + (e & 3) ? above_zero(r[e] + w) : r[e];
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) part_sum[e & 3] += r[e];
+      }
     }
-    for (; t < end; t += 32) sum += left_at(t, count);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    ptx::cp_async_wait<0>();
+    double sum = (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+    sum = warp_total(sum);
     if (lane == 0) warp_sum[warp] = sum;
     __syncthreads();
     const int slot = ++passes & 1;                                 // the pass before may still be read elsewhere
-    if (tid == 0) {
-      double all = 0.0;
-      for (int w = 0; w < VERIFY_WARPS; ++w) all += warp_sum[w];
-      cta_sum[slot] = all;
+    if (warp == 0) {
+      const double all = warp_total(lane < VERIFY_WARPS ? warp_sum[lane] : 0.0);
+      if (lane == 0) cta_sum[slot] = all;
     }
     cluster.sync();
-    double all = 0.0;
-    for (int c = 0; c < p.cluster; ++c) all += *cluster.map_shared_rank(&cta_sum[slot], c);
+    // every warp by itself, a lane for each CTA
+    const double all = warp_total(lane < p.cluster ? *cluster.map_shared_rank(&cta_sum[slot], lane) : 0.0);
     summed = count;
     return all;
   };
 
   if (tid == 0) node[0] = 0;
-  for (int i = 1; i < n; ++i) {
-    if (parent[i] != at) continue;
+  const int parent0 = lane < n ? parent[lane] : -1, parent1 = lane + 32 < n ? parent[lane + 32] : -1;
+  auto next_child = [&](int after) {                               // of the current node, behind `after`; n: none
+    const unsigned long long children = (unsigned long long)(__ballot_sync(0xffffffffu, parent1 == at)) << 32 | __ballot_sync(0xffffffffu, parent0 == at);
+    const unsigned long long left_ones = children & ~((2ull << after) - 1ull);
+    return left_ones ? __ffsll(left_ones) - 1 : n;
+  };
+  for (int i = next_child(0); i < n; i = next_child(i)) {
     if (ux[i] * qx[i] * Z < left(px[i], qx[i], tok[i], rejections)) {
       at = i;
       ++accepted;
@@ -176,27 +253,28 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const __grid_con
 
   // ---- the last token: the CTA, the warp's part, the token whose running sum passes the threshold -----------
   const double threshold = ux[0] * total;
-  double before = 0.0, running = 0.0;
-  int owner = -1;
-  auto choose = [&](double sum, int who, int& last, double& last_before) {
-    if (owner < 0 && running + sum > threshold) { owner = who; before = running; }
-    if (sum > 0.0) { last = who; last_before = running; }
-    running += sum;
+  // Which of `count` parts, whose sums the lanes hold, the threshold falls into, and the sum before it.
+  auto choose = [&](double sum, int count, double before, int& owner, double& start) {
+    double upto = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const double y = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += y;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, lane < count && before + upto > threshold);
+    const uint32_t any = __ballot_sync(0xffffffffu, lane < count && sum > 0.0);
+    owner = past ? __ffs(past) - 1 : any ? 31 - __clz(any) : 0;    // rounding: the last part with any mass
+    start = before + __shfl_sync(0xffffffffu, upto - sum, owner);
   };
-  int last = 0;
-  double last_before = 0.0;
-  for (int c = 0; c < p.cluster; ++c) choose(*cluster.map_shared_rank(&cta_sum[passes & 1], c), c, last, last_before);
-  if (owner < 0) { owner = last; before = last_before; }           // rounding: the last part with any mass
+  int owner;
+  double before;
+  choose(lane < p.cluster ? *cluster.map_shared_rank(&cta_sum[passes & 1], lane) : 0.0, p.cluster, 0.0, owner, before);
   if (owner == rank) {
-    running = last_before = before;
-    owner = -1;
-    last = 0;
-    for (int w = 0; w < VERIFY_WARPS; ++w) choose(warp_sum[w], w, last, last_before);
-    if (owner < 0) { owner = last; before = last_before; }
+    choose(lane < VERIFY_WARPS ? warp_sum[lane] : 0.0, VERIFY_WARPS, before, owner, before);
     if (tid == 0) { found = 0x7fffffff; found_last = -1; }
-    const int64_t from = int64_t(rank * VERIFY_WARPS + owner) * part;
-    const int to = int(from + part < V ? from + part : V), per = (part + VERIFY_THREADS - 1) / VERIFY_THREADS;
-    const int t0 = int(from < V ? from : V) + tid * per, t1 = min(t0 + per, to);
+    const int g_from = min((rank * VERIFY_WARPS + owner) * per_warp, granules), g_to = min(g_from + per_warp, granules);
+    const int to = min(g_to * EACH - off, V), per = (per_warp * EACH + VERIFY_THREADS - 1) / VERIFY_THREADS;
+    const int t0 = max(g_from * EACH - off, 0) + tid * per, t1 = min(t0 + per, to);
     double mine = 0.0;
     for (int t = t0; t < t1; ++t) mine += left_at(t, rejections);
     double scan = mine;
