@@ -17,9 +17,10 @@
 // not stored: it follows from p, q and the weights of the rejections so far.
 //
 // What bounds a pass is how much of the rows is under way: every thread copies 16-byte granules VERIFY_AHEAD ahead into slots of
-// its own in shared memory (its own copies are all it waits for). 32 trees of 26 nodes over 128257 tokens, the slowest of which
-// take 3 to 5 passes one after the other: 46 us with 8 tokens of both rows per thread in registers, of which the arithmetic in 64
-// bits was 8 us; 30 us so.
+// its own in shared memory (its own copies are all it waits for), and then the arithmetic: 64-bit numbers are made from the bits
+// of 32-bit ones by integer multiply-adds, and compared with zero by their upper words. 32 trees of 26 nodes over 128257 tokens,
+// the slowest of which take 4 or 5 passes one after the other: 171 us with a division per rejection and token, 46 without, 42 with
+// the granules, 35 so; reading two rows of each once at the copy bandwidth takes 5.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -35,9 +36,8 @@ constexpr int VERIFY_MAX_TOKENS = 64;
 constexpr int VERIFY_THREADS = 512;
 constexpr int VERIFY_WARPS = VERIFY_THREADS / 32;
 constexpr int VERIFY_MAX_CLUSTER = 8;
-constexpr int VERIFY_BATCH = 1;                  // granules a thread takes at a time (with 2 the registers do not last: 45 us)
-constexpr int VERIFY_AHEAD = 4;                  // batches of each row a thread has under way
-constexpr int VERIFY_SMEM_BYTES = VERIFY_THREADS * VERIFY_AHEAD * VERIFY_BATCH * 2 * 16;
+constexpr int VERIFY_AHEAD = 4;                  // granules of each row a thread has under way
+constexpr int VERIFY_SMEM_BYTES = VERIFY_THREADS * VERIFY_AHEAD * 2 * 16;
 
 struct VerifyParams {
   const void* tokens;          // (B, n) by strides, int64 or int32
@@ -58,20 +58,18 @@ template <> __device__ __forceinline__ double as_double(float x) { return x; }
 template <> __device__ __forceinline__ double as_double(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <> __device__ __forceinline__ double as_double(__half x) { return __half2float(x); }
 
-// A probability as a double by its bits: the conversion instruction runs at an eighth of the rate. Denormals of fp32 come out
-// near 2^-127; the 16 terms of a draw that are read again are converted properly.
+// A probability as a double by its bits, in one integer multiply-add: the conversion instruction runs at an eighth of the
+// rate. Zero and the denormals of fp32 come out near 2^-127; terms that decide something by themselves are converted properly.
 __device__ __forceinline__ double widen(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return __hiloint2double(int(b ? (b >> 3) + 0x38000000u : 0u), int(b << 29));
+  return __longlong_as_double((long long)((unsigned long long)(__float_as_uint(x) & 0x7fffffffu) * (1ull << 29) + 0x3800000000000000ull));
 }
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
-// max(x, 0) by the sign bit.
-__device__ __forceinline__ double above_zero(double x) {
-  const int keep = ~(__double2hiint(x) >> 31);
-  return __hiloint2double(__double2hiint(x) & keep, __double2loint(x) & keep);
-}
+// max(x, 0) but for less than 2^-1040: only the upper word is looked at, in one integer operation.
+__device__ __forceinline__ double above_zero(double x) { return __hiloint2double(max(__double2hiint(x), 0), __double2loint(x)); }
+// A sum over a row of no more than this is none: what zeros come out as above adds up to 2^-106 at most.
+constexpr double VERIFY_NOTHING = 0x1p-100;
 
 // The sum over a warp's lanes, the same in all of them.
 __device__ __forceinline__ double warp_total(double x) {
@@ -145,63 +143,54 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const __grid_
     const int g_end = min((rank * VERIFY_WARPS + warp + 1) * per_warp, granules);
     int g = (rank * VERIFY_WARPS + warp) * per_warp + lane;
     auto fetch = [&](int granule, int slot) {                      // always one commit group, possibly empty
-#pragma unroll
-      for (int k = 0; k < VERIFY_BATCH; ++k) {
-        if (granule + 32 * k < g_end) {
-          ptx::cp_async_16(slots + ((slot * VERIFY_BATCH + k) * 2) * SLOT, pg + granule + 32 * k, 16u);
-          if (together) ptx::cp_async_16(slots + ((slot * VERIFY_BATCH + k) * 2 + 1) * SLOT, qg + granule + 32 * k, 16u);
-        }
+      if (granule < g_end) {
+        ptx::cp_async_16(slots + slot * 2 * SLOT, pg + granule, 16u);
+        if (together) ptx::cp_async_16(slots + (slot * 2 + 1) * SLOT, qg + granule, 16u);
       }
       ptx::cp_async_commit();
     };
-    constexpr int STEP = 32 * VERIFY_BATCH;
 #pragma unroll
-    for (int k = 0; k < VERIFY_AHEAD - 1; ++k) fetch(g + STEP * k, k);
+    for (int k = 0; k < VERIFY_AHEAD - 1; ++k) fetch(g + 32 * k, k);
     double part_sum[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int slot = 0; g < g_end; g += STEP, slot = (slot + 1) % VERIFY_AHEAD) {
-      fetch(g + STEP * (VERIFY_AHEAD - 1), (slot + VERIFY_AHEAD - 1) % VERIFY_AHEAD);
+    for (int slot = 0; g < g_end; g += 32, slot = (slot + 1) % VERIFY_AHEAD) {
+      fetch(g + 32 * (VERIFY_AHEAD - 1), (slot + VERIFY_AHEAD - 1) % VERIFY_AHEAD);
       ptx::cp_async_wait<VERIFY_AHEAD - 1>();
-      // granule k of the batch: p, and VERIFY_THREADS granules further q
-      const uint4* const mine = verify_smem + slot * VERIFY_BATCH * 2 * VERIFY_THREADS + tid;
+      const uint4* const mine = verify_smem + slot * 2 * VERIFY_THREADS + tid;
+      const T* const pt = reinterpret_cast<const T*>(mine);
+      const T* const qt = reinterpret_cast<const T*>(mine + VERIFY_THREADS);
       const int t0 = g * EACH - off;
-      bool here[VERIFY_BATCH];                                     // a granule of this part with tokens of the row only
-#pragma unroll
-      for (int k = 0; k < VERIFY_BATCH; ++k) {
-        const int t = t0 + k * 32 * EACH;
-        here[k] = g + 32 * k < g_end && t >= 0 && t + EACH <= V && (!drawn || together);
-        if (!here[k] && g + 32 * k < g_end)                        // the ends of the row; rows that lie differently in memory
-          for (int e = 0; e < EACH; ++e)
-            if (t + e >= 0 && t + e < V) part_sum[0] += left_at(t + e, count);
+      if (t0 < 0 || t0 + EACH > V || (drawn && !together)) {       // the row's ends; rows that lie differently in memory
+        for (int e = 0; e < EACH; ++e)
+          if (t0 + e >= 0 && t0 + e < V) part_sum[0] += left_at(t0 + e, count);
+        continue;
       }
 #pragma unroll
-      for (int e0 = 0; e0 < EACH; e0 += 4) {                       // four tokens of each granule side by side
-        constexpr int N = 4 * VERIFY_BATCH;
-        double r[N];
-        float q[N];
+      for (int e0 = 0; e0 < EACH; e0 += 4) {
+        double r[4];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const uint4* const at = mine + (e >> 2) * 2 * VERIFY_THREADS;
-          r[e] = here[e >> 2] ? widen(as_float(reinterpret_cast<const T*>(at)[e0 + (e & 3)])) : 0.0;
-          q[e] = drawn && here[e >> 2] ? as_float(reinterpret_cast<const T*>(at + VERIFY_THREADS)[e0 + (e & 3)]) : 0.f;
-        }
-        if (drawn && count == 1) {                                 // the first rejection at a node, whose Z is 1
+        for (int e = 0; e < 4; ++e) r[e] = widen(as_float(pt[e0 + e]));
+        if (drawn) {
+          double q[4];
 #pragma unroll
-          for (int e = 0; e < N; ++e) r[e] = above_zero(r[e] - widen(q[e]));
+          for (int e = 0; e < 4; ++e) {
+            q[e] = widen(as_float(qt[e0 + e]));
+            r[e] = above_zero(r[e] - q[e]);                        // the first rejection at a node, whose Z is 1
+          }
+          for (int c = 1; c < count; ++c) {
+            const double w = -weight[c];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = above_zero(fma(w, q[e], r[e]));
+          }
         } else {
           for (int c = 0; c < count; ++c) {
             const double w = -weight[c];
-            if (drawn) {
+            const long long x = gone[c] - (t0 + e0);
 #pragma unroll
-              for (int e = 0; e < N; ++e) r[e] = above_zero(fma(w, widen(q[e]), r[e]));
-            } else {
-              const long long x = gone[c] - (t0 + e0);
-#pragma unroll
-              for (int e = 0; e < N; ++e) r[e] = x == (e >> 2) * 32 * EACH + (e & 3) ? above_zero(r[e] + w) : r[e];
-            }
+            for (int e = 0; e < 4; ++e) r[e] = x == e ? above_zero(r[e] + w) : r[e];
           }
         }
 #pragma unroll
-        for (int e = 0; e < N; ++e) part_sum[e & 3] += r[e];
+        for (int e = 0; e < 4; ++e) part_sum[e] += r[e];
       }
     }
     ptx::cp_async_wait<0>();
@@ -244,7 +233,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const __grid_
     if (tid == 0) { weight[rejections] = Z; gone[rejections] = tok[i]; }
     __syncthreads();
     const double rest = row_sum(rejections + 1);
-    if (rest > 0.0) {
+    if (rest > VERIFY_NOTHING) {
       ++rejections;
       Z = total = rest;
     }

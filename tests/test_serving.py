@@ -326,6 +326,11 @@ def test_verification_at_its_edges():
     got = verify_drafts(tokens, short, target, uniform)
     want = _verify_reference(tokens, short, target, uniform, None)
     assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want)) and got[0].tolist() == [0] * 4
+    # zeros of either sign
+    sparse = torch.where(torch.rand(target.shape, generator=_gen(2)).cuda() < 0.9, -0.0, target)
+    got = verify_drafts(tokens, sparse, draft, uniform)
+    want = _verify_reference(tokens, sparse, draft, uniform, None)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
     # drafts outside the vocabulary are rejected, and nothing outside the rows is read
     bad = tokens.clone()
     bad[0, 1], bad[1, 1], bad[2, 2] = -1, V, 2 ** 40
