@@ -61,7 +61,7 @@ template <> __device__ __forceinline__ double as_double(__half x) { return __hal
 // A probability as a double by its bits, in one integer multiply-add: the conversion instruction runs at an eighth of the
 // rate. Zero and the denormals of fp32 come out near 2^-127; terms that decide something by themselves are converted properly.
 __device__ __forceinline__ double widen(float x) {
-  return __longlong_as_double((long long)((unsigned long long)(__float_as_uint(x) & 0x7fffffffu) * (1ull << 29) + 0x3800000000000000ull));
+  return __longlong_as_double((long long)(__float_as_int(x)) * (1 << 29) + 0x3800000000000000ll);
 }
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
