@@ -133,11 +133,12 @@ int intra_b200_verify_drafts(const void* tokens, int tokens_int64, const void* t
                              int V, const int64_t target_strides[2], const int64_t draft_strides[2], int64_t tokens_batch_stride,
                              int64_t uniform_batch_stride, int64_t parents_batch_stride, int device, void* cuda_stream);
 
-/* Moves the rows of accepted tokens together, in place, in n_caches K or V caches of B x S x Hkv rows (strides: three per
- * cache, positive; the caches must not overlap): row lengths[b] + path[b][i] becomes row lengths[b] + i for every i < n with
+/* Moves the rows of accepted tokens together, in place, in n_caches K or V caches of B x S x Hkv rows (strides {batch,
+ * token, head}, positive: three for each cache where strides_step is 3, the same three for all where it is 0; the caches
+ * must not overlap): row lengths[b] + path[b][i] becomes row lengths[b] + i for every i < n with
  * path[b][i] in 0 .. n - 1, whatever the order; nothing moves for a sequence whose lengths[b] is not in 0 .. S - n. */
-int intra_b200_keep_drafts(void* const* caches, const int64_t* strides, int n_caches, const int* lengths, const int* path,
-                           int64_t path_batch_stride, int B, int S, int Hkv, int n, int device, void* cuda_stream);
+int intra_b200_keep_drafts(void* const* caches, const int64_t* strides, int strides_step, int n_caches, const int* lengths,
+                           const int* path, int64_t path_batch_stride, int B, int S, int Hkv, int n, int device, void* cuda_stream);
 
 /* Cuts a cache down to its heaviest keys. Of the lengths[b] (NULL: S; brought into 0 .. S) rows in use of each head, the last
  * `recent` and the heaviest of the others by weights[b][hk][j] stay, `keep` in all, in their order, ties going to the

@@ -38,7 +38,7 @@ SIGNATURES = {
                                   _I64x3, _I64x3, _I64x3, _i64, _i, _I64x3, _f, _i, _vp]),
     "intra_b200_verify_drafts": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _I64x3, _I64x3,
                                       _i64, _i64, _i64, _i, _vp]),
-    "intra_b200_keep_drafts": (_i, [ctypes.POINTER(_vp), _I64x3, _i, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
+    "intra_b200_keep_drafts": (_i, [_vp, _vp, _i, _i, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
     "intra_b200_evict": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _I64x3, _I64x3, _I64x3,
                               _I64x3, _I64x3, _I64x3, _i, _vp]),
     "intra_b200_strerror": (ctypes.c_char_p, [_i]),

@@ -313,15 +313,15 @@ int intra_b200_verify_drafts(const void* tokens, int tokens_int64, const void* t
   return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
 }
 
-int intra_b200_keep_drafts(void* const* caches, const int64_t* strides, int n_caches, const int* lengths, const int* path,
-                           int64_t path_batch_stride, int B, int S, int Hkv, int n, int device, void* cuda_stream) {
-  if (!caches || !strides || !lengths || !path || n_caches <= 0 || B <= 0 || S <= 0 || Hkv <= 0 || n <= 0 || n > S)
+int intra_b200_keep_drafts(void* const* caches, const int64_t* strides, int strides_step, int n_caches, const int* lengths,
+                           const int* path, int64_t path_batch_stride, int B, int S, int Hkv, int n, int device, void* cuda_stream) {
+  if (!caches || !strides || (strides_step != 0 && strides_step != 3) || !lengths || !path || n_caches <= 0 || B <= 0 || S <= 0 || Hkv <= 0 || n <= 0 || n > S)
     return INTRA_ERR_BAD_ARG;
   if (n > KEEP_MAX_TOKENS || int64_t(B) * Hkv > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
   if (!aligned4(lengths) || !aligned4(path)) return INTRA_ERR_ALIGNMENT;
   for (int i = 0; i < n_caches; ++i) {
     if (!caches[i]) return INTRA_ERR_BAD_ARG;
-    const int64_t* s = strides + 3 * i;
+    const int64_t* s = strides + strides_step * i;
     if (s[0] <= 0 || s[1] <= 0 || s[2] <= 0) return INTRA_ERR_BAD_ARG;       // rows that share memory cannot be moved apart
     if (!aligned16(caches[i]) || !rows_aligned(s)) return INTRA_ERR_ALIGNMENT;
   }
@@ -337,7 +337,7 @@ int intra_b200_keep_drafts(void* const* caches, const int64_t* strides, int n_ca
     const int count = imin(n_caches - first, KEEP_TENSORS);
     for (int i = 0; i < count; ++i) {
       p.cache[i] = static_cast<__nv_bfloat16*>(caches[first + i]);
-      p.s[i] = view_of(strides + 3 * (first + i));
+      p.s[i] = view_of(strides + strides_step * (first + i));
     }
     keep_rows_kernel<<<dim3(unsigned(B * Hkv), unsigned(count)), KEEP_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(p);
     const cudaError_t e = cudaGetLastError();

@@ -16,6 +16,7 @@ Forward only; nothing synchronises, nothing is remembered between calls, every c
 """
 from __future__ import annotations
 
+import array
 import ctypes
 
 import torch
@@ -162,7 +163,7 @@ def decode_attn_accumulate(q, k, v, weights, lengths=None, mask=None, softmax_sc
         raise ValueError(f"weights must be float32 (batch, KV heads, at least {S}) on {dev}")
     _no_grad(weights)
     if not (ws[2] == 1 and ws[1] >= wn[2] and ws[0] >= ws[1] * Hkv):     # else look closer
-        _distinct_rows(weights, "weights")
+        _distinct_rows(wn, ws, "weights")
     lengths, used, _ = _integers(lengths, "lengths", (B,), dev)
     ms = None
     if mask is not None:
@@ -183,9 +184,8 @@ def decode_attn_accumulate(q, k, v, weights, lengths=None, mask=None, softmax_sc
     return out
 
 
-def _distinct_rows(x, name):
+def _distinct_rows(shape, strides, name):
     """A tensor that is written needs unit stride in its last dimension and rows that do not share memory."""
-    shape, strides = x.shape, x.stride()
     if strides[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name} needs unit stride in the last dimension")
     reach = shape[-1]
@@ -232,9 +232,9 @@ def verify_drafts(tokens, target_probs, draft_probs, uniform, parents=None):
         if dn[1] == 0:                                       # no drafts
             draft_probs = None
     parents, up, up_stride = _integers(parents, "parents", (B, n), dev, (n,))
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    accepted = uniform.new_empty((B,), dtype=torch.int32)
     path = accepted.new_empty((B, n))
-    out = torch.empty((B, n), dtype=torch.int64, device=dev)
+    out = tokens.new_empty((B, n)) if wide else uniform.new_empty((B, n), dtype=torch.int64)
     if B == 0:
         return accepted, path, out
     if target_probs.stride(2) != 1:
@@ -299,23 +299,26 @@ def keep_drafts(caches, lengths, path):
     if not caches:
         return
     first, count = caches[0], len(caches)
-    dev, shape = first.device, first.shape
-    # what all of them have in common is looked at once
-    if not first.is_cuda or {x.dtype for x in caches} != {torch.bfloat16} or len(shape) != 4 or shape[3] != 128:
+    dev, shape, bf16 = first.device, first.shape, torch.bfloat16
+    index, grad, alike, pointers = dev.index, torch.is_grad_enabled(), first.is_contiguous(), []
+    if not first.is_cuda or len(shape) != 4 or shape[3] != 128:
         raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
-    if any([x.shape != shape for x in caches]) or {x.get_device() for x in caches} != {dev.index}:
-        raise ValueError("caches must agree in shape and device")
-    if torch.is_grad_enabled() and any([x.requires_grad for x in caches]):
-        raise RuntimeError("INTRA kernels are forward-only; call them under torch.no_grad()")
-    pointers, strides = [x.data_ptr() for x in caches], [x.stride() for x in caches]
-    layouts = {}
-    for s, x in zip(strides, caches):
-        if s not in layouts:
-            if not _rows_usable(x):
-                raise ValueError("caches need unit stride in the last dimension and 16-byte aligned rows")
-            _distinct_rows(x, "a cache")
-            layouts[s] = [s[d] if shape[d] > 1 else 8 for d in (0, 2, 1)]
-    if any([p & 15 for p in pointers]):
+    for x in caches:
+        if x.dtype is not bf16:
+            raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
+        if x.shape != shape or x.get_device() != index:
+            raise ValueError("caches must agree in shape and device")
+        if grad and x.requires_grad:
+            raise RuntimeError("INTRA kernels are forward-only; call them under torch.no_grad()")
+        alike = alike and x.is_contiguous()
+        pointers.append(x.data_ptr())
+    layouts = {x.stride() for x in caches} if not alike else {first.stride()}
+    for s in layouts:
+        if s[3] != 1 or (s[0] | s[1] | s[2]) & 7:
+            raise ValueError("caches need unit stride in the last dimension and 16-byte aligned rows")
+        _distinct_rows(shape, s, "a cache")
+    order = sorted(pointers)
+    if any([p & 15 for p in order]):
         raise ValueError("caches need unit stride in the last dimension and 16-byte aligned rows")
     B, Hkv, S, _ = shape
     if len(path.shape) != 2 or not 1 <= path.shape[1] <= min(MAX_TOKENS, S):
@@ -329,12 +332,13 @@ def keep_drafts(caches, lengths, path):
         return
     if count > 1:
         span = _byte_span(first)[1] - pointers[0]
-        order = sorted(pointers)
         if (len(layouts) > 1 or any([b - a < span for a, b in zip(order, order[1:])])) and _overlapping(caches):
             raise ValueError("caches must not share memory")
-    c_strides = (ctypes.c_int64 * (3 * count))(*[st for s in strides for st in layouts[s]])
-    rc = lib.intra_b200_keep_drafts((ctypes.c_void_p * count)(*pointers), c_strides, count, used, nodes, path_stride, B, S, Hkv, n,
-                                    dev.index, _raw_stream(dev.index))
+    # {batch, token, head}, once for all where they are the same; dimensions of one entry get some positive stride
+    strides = [s[d] if shape[d] > 1 else 8 for s in ([first.stride()] if len(layouts) == 1 else [x.stride() for x in caches]) for d in (0, 2, 1)]
+    addresses, c_strides = array.array("Q", pointers), array.array("q", strides)
+    rc = lib.intra_b200_keep_drafts(addresses.buffer_info()[0], c_strides.buffer_info()[0], 0 if len(layouts) == 1 else 3, count, used,
+                                    nodes, path_stride, B, S, Hkv, n, index, _raw_stream(index))
     if rc != 0:
         _raise(rc)
 
@@ -378,10 +382,10 @@ def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
             raise ValueError(f"out needs float32 ({B}, {Hkv}, at least {keep}) for the weights on {dev}")
         _no_grad(k2, v2, w2)
         for x in (k2, v2, w2):
-            _distinct_rows(x, "out")
+            _distinct_rows(x.shape, x.stride(), "out")
         if _overlapping((k2, v2, w2)) or any(_overlapping((x, y)) for x in (k2, v2, w2) for y in (k, v, weights)):
             raise ValueError("out must not overlap the cache: rows are still read while it is written")
-    kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
+    kept = w2.new_empty((B, Hkv, keep), dtype=torch.int32)
     if B > 0 and Hkv > 0:
         ks, vs, ws = k.stride(), v.stride(), weights.stride()
         rc = lib.intra_b200_evict(k.data_ptr(), v.data_ptr(), weights.data_ptr(), used, k2.data_ptr(), v2.data_ptr(),

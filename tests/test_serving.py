@@ -380,6 +380,8 @@ def test_accepted_rows_move_together(B, Hkv, S, n, layers, layout):
                 if 0 <= node < n and lengths[b] <= S - n:
                     y[b, :, lengths[b] + i] = x[b, :, lengths[b] + node]
         want.append(y)
+    if layers == 3:                                          # layouts of two kinds in one call
+        caches[1] = caches[1].transpose(1, 2).contiguous().transpose(1, 2)
     keep_drafts(caches, torch.tensor(lengths, dtype=torch.int32).cuda(), torch.tensor(paths, dtype=torch.int32).cuda())
     for x, y in zip(caches, want):
         assert torch.equal(x, y)
@@ -585,10 +587,10 @@ def test_c_entries_reject_bad_arguments_without_a_gpu(lib):
 
     assert verify(t=None) == verify(n=0) == verify(V=0) == verify(kind=3) == verify(ts=None) == -1 and verify(n=65) == -2 and verify(t=p + 1) == -3
 
-    def keep(ptrs=(p,), n=4, S=8, s=(1024, 128, 128)):
-        return lib.intra_b200_keep_drafts((ctypes.c_void_p * 1)(*ptrs), (ctypes.c_int64 * 3)(*s), 1, p, p, 4, 1, S, 1, n, 0, None)
+    def keep(ptrs=(p,), n=4, S=8, s=(1024, 128, 128), step=3):
+        return lib.intra_b200_keep_drafts((ctypes.c_void_p * 1)(*ptrs), (ctypes.c_int64 * 3)(*s), step, 1, p, p, 4, 1, S, 1, n, 0, None)
 
-    assert keep(ptrs=(None,)) == keep(n=9) == keep(s=(0, 128, 128)) == -1 and keep(n=65, S=70) == -2 and keep(ptrs=(p + 8,)) == -3
+    assert keep(ptrs=(None,)) == keep(n=9) == keep(s=(0, 128, 128)) == keep(step=2) == -1 and keep(n=65, S=70) == -2 and keep(ptrs=(p + 8,)) == -3
 
     def evict(k=p, keep=4, recent=1, out=st):
         return lib.intra_b200_evict(k, p, p, None, p, p, p, p, 1, 8, 1, keep, recent, st, st, st, out, st, st, 0, None)
