@@ -66,35 +66,136 @@ __device__ __forceinline__ const uint32_t* tree_bits(const TreeParams& p, int b,
   return p.bits + (int64_t(b) * p.bits_tokens + (p.bits_tokens == 1 ? 0 : token)) * p.bits_words;
 }
 
-// Where a row's result goes: bf16 into the output where its unit is whole, else fp32.
-struct TreeRowOut {
-  __nv_bfloat16* out;
-  float* part;                 // null: whole
-  int part_step;               // floats between columns
-};
-
-// COLS columns from `col` on of one row of a piece, key by key, for rows whose sums are not finite: an infinite or NaN value row
-// makes every row's sum NaN, also those of tokens that do not see it (zero times infinity). m and l are the row's.
-template <int COLS>
-__device__ __noinline__ void tree_exact_row(const TreeParams& p, const TreePiece& pc, unsigned long long own, int token, int head, int col,
-                                            float m, float l, const TreeRowOut& dst) {
-  float acc[COLS];
-  for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
-  const __nv_bfloat16* const q = p.q + pc.b * p.q_sb + head * p.q_sh + token * p.q_sn;
-  const int last = min((pc.first + pc.count) * TILE_N, pc.n_keys);
-  for (int key = pc.first * TILE_N; key < last; ++key) {
-    if (key >= pc.ctx && !((own >> (key - pc.ctx)) & 1ull)) continue;
-    if (p.bits != nullptr && !((tree_bits(p, pc.b, token)[key >> 5] >> (key & 31)) & 1u)) continue;
-    const __nv_bfloat16* const k = p.k + pc.b * p.ks.sb + pc.hk * p.ks.sh + key * p.ks.ss;
-    const __nv_bfloat16* const v = p.v + pc.b * p.vs.sb + pc.hk * p.vs.sh + key * p.vs.ss + col;
-    float s = 0.f;
-    for (int c = 0; c < HEAD_DIM; ++c) s += __bfloat162float(q[c]) * __bfloat162float(k[c]);
-    const float prob = ptx::ex2(s * p.scale_log2 - m);
-    for (int c = 0; c < COLS; ++c) acc[c] += prob * __bfloat162float(v[c]);
-  }
-  for (int c = 0; c < COLS; ++c) {
-    if (dst.part != nullptr) dst.part[(col + c) * dst.part_step] = acc[c];
-    else dst.out[col + c] = __float2bfloat16(l == 0.f ? 0.f : acc[c] / l);
+// Rows whose sums are not finite, once more: an infinite or NaN value row makes every row's sum NaN, also those of tokens that do
+// not see it (zero times infinity). Called by whole softmax warps, whose lanes hold the maximum and sum of their rows and
+// whether they need it; 16 rows at a time, by warp-level MMAs with operands straight from global memory: finite values as such,
+// others added key by key, each only to the rows that see it. Results go over what was written. 8 sequences of 2 x 4,096 keys
+// of which one holds a NaN: 0.18 ms for 0.063 (one row at a time in 32 bits: 32 ms). Having the call costs the other inputs
+// 1 to 3 %, in registers; hence its few arguments.
+template <bool PAIR>
+__device__ __noinline__ void tree_exact_rows(const TreeUmmaParams& params, const TreePiece& pc, float m, float l, bool redo) {
+  constexpr int COLS = PAIR ? 128 : 64, ROWS = UMMA_ROWS<PAIR>, NT = COLS / 8;
+  const TreeParams& p = params.t;
+  const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3, warp = threadIdx.x >> 5;
+  const int rep = p.H / p.Hkv, all_rows = p.n * rep;
+  const int col = PAIR ? 0 : (warp >> 2) * COLS, at0 = 32 * (PAIR ? warp : warp & 3), r0 = pc.rg * ROWS + at0;
+  float* const part = pc.count != pc.of ? p.scratch + (int64_t(blockIdx.x) * 2 + pc.starts) * UMMA_PARTIAL<PAIR> + at0 : nullptr;
+  const __nv_bfloat16* const kb = p.k + pc.b * p.ks.sb + pc.hk * p.ks.sh;
+  const __nv_bfloat16* const vb = p.v + pc.b * p.vs.sb + pc.hk * p.vs.sh + col;
+  const uint32_t wanted = __ballot_sync(0xffffffffu, redo);
+#pragma unroll 1
+  for (int group = 0; group < 2; ++group) {
+    if (((wanted >> (16 * group)) & 0xffffu) == 0u) continue;
+    int token[2], head[2];
+    float m_row[2], l_row[2];
+    unsigned long long own[2];
+    const uint32_t* mask_row[2] = {nullptr, nullptr};
+    uint32_t qf[8][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = min(r0 + 16 * group + 8 * h + g, all_rows - 1);
+      token[h] = fdiv(r, params.by_rep);
+      head[h] = pc.hk * rep + r - token[h] * rep;
+      m_row[h] = __shfl_sync(0xffffffffu, m, 16 * group + 8 * h + g);
+      l_row[h] = __shfl_sync(0xffffffffu, l, 16 * group + 8 * h + g);
+      own[h] = tree_own_keys(p, pc.b, token[h]);
+      if (p.bits != nullptr) mask_row[h] = tree_bits(p, pc.b, token[h]);
+      const uint32_t* const q = reinterpret_cast<const uint32_t*>(p.q + pc.b * p.q_sb + head[h] * p.q_sh + token[h] * p.q_sn) + j;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        qf[t][h] = q[8 * t];
+        qf[t][2 + h] = q[8 * t + 4];
+      }
+    }
+    float o[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+    const int last = min((pc.first + pc.count) * TILE_N, pc.n_keys);
+#pragma unroll 1
+    for (int key0 = pc.first * TILE_N; key0 < last; key0 += 16) {
+      float s[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        const uint32_t* const k = reinterpret_cast<const uint32_t*>(kb + int64_t(min(key0 + 8 * n + g, last - 1)) * p.ks.ss) + j;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) mma_m16n8k16(s[n], qf[t][0], qf[t][1], qf[t][2], qf[t][3], k[8 * t], k[8 * t + 4]);
+      }
+      uint32_t seen[2], hi[4], lo[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = key0 - pc.ctx;
+        seen[h] = (last - key0 >= 16 ? 0xffffu : (1u << (last - key0)) - 1u) &
+                  (at >= 0 ? (at < 64 ? uint32_t(own[h] >> at) : 0u) : at <= -16 ? 0xffffu : uint32_t(own[h] << -at) | ((1u << -at) - 1u));
+        if (p.bits != nullptr) seen[h] &= mask_row[h][key0 >> 5] >> (key0 & 31);
+        float pr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = 2 * j + (i & 1) + 8 * (i >> 1);
+          pr[i] = (seen[h] >> key) & 1u ? ptx::ex2(s[i >> 1][2 * h + (i & 1)] * p.scale_log2 - m_row[h]) : 0.f;
+        }
+        split_bf16(pr[0], pr[1], hi[h], lo[h]);
+        split_bf16(pr[2], pr[3], hi[2 + h], lo[2 + h]);
+      }
+      bool odd = false;                                   // some value is not finite
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        uint32_t b[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = key0 + 8 * n + 2 * j + e;
+            const uint32_t x = key < last ? reinterpret_cast<const uint16_t*>(vb + int64_t(key) * p.vs.ss)[8 * t + g] : 0u;
+            const bool fine = (x & 0x7f80u) != 0x7f80u;
+            odd = odd || !fine;
+            w |= fine ? x << (16 * e) : 0u;
+          }
+          b[n] = w;
+        }
+        mma_m16n8k16(o[t], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
+        mma_m16n8k16(o[t], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
+      }
+      if (!__any_sync(0xffffffffu, odd)) continue;
+      bool all_nan = true;
+#pragma unroll 1
+      for (int c = 0; c < 16 && key0 + c < last; ++c) {
+        const int from = (lane & ~3) | ((c & 7) >> 1);    // the lane that has this key's probabilities
+        const uint32_t* const v = reinterpret_cast<const uint32_t*>(vb + int64_t(key0 + c) * p.vs.ss) + j;
+        all_nan = true;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t ph = __shfl_sync(0xffffffffu, c < 8 ? hi[h] : hi[2 + h], from);
+          const float prob = __uint_as_float(c & 1 ? ph & 0xffff0000u : ph << 16);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const uint32_t w = v[4 * t];
+            if (((seen[h] >> c) & 1u) && (w & 0x7f80u) == 0x7f80u) o[t][2 * h] += prob * __uint_as_float(w << 16);
+            if (((seen[h] >> c) & 1u) && (w & 0x7f800000u) == 0x7f800000u) o[t][2 * h + 1] += prob * __uint_as_float(w & 0xffff0000u);
+            all_nan = all_nan && isnan(o[t][2 * h]) && isnan(o[t][2 * h + 1]);
+          }
+        }
+      }
+      if (__all_sync(0xffffffffu, all_nan)) break;        // nothing changes any more
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = 16 * group + 8 * h + g;
+      if (r0 + i >= all_rows) continue;
+      const float inv = l_row[h] == 0.f ? 0.f : 1.f / l_row[h];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int c = col + 8 * t + 2 * j;
+        if (part != nullptr) {
+          part[c * ROWS + i] = o[t][2 * h];
+          part[(c + 1) * ROWS + i] = o[t][2 * h + 1];
+        } else {
+          *reinterpret_cast<uint32_t*>(p.o + ((int64_t(pc.b) * p.n + token[h]) * p.H + head[h]) * HEAD_DIM + c) =
+              ptx::pack_bf16(o[t][2 * h] * inv, o[t][2 * h + 1] * inv);
+        }
+      }
+    }
   }
 }
 
@@ -361,12 +462,13 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
       };
       bool finite = true;
       if (busy) {
-        TreeRowOut dst = {t.o + ((int64_t(pc.b) * t.n + token) * t.H + head) * HEAD_DIM, nullptr, ROWS};
+        __nv_bfloat16* const out = t.o + ((int64_t(pc.b) * t.n + token) * t.H + head) * HEAD_DIM;
+        float* part = nullptr;                            // column c of the row at part[c * ROWS]
         if (pc.count != pc.of) {
-          float* const part = t.scratch + (int64_t(blockIdx.x) * 2 + pc.starts) * UMMA_PARTIAL<PAIR>;
+          part = t.scratch + (int64_t(blockIdx.x) * 2 + pc.starts) * UMMA_PARTIAL<PAIR>;
           const int at = r - pc.rg * ROWS;
-          dst.part = part + at;
           if (valid && col == 0) reinterpret_cast<float2*>(part + int64_t(ROWS) * HEAD_DIM)[at] = make_float2(m, l);
+          part += at;
         }
         const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
 #pragma unroll 1
@@ -376,18 +478,21 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
 #pragma unroll
           for (int e = 0; e < 32; ++e) finite = finite && fabsf(o[e]) < CUDART_INF_F;
           if (!valid) continue;
-          if (dst.part != nullptr) {
+          if (part != nullptr) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) dst.part[(col + c + e) * ROWS] = o[e];
+            for (int e = 0; e < 32; ++e) part[(col + c + e) * ROWS] = o[e];
           } else {
-            uint4* const d = reinterpret_cast<uint4*>(dst.out + col + c);
+            uint4* const d = reinterpret_cast<uint4*>(out + col + c);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               d[e] = make_uint4(ptx::pack_bf16(o[8 * e] * inv, o[8 * e + 1] * inv), ptx::pack_bf16(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
                                 ptx::pack_bf16(o[8 * e + 4] * inv, o[8 * e + 5] * inv), ptx::pack_bf16(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
           }
         }
-        if (valid && !finite) tree_exact_row<COLS>(t, pc, own, token, head, col, m, l, dst);       // over what was just written
+        if (__any_sync(0xffffffffu, valid && !finite)) {
+          __syncwarp();
+          tree_exact_rows<PAIR>(p, pieces[warp], m, l, valid && !finite);
+        }
       }
       ptx::tc_fence_before();
       __syncwarp();
