@@ -3,6 +3,7 @@
     python -m intra_b200.bench_kernel llm   [--seqlens 4096,...] [--groups 2,8] [--out file.json]
     python -m intra_b200.bench_kernel image [--out file.json]
     python -m intra_b200.bench_kernel stack [--seqlens 32768] [--layers 32] [--out file.json]
+    python -m intra_b200.bench_kernel serve [--seqlens 4096,...] [--batch 1] [--drafts 8] [--out file.json]
 
 Same flags, same protocol (CUDA events around each call, 10 warm-ups, median of 50) and the same row
 keys as the reference's benchmarks/results/*.json, so B200 rows can sit next to its A100 ones; each
@@ -23,6 +24,13 @@ reference's table does (benchmarks/bench_kernel.py:67): `--layers` attention cal
 on its own seeded q/k/v (seed 1000 + l), Scatter G=2 on every eighth layer and window 576 on the others,
 timed as one region with CUDA events, against the same number of dense causal SDPA calls on the same
 tensors.
+
+`serve` times what a server runs between two tokens of an answer on caches of `--seqlens` rows: `tree`, attention of the last token
+and `--drafts` drafted ones, beside `dense`, SDPA with the same boolean mask and K/V expanded to the query heads; `verify` over
+`--vocab` entries; `keep`, the accepted rows of K and V of `--layers` layers; `step`, these one after the other, `--layers`
+attention calls among them, each on its own cache; `decode_weights`, a decode step that accumulates what each key receives, beside
+`decode`, one that does not; `evict`, a cache cut to a quarter. `<key>_gbs` is the bytes that an attention call has to read, over
+its time. The reference has no counterpart.
 """
 from __future__ import annotations
 
@@ -33,7 +41,7 @@ import statistics
 import torch
 import torch.nn.functional as F
 
-from . import intra_image_attn, intra_llm_attn
+from . import decode_attn_accumulate, evict_cache, intra_image_attn, intra_llm_attn, keep_drafts, tree_attn, verify_drafts
 
 TEXT_LEN = 512
 
@@ -245,14 +253,70 @@ def bench_stack(args):
     return rows
 
 
+@torch.no_grad()
+def bench_serve(args):
+    from .interface import decode_attn
+    B, H, Hkv, n = args.batch, args.heads, args.kv_heads, args.drafts + 1
+    rows = []
+    g = torch.Generator(device="cuda").manual_seed(2000)
+    parents = torch.tensor([i - 1 if i < 2 else (i - 1) // 2 for i in range(n)], dtype=torch.int32, device="cuda")  # two children a node
+    sees = torch.eye(n, dtype=torch.bool)
+    for i, follows in enumerate(parents.tolist()):
+        if follows >= 0:
+            sees[i] |= sees[follows]
+    target = torch.softmax(4 * torch.randn(B, n, args.vocab, device="cuda", generator=g), -1)
+    draft = torch.softmax(4 * torch.randn(B, n, args.vocab, device="cuda", generator=g), -1)
+    drafts = torch.randint(args.vocab, (B, n), device="cuda", generator=g)
+    uniform = torch.rand(B, n, device="cuda", generator=g)
+    for S in args.seqlens:
+        if S < n:
+            raise ValueError(f"a cache of {S} rows has no room for {n} tokens")
+        caches = [randn(B, Hkv, S, 128) for _ in range(2 * args.layers)]
+        q, q1 = randn(B, H, n, 128), randn(B, H, 1, 128)
+        lengths = torch.full((B,), S - n, dtype=torch.int32, device="cuda")
+        weights = torch.zeros(B, Hkv, S, device="cuda")
+        mask = torch.cat([torch.ones(n, S - n, dtype=torch.bool), sees], 1).cuda()
+        k, v = caches[:2]
+
+        def dense():
+            rep = H // Hkv
+            kx, vx = (x.repeat_interleave(rep, 1) if rep > 1 else x for x in (k, v))
+            return F.scaled_dot_product_attention(q, kx, vx, attn_mask=mask)
+
+        def step():
+            for layer in range(args.layers):
+                tree_attn(q, caches[2 * layer], caches[2 * layer + 1], parents, lengths)
+            keep_drafts(caches, lengths, verify_drafts(drafts, target, draft, uniform, parents)[1])
+
+        path = verify_drafts(drafts, target, draft, uniform, parents)[1]
+        calls = {"dense": dense,
+                 "tree": lambda: tree_attn(q, k, v, parents, lengths),
+                 "verify": lambda: verify_drafts(drafts, target, draft, uniform, parents),
+                 "keep": lambda: keep_drafts(caches, lengths, path),
+                 "step": step,
+                 "decode": lambda: decode_attn(q1, k, v),
+                 "decode_weights": lambda: decode_attn_accumulate(q1, k, v, weights),
+                 "evict": lambda: evict_cache(k, v, weights, max(1, S // 4), S // 16)}
+        r = {"seqlen": S}
+        for key, call in calls.items():
+            r[key] = median_ms(call, args.warmup, args.iters)
+            if key in ("tree", "decode", "decode_weights"):
+                r[key + "_gbs"] = (k.nbytes + v.nbytes + (2 * weights.nbytes if key == "decode_weights" else 0)) / r[key] / 1e6
+        rows.append(r)
+        print("  ".join(f"{a}={b:.3f}" if isinstance(b, float) else f"{a}={b}" for a, b in r.items()), flush=True)
+    return rows
+
+
 def main():
     p = argparse.ArgumentParser()
-    p.add_argument("mode", choices=["llm", "image", "stack"])
+    p.add_argument("mode", choices=["llm", "image", "stack", "serve"])
     p.add_argument("--layers", type=int, default=32)
     p.add_argument("--stack-iters", type=int, default=5)
     p.add_argument("--seqlens", default="4096,8192,16384,32768,65536")
     p.add_argument("--groups", default="2,8")
     p.add_argument("--batch", type=int, default=1)
+    p.add_argument("--drafts", type=int, default=8)
+    p.add_argument("--vocab", type=int, default=131072)
     p.add_argument("--heads", type=int, default=32)
     p.add_argument("--kv-heads", type=int, default=8)
     p.add_argument("--image-heads", type=int, default=24)
@@ -267,7 +331,7 @@ def main():
     print(f"device: {torch.cuda.get_device_name()}  torch {torch.__version__}")
     if args.mode == "stack" and args.seqlens == [4096, 8192, 16384, 32768, 65536]:
         args.seqlens = [32768]
-    rows = {"llm": bench_llm, "image": bench_image, "stack": bench_stack}[args.mode](args)
+    rows = {"llm": bench_llm, "image": bench_image, "stack": bench_stack, "serve": bench_serve}[args.mode](args)
     if args.out:
         with open(args.out, "w") as f:
             json.dump({"device": torch.cuda.get_device_name(), "torch": torch.__version__,

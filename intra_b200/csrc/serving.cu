@@ -283,7 +283,7 @@ int intra_b200_verify_drafts(const void* tokens, int tokens_int64, const void* t
   if (!tokens || !target || !uniform || !accepted || !path || !out_tokens || !target_strides || (draft && !draft_strides) ||
       B <= 0 || n <= 0 || V <= 0 || prob_type < 0 || prob_type > 2)
     return INTRA_ERR_BAD_ARG;
-  if (n > VERIFY_MAX_TOKENS || B > 0x7fffffff / VERIFY_MAX_CLUSTER) return INTRA_ERR_UNSUPPORTED;
+  if (n > VERIFY_MAX_TOKENS || V > VERIFY_MAX_VOCABULARY || B > 0x7fffffff / VERIFY_MAX_CLUSTER) return INTRA_ERR_UNSUPPORTED;
   const uintptr_t size = prob_type == INTRA_PROB_F32 ? 4 : 2, token_size = tokens_int64 ? 8 : 4;
   if (reinterpret_cast<uintptr_t>(target) % size || reinterpret_cast<uintptr_t>(draft) % size || !aligned4(uniform) ||
       !aligned4(parents) || !aligned4(accepted) || !aligned4(path) || reinterpret_cast<uintptr_t>(out_tokens) % 8 ||

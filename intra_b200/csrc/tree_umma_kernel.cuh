@@ -13,9 +13,9 @@
 //
 // Warp roles (512 threads): warps 0-3 and 4-7 softmax sets of the streams, a thread owning a row, which also write
 // the results; 8-11 request the tiles: TMA where a tile's rows are all keys of the sequence and the cache's strides
-// allow, else 16-byte copies in which rows past its last key, and rows no token sees, become zeros; 12 issues QK^T (and, but for PAIR, PV), 13 PV;
-// 14 and 15 bring the query rows of the units after the first, whose rows the softmax sets fetch. Whoever writes operands by plain copies fences them for the tensor cores' proxy before it
-// reports them.
+// allow, else 16-byte copies in which rows past its last key, and rows no token sees, become zeros; 12 issues QK^T (and, but
+// for PAIR, PV), 13 PV; 14 and 15 bring the query rows of the units after the first, whose rows the softmax sets fetch.
+// Whoever writes operands by plain copies fences them for the tensor cores' proxy before it reports them.
 //
 // Barriers, all waits bounded (2 s; see attn_kernel.cuh for what a CTA does that gives up):
 //   full[r], free[r]   ring of tile buffers, in the order K0 K1 V0 K2 V1 .. over the CTA's tiles

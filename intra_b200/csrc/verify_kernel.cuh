@@ -6,10 +6,10 @@
 //
 //   R <- max(R - Z q, 0),  Z <- sum R            (both stay where nothing would be left),
 //
-// so that tokens come out distributed as p whatever q is (R / Z is the target's distribution given the rejections). When no child is accepted the walk ends, and one more token
-// is drawn from R: the smallest t with R(0) + .. + R(t) > u_0 sum R. Drafts without a distribution count as
-// certain: q is one at their token. All of it in 64 bits: an error of 2^-24 in a running sum over 10^5 tokens decides
-// the token in one draw of a hundred, 2^-53 in none.
+// so that tokens come out distributed as p whatever q is (R / Z is the target's distribution given the rejections). When no child is
+// accepted the walk ends, and one more token is drawn from R: the smallest t with R(0) + .. + R(t) > u_0 sum R. Drafts
+// without a distribution count as certain: q is one at their token. All of it in 64 bits: an error of 2^-24 in a running
+// sum over 10^5 tokens decides the token in one draw of a hundred, 2^-53 in none.
 //
 // A sequence is a thread-block cluster; each CTA holds a contiguous part of the vocabulary, each warp a contiguous part of
 // that. Every CTA walks the tree by itself, from the n probabilities of the drafted tokens, fetched at once; only a
@@ -33,6 +33,7 @@
 namespace intra {
 
 constexpr int VERIFY_MAX_TOKENS = 64;
+constexpr int VERIFY_MAX_VOCABULARY = 1 << 30;   // places in a row, with what a CTA's parts round up, fit 31 bits
 constexpr int VERIFY_THREADS = 512;
 constexpr int VERIFY_WARPS = VERIFY_THREADS / 32;
 constexpr int VERIFY_MAX_CLUSTER = 8;
@@ -127,7 +128,8 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const __grid_
   auto left_at = [&](int t, int count) {
     return left(as_double(p_row[t]), draft != nullptr && count > 0 ? as_double(q_row[t]) : 0.0, t, count);
   };
-  // The current row's granules, the first of which begins `off` tokens before token 0, and those of a warp.
+  // The current row's granules, the first of which begins `off` tokens before token 0, and those of a warp. They lie on 16-byte
+  // boundaries and each holds a token of the row, so none leaves the row's memory page; what else they hold is not used.
   int off = 0, per_warp = 0, granules = 0;
   const uint32_t slots = ptx::smem_u32(verify_smem) + tid * 16;
   constexpr uint32_t SLOT = VERIFY_THREADS * 16;
