@@ -152,10 +152,14 @@ int launch_tree_umma(const TreeParams& t, const ServingState& st, int64_t scratc
   const int64_t parts = (tiles + UMMA_MIN_TILES - 1) / UMMA_MIN_TILES;
   const int64_t rows = int64_t(B) * t.n * t.H;
   const int64_t places = tiles + int64_t(B) * t.Hkv * p.t.row_groups * UMMA_UNIT_COST<PAIR>;
-  const int64_t merge_ctas = int64_t(B) * t.Hkv * p.t.row_groups * UMMA_MERGE_CTAS<PAIR>;
+  const int row_blocks = ceil_div(imin(t.n * (t.H / t.Hkv), UMMA_ROWS<PAIR>), 32);
+  const bool split = int64_t(B) * t.Hkv * p.t.row_groups * UMMA_MERGE_FEW < st.sm_count;      // many parts a unit
+  const int64_t merge_ctas = int64_t(B) * t.Hkv * p.t.row_groups * row_blocks * (split ? UMMA_MERGE_CTAS<4, 2> : UMMA_MERGE_CTAS<8, 1>);
   if (places + st.sm_count > 0x7fffffffLL || rows > 0x7fffffffLL || merge_ctas > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
-  const int grid = parts < st.sm_count ? int(parts) : st.sm_count;
+  const int64_t units = int64_t(B) * t.Hkv * p.t.row_groups, ctas = parts > units ? parts : units;
+  const int grid = ctas < st.sm_count ? int(ctas) : st.sm_count;
   p.t.unit_cost = UMMA_UNIT_COST<PAIR>;
+  p.t.split_cost = umma_split_cost(imin(t.n * (t.H / t.Hkv), UMMA_ROWS<PAIR>));
   p.t.min_tiles = UMMA_MIN_TILES;
   *scratch_needed = grid * 2 * UMMA_PARTIAL<PAIR> * int64_t(sizeof(float));
   if (t.mask) {                   // behind the partial results: the mask's bits, those of any token, the tiles
@@ -178,8 +182,12 @@ int launch_tree_umma(const TreeParams& t, const ServingState& st, int64_t scratc
   if (e == cudaSuccess)
     e = t.mask ? launch_early(tree_umma_kernel<PAIR, true>, dim3(unsigned(grid)), UMMA_THREADS, UMMA_SMEM_BYTES<PAIR>, stream, p)
                : launch_early(tree_umma_kernel<PAIR, false>, dim3(unsigned(grid)), UMMA_THREADS, UMMA_SMEM_BYTES<PAIR>, stream, p);
+  // Nothing to join where all sequences are alike and their units are dealt whole.
+  if (!t.lengths && !t.mask && tree_whole(uint32_t(units), uint32_t(tiles), ceil_div(t.S, TILE_N), grid, p.t.split_cost))
+    return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
   if (e == cudaSuccess)
-    e = launch_early(tree_umma_merge_kernel<PAIR>, dim3(unsigned(merge_ctas)), 32 * UMMA_MERGE_WARPS, 0, stream, p, uint32_t(grid));
+    e = launch_early(split ? tree_umma_merge_kernel<PAIR, 4, 2> : tree_umma_merge_kernel<PAIR, 8, 1>, dim3(unsigned(merge_ctas)),
+                     32 * UMMA_MERGE_WARPS, 0, stream, p, uint32_t(grid), row_blocks);
   return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
 }
 

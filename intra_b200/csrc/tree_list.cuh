@@ -43,6 +43,7 @@ struct TreeParams {
   int S, H, Hkv, n, B;
   int row_groups;              // units per KV head
   int unit_cost, min_tiles;    // see TreeList; a CTA's part is at least this many tiles
+  int split_cost;              // tiles a CTA may have more where in return no unit is divided
   float scale_log2;
 };
 
@@ -84,34 +85,46 @@ __device__ __forceinline__ int tree_tiles(const TreeParams& p, int b, int* first
   return hi - lo;
 }
 
+// Are `units` units of at most `longest` tiles, `tiles` in all, dealt whole? See TreeList.
+__host__ __device__ __forceinline__ bool tree_whole(uint32_t units, uint32_t tiles, uint32_t longest, uint32_t grid, int split_cost) {
+  return split_cost > 0 && uint64_t((units + grid - 1) / grid) * longest <= uint64_t(tiles / grid) + split_cost;
+}
+
 // The list of all units' key tiles. A unit counts for `cost` places more than it has tiles, in front of them: what the end
 // of one unit and the start of the next cost the CTA that has both (parts of a few tiles would only be spread unevenly by
-// it). At most 2^31 - 1 places.
+// it). Where CTAs that each take the same number of whole units are done about as early as with parts of equal size - by
+// p.split_cost tiles, what partial results and their merge take - the list is dealt so: every unit then has as many places as the
+// longest. At most 2^31 - 1 places.
 template <int KEYS>
 struct TreeList {
   uint32_t units, cost, per, total;      // units per sequence; places of a CTA's part, of all
-  // Called by whole warps; all lanes get the same. `before`: tiles and units of sequences before `b`.
+  uint32_t even;                         // places of every unit, 0: units are divided
+  __device__ __forceinline__ uint32_t places(uint32_t tiles) const { return even ? even : tiles + cost; }
+  // Called by whole warps; all lanes get the same. `before`: places of sequences before `b`.
   __device__ __forceinline__ TreeList(const TreeParams& p, int B, uint32_t grid, int b = 0, uint32_t* before = nullptr) {
     units = p.Hkv * p.row_groups;
-    uint32_t tiles = 0, front = 0;
+    uint32_t tiles = 0, front = 0, longest = 0;
     if (p.lengths == nullptr && p.live == nullptr) {               // all sequences alike
-      tiles = uint32_t(B) * uint32_t(tree_tiles<KEYS>(p, 0));
-      front = uint32_t(b) * uint32_t(tree_tiles<KEYS>(p, 0));
+      longest = uint32_t(tree_tiles<KEYS>(p, 0));
+      tiles = uint32_t(B) * longest;
+      front = uint32_t(b) * longest;
     } else {
       for (int s = threadIdx.x & 31; s < B; s += 32) {
         const uint32_t n = tree_tiles<KEYS>(p, s);
         tiles += n;
         front += s < b ? n : 0u;
+        longest = max(longest, n);
       }
       tiles = __reduce_add_sync(0xffffffffu, tiles);
       front = __reduce_add_sync(0xffffffffu, front);
+      longest = __reduce_max_sync(0xffffffffu, longest);
     }
     const uint32_t share = tiles * units / grid;
+    even = tree_whole(units * B, tiles * units, longest, grid, p.split_cost) ? longest : 0;
     cost = share < 8 ? 0 : share < 16 ? min(p.unit_cost, 1) : p.unit_cost;
-    total = (tiles + cost * B) * units;
-    per = (total + grid - 1) / grid;
-    per = max(per, uint32_t(p.min_tiles));
-    if (before) *before = (front + cost * b) * units;
+    total = (even ? even * B : tiles + cost * B) * units;
+    per = even ? (units * B + grid - 1) / grid * even : max((total + grid - 1) / grid, uint32_t(p.min_tiles));
+    if (before) *before = (even ? even * b : front + cost * b) * units;
   }
 };
 
@@ -121,7 +134,7 @@ template <int KEYS>
 struct TreeWalk {
   uint32_t next, end;
   uint32_t b_start;            // place of sequence b's first unit
-  uint32_t units, cost;
+  uint32_t units, cost, even;
   int b, b_tiles, b_first;     // of one unit: its tiles, the first of them
   // Called by whole warps; all lanes get the same.
   __device__ __forceinline__ void start(const TreeParams& p, int B, uint32_t cta, uint32_t grid) {
@@ -129,13 +142,14 @@ struct TreeWalk {
     const TreeList<KEYS> list(p, B, grid);
     units = list.units;
     cost = list.cost;
+    even = list.even;
     next = list.per * cta < list.total ? list.per * cta : list.total;
     end = list.total - next > list.per ? next + list.per : list.total;
     b = b_tiles = b_first = 0;
     b_start = 0;
     if (next >= end) return;
     for (int s0 = 0; s0 < B; s0 += 32) {                           // the sequence that holds `next`
-      const uint32_t mine = s0 + lane < B ? (uint32_t(tree_tiles<KEYS>(p, s0 + lane)) + cost) * units : 0u;
+      const uint32_t mine = s0 + lane < B ? list.places(tree_tiles<KEYS>(p, s0 + lane)) * units : 0u;
       uint32_t upto = mine;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
@@ -155,16 +169,17 @@ struct TreeWalk {
   __device__ __forceinline__ void piece(const TreeParams& p, TreePiece& x) {
     x.count = 0;
     while (next < end) {
-      uint32_t places = b_tiles + cost;
+      uint32_t places = even ? even : b_tiles + cost;
       if (next - b_start >= places * units) {
         b_start += places * units;
         b_tiles = tree_tiles<KEYS>(p, ++b, &b_first);
-        places = b_tiles + cost;
+        places = even ? even : b_tiles + cost;
       }
       const uint32_t local = next - b_start, unit = local / places, at = local - unit * places;
       const uint32_t take = min(end - next, places - at);
       next += take;
-      const int first = max(int(at) - int(cost), 0), last = int(at + take) - int(cost);
+      const int in_front = int(places) - b_tiles;                  // places without tiles
+      const int first = max(int(at) - in_front, 0), last = int(at + take) - in_front;
       if (last <= first) continue;                                 // of this unit only places without tiles
       x.b = b;
       x.hk = p.row_groups == 1 ? unit : unit / p.row_groups;

@@ -386,7 +386,7 @@ struct TreeParts {
     uint32_t start;
     const TreeList<TREE_BLOCK> list(p, p.B, grid, b, &start);
     const int tiles = tree_tiles<TREE_BLOCK>(p, b);
-    start += uint32_t(in_b) * (tiles + list.cost) + list.cost;     // place of the unit's first tile
+    start += uint32_t(in_b + 1) * list.places(tiles) - tiles;      // place of the unit's first tile
     first = int(start / list.per);
     count = int((start + tiles - 1) / list.per) - first + 1;
   }

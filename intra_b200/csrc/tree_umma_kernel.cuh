@@ -53,6 +53,14 @@ constexpr int UMMA_MIN_TILES = 2;
 // tokens over 8 sequences of 4096 to 8192 keys 59.8 / 59.2 / 67.8.
 template <bool PAIR> constexpr int UMMA_UNIT_COST = PAIR ? 3 : 1;
 
+// Tiles that partial results and their merge are worth. Measured, us, dealt in equal parts / in whole units:
+//   rows of a unit                               32          96         256
+//   128 units of 32 tiles (27.7 a CTA)    63.3 / 61.8 72.4 / 64.8 96.7 / 78.1
+//   128 units of 8 tiles (6.9)            33.3 / 26.7 40.4 / 29.9 59.7 / 37.6
+//   96 units of 32 tiles (20.8)           51.9 / 58.9 59.4 / 62.1 76.4 / 72.5
+//   72 units of 64 tiles (31.1)          66.2 / 100.5 73.6 / 103.2 91.6 / 116.2
+constexpr int umma_split_cost(int rows) { return 4 + rows / 24; }
+
 struct TreeUmmaParams {
   TreeParams t;                // row_groups: units per KV head
   FastDiv by_rep;              // query heads per KV head
@@ -238,7 +246,6 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
   }
   if (warp == 8 && lane < 2) ptx::prefetch_tensormap(&p.maps[lane]);
   cudaGridDependencySynchronize();                       // what is above ran beside the end of the kernel before this one
-  cudaTriggerProgrammaticLaunchCompletion();             // the merge may be set up; it waits for this kernel's end by itself
   TreeWalk<TILE_N>& walk = walks[warp];
   const TreePiece& pc = pieces[warp];
   {
@@ -696,70 +703,120 @@ __global__ void __launch_bounds__(32 * TREE_MASK_ROWS) tree_mask_kernel(const __
   }
 }
 
-// Joins the partial results of units that several CTAs had a part of. A thread has UMMA_MERGE_COLS columns of a row, a
-// warp 32 rows. Loads of rows that do not exist stay inside the buffer and are not used.
-constexpr int UMMA_MERGE_COLS = 4, UMMA_MERGE_WARPS = 4;
-constexpr int UMMA_MERGE_SPLIT = HEAD_DIM / (UMMA_MERGE_COLS * UMMA_MERGE_WARPS);       // CTAs per 32 rows
-template <bool PAIR> constexpr int UMMA_MERGE_CTAS = UMMA_ROWS<PAIR> / 32 * UMMA_MERGE_SPLIT;      // per unit
-template <bool PAIR>
-__global__ void __launch_bounds__(32 * UMMA_MERGE_WARPS) tree_umma_merge_kernel(const __grid_constant__ TreeUmmaParams p, uint32_t grid) {
-  constexpr int ROWS = UMMA_ROWS<PAIR>;
+// Joins the partial results of units that several CTAs had a part of. A thread has four rows and COLS columns, a warp 32 rows and
+// four times as many columns, and every SPLIT-th part; AT_ONCE parts' loads are under way together. What takes time is the
+// loads' latency, so with units of many parts two warps share them (COLS 4, SPLIT 2), and where there are more units one
+// warp has as much of two parts as it can hold (COLS 8, SPLIT 1). 32 rows: 8 units of 18 parts, the whole call 61.5 us against 68.1 with
+// the other form; 128 rows, 96 units of 2 or 3: 55.3 against 81.6 with (2, 4); a thread with one row and scalar loads 62.8.
+// `row_blocks`: 32-row blocks of a unit. Loads of rows that do not exist stay inside the buffer and are not used.
+constexpr int UMMA_MERGE_WARPS = 4;
+constexpr int UMMA_MERGE_FEW = 4;                // parts a unit up to which a warp takes them all
+template <int COLS, int SPLIT> constexpr int UMMA_MERGE_CTAS = HEAD_DIM / (4 * COLS * UMMA_MERGE_WARPS / SPLIT);      // per 32 rows
+template <bool PAIR, int COLS, int SPLIT>
+__global__ void __launch_bounds__(32 * UMMA_MERGE_WARPS) tree_umma_merge_kernel(const __grid_constant__ TreeUmmaParams p, uint32_t grid, int row_blocks) {
+  constexpr int ROWS = UMMA_ROWS<PAIR>, CTAS = UMMA_MERGE_CTAS<COLS, SPLIT>, AT_ONCE = COLS == 8 ? 2 : 4;
+  __shared__ float joined[SPLIT > 1 ? UMMA_MERGE_WARPS : 1][SPLIT > 1 ? 4 * (COLS + 2) : 1][32];
   const TreeParams& t = p.t;
-  const int lane = threadIdx.x & 31, rep = t.H / t.Hkv;
-  const int unit = blockIdx.x / UMMA_MERGE_CTAS<PAIR>, block = blockIdx.x - unit * UMMA_MERGE_CTAS<PAIR>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rep = t.H / t.Hkv;
+  const int block = blockIdx.x / CTAS, col_block = blockIdx.x - block * CTAS;
+  const int unit = block / row_blocks, block_row = (block - unit * row_blocks) * 32, at = block_row + (lane & 7) * 4;
   const int units = t.Hkv * t.row_groups, b = unit / units, in_b = unit - b * units;
   const int hk = in_b / t.row_groups, rg = in_b - hk * t.row_groups;
-  const int at = block / UMMA_MERGE_SPLIT * 32 + lane, row = rg * ROWS + at;
-  const int col = (block % UMMA_MERGE_SPLIT * UMMA_MERGE_WARPS + (threadIdx.x >> 5)) * UMMA_MERGE_COLS;
-  if (row - lane >= t.n * rep) return;                    // no such rows
+  const int col = ((col_block * (UMMA_MERGE_WARPS / SPLIT) + warp / SPLIT) * 4 + (lane >> 3)) * COLS;
+  if (rg * ROWS + block_row >= t.n * rep) return;         // the last row group's blocks without rows
   uint32_t start;
   const TreeList<TILE_N> list(t, t.B, grid, b, &start);
   const int tiles = tree_tiles<TILE_N>(t, b);
-  start += uint32_t(in_b) * (tiles + list.cost) + list.cost;       // place of the unit's first tile
+  start += uint32_t(in_b + 1) * list.places(tiles) - tiles;        // place of the unit's first tile
   const int c0 = int(start / list.per), c1 = int((start + tiles - 1) / list.per);
   cudaGridDependencySynchronize();                        // everything before this ran beside the main kernel's end
   if (c0 == c1) return;                                   // one CTA held the unit and wrote its rows
   // The part in the CTA the unit begins in is that CTA's second slot, in the others the first.
   const float* const first = t.scratch + (int64_t(c0) * 2 + 1) * UMMA_PARTIAL<PAIR>;
-  auto slot = [&](int i) { return first + (i == 0 ? 0 : (int64_t(i) * 2 - 1) * UMMA_PARTIAL<PAIR>); };
-  auto ml = [&](int i) { return reinterpret_cast<const float2*>(slot(i) + ROWS * HEAD_DIM)[at]; };
   const int parts = c1 - c0 + 1;
-  float acc[UMMA_MERGE_COLS];
+  float m_all[4], l_all[4], acc[COLS][4];                 // [column][row]
 #pragma unroll
-  for (int e = 0; e < UMMA_MERGE_COLS; ++e) acc[e] = 0.f;
-  float m_all = -CUDART_INF_F, l_all = 0.f;
-  constexpr int AT_ONCE = 8;                              // parts whose loads are under way together
-  for (int i0 = 0; i0 < parts; i0 += AT_ONCE) {           // running maximum over batches of parts
-    float2 x[AT_ONCE];
-    float o[AT_ONCE][UMMA_MERGE_COLS];
+  for (int r = 0; r < 4; ++r) {
+    m_all[r] = -CUDART_INF_F;
+    l_all[r] = 0.f;
 #pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      const int c = min(i0 + i, parts - 1);
-      x[i] = ml(c);
-#pragma unroll
-      for (int e = 0; e < UMMA_MERGE_COLS; ++e) o[i][e] = slot(c)[(col + e) * ROWS + at];
-    }
-    float m_new = m_all;
-#pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) m_new = fmaxf(m_new, x[i].x);
-    const float alpha = merge_weight(m_all, m_new);
-    l_all *= alpha;
-#pragma unroll
-    for (int e = 0; e < UMMA_MERGE_COLS; ++e) acc[e] *= alpha;
-#pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      const float f = i0 + i < parts ? merge_weight(x[i].x, m_new) : 0.f;
-      l_all += i0 + i < parts ? f * x[i].y : 0.f;
-#pragma unroll
-      for (int e = 0; e < UMMA_MERGE_COLS; ++e) acc[e] += i0 + i < parts ? f * o[i][e] : 0.f;
-    }
-    m_all = m_new;
+    for (int c = 0; c < COLS; ++c) acc[c][r] = 0.f;
   }
-  if (row >= t.n * rep) return;
-  const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
-  const int token = fdiv(row, p.by_rep), head = hk * rep + row - token * rep;
-  *reinterpret_cast<uint2*>(t.o + ((int64_t(b) * t.n + token) * t.H + head) * HEAD_DIM + col) =
-      make_uint2(ptx::pack_bf16(acc[0] * inv, acc[1] * inv), ptx::pack_bf16(acc[2] * inv, acc[3] * inv));
+  for (int i0 = warp % SPLIT; i0 < parts; i0 += AT_ONCE * SPLIT) {         // running maximum over batches of parts
+    float4 x[AT_ONCE][2], o[AT_ONCE][COLS];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int c = min(i0 + i * SPLIT, parts - 1);
+      const float* const slot = first + (c == 0 ? 0 : (int64_t(c) * 2 - 1) * UMMA_PARTIAL<PAIR>);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) x[i][h] = reinterpret_cast<const float4*>(slot + ROWS * HEAD_DIM + 2 * at)[h];
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) o[i][e] = *reinterpret_cast<const float4*>(slot + (col + e) * ROWS + at);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      auto max_of = [&](int i) { return r == 0 ? x[i][0].x : r == 1 ? x[i][0].z : r == 2 ? x[i][1].x : x[i][1].z; };
+      auto sum_of = [&](int i) { return r == 0 ? x[i][0].y : r == 1 ? x[i][0].w : r == 2 ? x[i][1].y : x[i][1].w; };
+      float m_new = m_all[r];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) m_new = fmaxf(m_new, max_of(i));
+      const float alpha = merge_weight(m_all[r], m_new);
+      l_all[r] *= alpha;
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) acc[e][r] *= alpha;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const bool there = i0 + i * SPLIT < parts;
+        const float f = there ? merge_weight(max_of(i), m_new) : 0.f;
+        l_all[r] += there ? f * sum_of(i) : 0.f;
+#pragma unroll
+        for (int e = 0; e < COLS; ++e) {
+          const float4& y = o[i][e];
+          acc[e][r] += there ? f * (r == 0 ? y.x : r == 1 ? y.y : r == 2 ? y.z : y.w) : 0.f;
+        }
+      }
+      m_all[r] = m_new;
+    }
+  }
+  if (SPLIT > 1) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      joined[warp][r][lane] = m_all[r];
+      joined[warp][4 + r][lane] = l_all[r];
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) joined[warp][8 + 4 * e + r][lane] = acc[e][r];
+    }
+    __syncthreads();
+    if (warp % SPLIT != 0) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int w = 1; w < SPLIT; ++w) m_all[r] = fmaxf(m_all[r], joined[warp + w][r][lane]);
+      l_all[r] = 0.f;
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) acc[e][r] = 0.f;
+#pragma unroll
+      for (int w = 0; w < SPLIT; ++w) {
+        const float f = merge_weight(joined[warp + w][r][lane], m_all[r]);
+        l_all[r] += f * joined[warp + w][4 + r][lane];
+#pragma unroll
+        for (int e = 0; e < COLS; ++e) acc[e][r] += f * joined[warp + w][8 + 4 * e + r][lane];
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int row = rg * ROWS + at + r;
+    if (row >= t.n * rep) break;
+    const float inv = l_all[r] == 0.f ? 0.f : 1.f / l_all[r];
+    const int token = fdiv(row, p.by_rep), head = hk * rep + row - token * rep;
+    __nv_bfloat16* const out = t.o + ((int64_t(b) * t.n + token) * t.H + head) * HEAD_DIM + col;
+    uint32_t w[COLS / 2];
+#pragma unroll
+    for (int e = 0; e < COLS / 2; ++e) w[e] = ptx::pack_bf16(acc[2 * e][r] * inv, acc[2 * e + 1][r] * inv);
+    if constexpr (COLS == 8) *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+  }
 }
 
 }  // namespace intra
