@@ -112,8 +112,9 @@ int launch_tree_mma(TreeParams p, const ServingState& st, int64_t scratch_bytes,
   const int64_t blocks = units * ceil_div(p.S, TREE_BLOCK), places = blocks + units * TREE_UNIT_COST;      // at most
   const int slots = st.sm_count * TREE_CTAS_PER_SM;
   if (places + slots * int64_t(TREE_MIN_BLOCKS) > 0x7fffffffLL || rows > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
-  const int64_t parts = (blocks + TREE_MIN_BLOCKS - 1) / TREE_MIN_BLOCKS;
-  const int grid = parts < slots ? int(parts) : slots;
+  const int64_t parts = (blocks + TREE_MIN_BLOCKS - 1) / TREE_MIN_BLOCKS, ctas = parts > units ? parts : units;
+  const int grid = ctas < slots ? int(ctas) : slots;
+  p.split_cost = TREE_SPLIT_COST;
   int64_t floats = (grid + units) * int64_t(TREE_PARTIAL);
   if (ACCUMULATE) {
     if (int64_t(p.B) * p.Hkv > 65535) return INTRA_ERR_UNSUPPORTED;      // grid.y of the accumulation
@@ -126,6 +127,8 @@ int launch_tree_mma(TreeParams p, const ServingState& st, int64_t scratch_bytes,
   const int smem = tree_smem_bytes(p.mask ? (p.mask_sn ? p.n : 1) : 0);
   cudaError_t e = all_rows <= TREE_ROWS / 2 ? launch_early(tree_mma_kernel<ACCUMULATE, true>, dim3(unsigned(grid)), TREE_THREADS, smem, stream, p)
                                             : launch_early(tree_mma_kernel<ACCUMULATE, false>, dim3(unsigned(grid)), TREE_THREADS, smem, stream, p);
+  if (!ACCUMULATE && !p.lengths && tree_whole(uint32_t(units), uint32_t(blocks), ceil_div(p.S, TREE_BLOCK), grid, p.split_cost))
+    return e == cudaSuccess ? INTRA_OK : cuda_fail(e);             // nothing to join
   if (e == cudaSuccess)
     e = ACCUMULATE ? launch_early(tree_weights_kernel, dim3(unsigned(ceil_div(p.S, TREE_WEIGHT_KEYS)) + 1, unsigned(p.B * p.Hkv)), TREE_WEIGHT_THREADS, 0, stream, p, uint32_t(grid))
                    : launch_early(tree_merge_kernel, dim3(unsigned((rows + TREE_MERGE_WARPS - 1) / TREE_MERGE_WARPS)), 32 * TREE_MERGE_WARPS, 0, stream, p, uint32_t(grid));
