@@ -130,7 +130,8 @@ int launch_tree_mma(TreeParams p, const ServingState& st, int64_t scratch_bytes,
   if (!ACCUMULATE && !p.lengths && tree_whole(uint32_t(units), uint32_t(blocks), ceil_div(p.S, TREE_BLOCK), grid, p.split_cost))
     return e == cudaSuccess ? INTRA_OK : cuda_fail(e);             // nothing to join
   if (e == cudaSuccess)
-    e = ACCUMULATE ? launch_early(tree_weights_kernel, dim3(unsigned(ceil_div(p.S, TREE_WEIGHT_KEYS)) + 1, unsigned(p.B * p.Hkv)), TREE_WEIGHT_THREADS, 0, stream, p, uint32_t(grid))
+    e = ACCUMULATE ? launch_early(tree_weights_kernel, dim3(unsigned(imin(ceil_div(p.S, TREE_WEIGHT_KEYS), ceil_div(st.sm_count * TREE_WEIGHT_CTAS_PER_SM, p.B * p.Hkv))) + 1, unsigned(p.B * p.Hkv)),
+                                  TREE_WEIGHT_THREADS, 0, stream, p, uint32_t(grid))
                    : launch_early(tree_merge_kernel, dim3(unsigned((rows + TREE_MERGE_WARPS - 1) / TREE_MERGE_WARPS)), 32 * TREE_MERGE_WARPS, 0, stream, p, uint32_t(grid));
   return e == cudaSuccess ? INTRA_OK : cuda_fail(e);
 }
@@ -274,6 +275,7 @@ int intra_b200_decode_accumulate(const void* q, const void* k, const void* v, co
   p.o = static_cast<__nv_bfloat16*>(out);
   p.weights = weights;
   p.weights_sb = weights_batch_stride; p.weights_sh = weights_head_stride;
+  p.weights_vec = aligned16(weights) && ((p.weights_sb | p.weights_sh) & 3) == 0;
   p.scratch = static_cast<float*>(scratch);
   p.q_sb = q_strides[0]; p.q_sn = q_strides[1]; p.q_sh = q_strides[2];
   p.ks = view_of(k_strides);

@@ -38,6 +38,7 @@ struct TreeParams {
   // every visible key, [unit][row][score_keys], times scale_log2
   float* weights;
   int64_t weights_sb, weights_sh;
+  int weights_vec;             // four weights can be loaded at once
   float* scores;
   int score_keys;
   int S, H, Hkv, n, B;

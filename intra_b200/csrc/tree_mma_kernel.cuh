@@ -397,12 +397,12 @@ struct TreeParts {
 
 // Joins the parts of units that several CTAs had a part of. A warp per row, a lane for four dims.
 constexpr int TREE_MERGE_WARPS = 4;
+template <int AT_ONCE>                                             // parts whose loads are under way together
 __device__ __forceinline__ void tree_merge_row(const TreeParams& p, const TreeParts& parts, int unit, int b, int hk, int row, int at) {
   const int lane = threadIdx.x & 31, rep = p.H / p.Hkv;
   const float* const first = p.scratch + (int64_t(parts.first) + unit) * TREE_PARTIAL;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float m_all = -CUDART_INF_F, l_all = 0.f;
-  constexpr int AT_ONCE = 8;                                       // parts whose loads are under way together
   for (int i0 = 0; i0 < parts.count; i0 += AT_ONCE) {
     float2 x[AT_ONCE];
     float4 o[AT_ONCE];
@@ -441,81 +441,107 @@ __global__ void __launch_bounds__(32 * TREE_MERGE_WARPS) tree_merge_kernel(const
   const TreeParts parts(p, b, hk * p.row_groups + rg, grid);
   cudaGridDependencySynchronize();
   if (parts.count == 1) return;                                    // one CTA held the unit and wrote its rows
-  tree_merge_row(p, parts, kv * p.row_groups + rg, b, hk, row, row - rg * TREE_ROWS);
+  tree_merge_row<8>(p, parts, kv * p.row_groups + rg, b, hk, row, row - rg * TREE_ROWS);
 }
 
 // weights += each visible key's probabilities summed over its KV head's query heads, from the scores and every row's
-// maximum and weight; a thread per key, so the order of the sum is fixed. The last CTA of a KV head joins its output rows
-// instead.
-constexpr int TREE_WEIGHT_THREADS = 256, TREE_WEIGHT_KEYS = 4 * TREE_WEIGHT_THREADS;
-__global__ void __launch_bounds__(TREE_WEIGHT_THREADS) tree_weights_kernel(const __grid_constant__ TreeParams p, uint32_t grid) {
+// maximum and weight; a thread per four keys, so the order of the sum is fixed. The last CTA of a KV head joins its output rows
+// instead. What takes time is the chain of loads - the list, the scores, the rows' statistics - so there are as many CTAs as run
+// together, each with several blocks of keys. The whole call, 288 heads of 4,000 keys 111.0 us, 128 heads of 2,048 to 8,192 75.7; with
+// a CTA per 1,024 keys and 20 scalar loads a thread 114.7 and 79.2. 92 without the weights.
+constexpr int TREE_WEIGHT_THREADS = 256, TREE_WEIGHT_KEYS = 4 * TREE_WEIGHT_THREADS, TREE_WEIGHT_CTAS_PER_SM = 4;
+__global__ void __launch_bounds__(TREE_WEIGHT_THREADS, TREE_WEIGHT_CTAS_PER_SM) tree_weights_kernel(const __grid_constant__ TreeParams p, uint32_t grid) {
   __shared__ float2 stats[TREE_ROWS];                              // maximum, inverse sum
   const int hk = blockIdx.y % p.Hkv, b = blockIdx.y / p.Hkv, rows = p.H / p.Hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool joins = blockIdx.x == gridDim.x - 1;
-  const int keys = tree_context(p, b) + 1, key0 = blockIdx.x * TREE_WEIGHT_KEYS + threadIdx.x;
+  const int keys = tree_context(p, b) + 1;
   if (!joins && int(blockIdx.x) * TREE_WEIGHT_KEYS >= keys) return;
   float* const weights = p.weights + b * p.weights_sb + hk * p.weights_sh;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f}, before[4] = {0.f, 0.f, 0.f, 0.f};
-  bool seen[4] = {false, false, false, false};
+  const uint8_t* const mask = p.mask + b * p.mask_sb;
   for (int rg = 0; rg < p.row_groups; ++rg) {
     const int unit = (b * p.Hkv + hk) * p.row_groups + rg, n_rows = min(rows - rg * TREE_ROWS, TREE_ROWS);
     const TreeParts parts(p, b, hk * p.row_groups + rg, grid);
     if (rg == 0) cudaGridDependencySynchronize();
     if (joins) {
       if (parts.count > 1)
-        for (int r = warp; r < n_rows; r += TREE_WEIGHT_THREADS / 32) tree_merge_row(p, parts, unit, b, hk, rg * TREE_ROWS + r, r);
+        for (int r = warp; r < n_rows; r += TREE_WEIGHT_THREADS / 32) tree_merge_row<4>(p, parts, unit, b, hk, rg * TREE_ROWS + r, r);
       continue;
     }
     const float* const x = p.scores + int64_t(unit) * TREE_ROWS * p.score_keys;
-    constexpr int AT_ONCE = 4;                                     // rows whose scores are under way together, before the statistics are there
-    float y[AT_ONCE][4];
+    constexpr int AT_ONCE = 4;                                     // rows whose scores are under way together
+    bool first_block = true;
+    for (int key0 = blockIdx.x * TREE_WEIGHT_KEYS + 4 * threadIdx.x; key0 - 4 * int(threadIdx.x) < keys; key0 += (gridDim.x - 1) * TREE_WEIGHT_KEYS) {
+      const bool whole = key0 + 4 <= keys;                         // four keys of the sequence
+      float4 y[AT_ONCE];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int key = key0 + c * TREE_WEIGHT_THREADS;
-      if (rg == 0) {
-        seen[c] = key < keys && (p.mask == nullptr || p.mask[b * p.mask_sb + key * p.mask_ss] != 0);
-        before[c] = seen[c] ? weights[key] : 0.f;
+      for (int r = 0; r < AT_ONCE; ++r)
+        y[r] = key0 < keys ? *reinterpret_cast<const float4*>(x + int64_t(min(r, n_rows - 1)) * p.score_keys + key0) : make_float4(0.f, 0.f, 0.f, 0.f);
+      uint32_t seen = 0;                                           // a bit for each key
+      if (whole && (p.mask == nullptr || p.mask_vec)) {
+        const uint32_t m = p.mask ? *reinterpret_cast<const uint32_t*>(mask + key0) : 0x01010101u;
+        seen = (__vminu4(m, 0x01010101u) * 0x10204080u) >> 28;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) seen |= key0 + c < keys && (p.mask == nullptr || mask[(key0 + c) * p.mask_ss] != 0) ? 1u << c : 0u;
       }
+      float before[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+      if (whole && p.weights_vec) {
+        const float4 w = *reinterpret_cast<const float4*>(weights + key0);
+        before[0] = w.x; before[1] = w.y; before[2] = w.z; before[3] = w.w;
+      } else {
 #pragma unroll
-      for (int r = 0; r < AT_ONCE; ++r) y[r][c] = seen[c] && r < n_rows ? x[int64_t(r) * p.score_keys + key] : 0.f;
-    }
-    const float2* const first = reinterpret_cast<const float2*>(p.scratch + (int64_t(parts.first) + unit) * TREE_PARTIAL + TREE_ROWS * HEAD_DIM);
-    __syncthreads();
-    for (int r = warp; r < n_rows; r += TREE_WEIGHT_THREADS / 32) {
-      float m = -CUDART_INF_F, l = 0.f;
-      for (int i = lane; i < parts.count; i += 32) {
-        const float2 z = first[int64_t(i) * (TREE_PARTIAL / 2) + r];
-        const float m_new = fmaxf(m, z.x);
-        l = l * merge_weight(m, m_new) + z.y * merge_weight(z.x, m_new);
-        m = m_new;
+        for (int c = 0; c < 4; ++c) before[c] = (seen >> c) & 1u ? weights[key0 + c] : 0.f;
       }
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d), m_new = fmaxf(m, m2);
-        l = l * merge_weight(m, m_new) + l2 * merge_weight(m2, m_new);
-        m = m_new;
-      }
-      if (lane == 0) stats[r] = make_float2(m, 1.f / l);
-    }
-    __syncthreads();
-    for (int r0 = 0; r0 < n_rows; r0 += AT_ONCE) {
-#pragma unroll
-      for (int r = 0; r < AT_ONCE; ++r) {
-        if (r0 + r >= n_rows) break;
-        const float2 st = stats[r0 + r];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float s = r0 == 0 ? y[r][c] : seen[c] ? x[int64_t(r0 + r) * p.score_keys + key0 + c * TREE_WEIGHT_THREADS] : 0.f;
-          sum[c] += ptx::ex2(s - st.x) * st.y;
+      if (first_block) {                                           // the rows' statistics, while the first loads are under way
+        first_block = false;
+        const float2* const first = reinterpret_cast<const float2*>(p.scratch + (int64_t(parts.first) + unit) * TREE_PARTIAL + TREE_ROWS * HEAD_DIM);
+        __syncthreads();                                           // those of the rows before have been read
+        for (int r = warp; r < n_rows; r += TREE_WEIGHT_THREADS / 32) {
+          float m = -CUDART_INF_F, l = 0.f;
+          for (int i = lane; i < parts.count; i += 32) {
+            const float2 z = first[int64_t(i) * (TREE_PARTIAL / 2) + r];
+            const float m_new = fmaxf(m, z.x);
+            l = l * merge_weight(m, m_new) + z.y * merge_weight(z.x, m_new);
+            m = m_new;
+          }
+          for (int d = 1; d < 32 && d < parts.count; d *= 2) {     // lanes from parts.count on have none
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d), m_new = fmaxf(m, m2);
+            l = l * merge_weight(m, m_new) + l2 * merge_weight(m2, m_new);
+            m = m_new;
+          }
+          if (lane == 0) stats[r] = make_float2(m, 1.f / l);
         }
+        __syncthreads();
+      }
+      for (int r0 = 0; r0 < n_rows; r0 += AT_ONCE) {
+        if (r0 > 0) {
+#pragma unroll
+          for (int r = 0; r < AT_ONCE; ++r)
+            y[r] = key0 < keys ? *reinterpret_cast<const float4*>(x + int64_t(min(r0 + r, n_rows - 1)) * p.score_keys + key0) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; ++r) {
+          if (r0 + r >= n_rows) break;
+          const float2 st = stats[r0 + r];
+          sum[0] += ptx::ex2(y[r].x - st.x) * st.y;                // of keys that are not seen anything, and not used
+          sum[1] += ptx::ex2(y[r].y - st.x) * st.y;
+          sum[2] += ptx::ex2(y[r].z - st.x) * st.y;
+          sum[3] += ptx::ex2(y[r].w - st.x) * st.y;
+        }
+      }
+      if (seen == 0u) continue;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) before[c] = (seen >> c) & 1u ? before[c] + sum[c] : before[c];
+      if (whole && p.weights_vec) {
+        *reinterpret_cast<float4*>(weights + key0) = make_float4(before[0], before[1], before[2], before[3]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if ((seen >> c) & 1u) weights[key0 + c] = before[c];
       }
     }
   }
-  if (joins) return;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (seen[c]) weights[key0 + c * TREE_WEIGHT_THREADS] = before[c] + sum[c];
 }
 
 }  // namespace intra
