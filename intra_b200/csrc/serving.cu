@@ -163,7 +163,7 @@ int launch_tree_umma(const TreeParams& t, const ServingState& st, int64_t scratc
   const int64_t units = int64_t(B) * t.Hkv * p.t.row_groups, ctas = parts > units ? parts : units;
   const int grid = ctas < st.sm_count ? int(ctas) : st.sm_count;
   p.t.unit_cost = UMMA_UNIT_COST<PAIR>;
-  p.t.split_cost = umma_split_cost(imin(t.n * (t.H / t.Hkv), UMMA_ROWS<PAIR>));
+  p.t.split_cost = umma_split_cost(imin(t.n * (t.H / t.Hkv), UMMA_ROWS<PAIR>), !t.lengths && !t.mask);
   p.t.min_tiles = UMMA_MIN_TILES;
   *scratch_needed = grid * 2 * UMMA_PARTIAL<PAIR> * int64_t(sizeof(float));
   if (t.mask) {                   // behind the partial results: the mask's bits, those of any token, the tiles
@@ -244,6 +244,10 @@ int intra_b200_tree_attn(const void* q, const void* k, const void* v, const int*
   p.S = S; p.H = H; p.Hkv = Hkv; p.n = n; p.B = B;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  // By rows of a KV head. 12 and 16 rows on the kernel for few / for more, us: 16 sequences of 4,096 keys 52.8 / 60.5, of 1,000 23.1 / 20.2,
+  // one of 30,000 40.7 / 39.6, of 3,001 16.0 / 15.0; with a mask or lengths the first has no kernel before it. 96 and 128 rows as two streams of key tiles /
+  // in the form for two tiles of rows: 56.6 and 58.9 / 58.4 and 59.9, one of 30,000 40.9 and 42.3 / 41.2 and 41.0, and more
+  // of the probabilities' bits.
   if (n * (H / Hkv) > 128) return launch_tree_umma<true>(p, *st, scratch_bytes, scratch_needed, stream);
   if (n * (H / Hkv) > TREE_ROWS) return launch_tree_umma<false>(p, *st, scratch_bytes, scratch_needed, stream);
   return launch_tree_mma<false>(p, *st, scratch_bytes, scratch_needed, stream);
@@ -315,8 +319,11 @@ int intra_b200_verify_drafts(const void* tokens, int tokens_int64, const void* t
   if (draft) { p.draft_sb = draft_strides[0]; p.draft_sn = draft_strides[1]; }
   p.tokens_sb = tokens_batch_stride; p.uniform_sb = uniform_batch_stride; p.parents_sb = parents_batch_stride;
   p.n = n; p.V = V;
+  // CTAs of a sequence's cluster: as many as fit the GPU at once (two CTAs an SM) and have a few thousand tokens each. Measured with
+  // 1 / 2 / 4 / 8, us: 1 x 50257 tokens 15.9 / 11.8 / 9.5 / 8.6, 32 x 128257 37.7 / 23.2 / 16.5 / 17.3, 64 x 50257 19.8 / 15.0 / 14.9 /
+  // 22.8, 150 x 30000 17.4 / 19.1 / 23.9 / 39.4; 1 x 4000 6.7 / 6.2 / 6.0 / 6.1.
   int c = 1;
-  while (c < VERIFY_MAX_CLUSTER && int64_t(B) * 2 * c <= 4 * st->sm_count && V >= 2048 * c) c *= 2;
+  while (c < VERIFY_MAX_CLUSTER && int64_t(B) * 2 * c <= 2 * st->sm_count && V >= 2048 * c) c *= 2;
   p.cluster = c;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   cudaError_t e;
@@ -395,6 +402,9 @@ int intra_b200_evict(const void* k, const void* v, const float* weights, const i
   p.weights_sb = weights_strides[0]; p.weights_sh = weights_strides[1];
   p.weights2_sb = weights_out_strides[0]; p.weights2_sh = weights_out_strides[1];
   p.S = S; p.Hkv = Hkv; p.keep = keep; p.recent = recent;
+  // CTAs of a head's cluster: as many as fit the GPU at once (two an SM) and have a few thousand weights each; more where a part
+  // would not fit shared memory. Measured with 1 / 2 / 4 / 8, us: 8 heads of 4,096 rows 10.0 / 10.8 / 12.5 / 15.5, of 65,536 - / 28.0 /
+  // 21.3 / 20.3, 32 heads of 16,384 - / 20.7 / 20.6 / 34.5, 128 heads of 16,384 - / 59.3 / 73.1 / 139.5.
   int c = 1;
   while (c < EVICT_MAX_CLUSTER && units * 2 * c <= 2 * st->sm_count && S > 6144 * c) c *= 2;
   while (c < EVICT_MAX_CLUSTER && ceil_div(S, c) > EVICT_SMEM_KEYS) c *= 2;

@@ -53,13 +53,14 @@ constexpr int UMMA_MIN_TILES = 2;
 // tokens over 8 sequences of 4096 to 8192 keys 59.8 / 59.2 / 67.8.
 template <bool PAIR> constexpr int UMMA_UNIT_COST = PAIR ? 3 : 1;
 
-// Tiles that partial results and their merge are worth. Measured, us, dealt in equal parts / in whole units:
+// Tiles that partial results and their merge are worth; more where the host can tell that the merge need not be launched
+// (`no_merge`). Measured, us, divided / whole:
 //   rows of a unit                               32          96         256
-//   128 units of 32 tiles (27.7 a CTA)    63.3 / 61.8 72.4 / 64.8 96.7 / 78.1
-//   128 units of 8 tiles (6.9)            33.3 / 26.7 40.4 / 29.9 59.7 / 37.6
-//   96 units of 32 tiles (20.8)           51.9 / 58.9 59.4 / 62.1 76.4 / 72.5
+//   128 units of 32 tiles (27.7 a CTA)    63.3 / 53.8 72.4 / 57.3 96.7 / 70.2    no lengths; with lengths 49.2 / 46.6 (20 a CTA)
+//   128 units of 8 tiles (6.9)            33.3 / 20.2 40.4 / 21.6 59.7 / 26.4
+//   96 units of 32 tiles (20.8)           50.8 / 58.9 55.3 / 62.1 75.8 / 62.7    the merge launched in all but the last
 //   72 units of 64 tiles (31.1)          66.2 / 100.5 73.6 / 103.2 91.6 / 116.2
-constexpr int umma_split_cost(int rows) { return 4 + rows / 24; }
+__host__ __device__ constexpr int umma_split_cost(int rows, bool no_merge) { return 5 + rows / 40 + (no_merge ? 3 : 0); }
 
 struct TreeUmmaParams {
   TreeParams t;                // row_groups: units per KV head
