@@ -155,14 +155,14 @@ int launch_tree_umma(const TreeParams& t, const ServingState& st, int64_t scratc
   const int64_t tiles = int64_t(B) * t.Hkv * p.t.row_groups * ceil_div(t.S, TILE_N);       // at most
   const int64_t parts = (tiles + UMMA_MIN_TILES - 1) / UMMA_MIN_TILES;
   const int64_t rows = int64_t(B) * t.n * t.H;
-  const int64_t places = tiles + int64_t(B) * t.Hkv * p.t.row_groups * UMMA_UNIT_COST<PAIR>;
+  const int64_t places = tiles + int64_t(B) * t.Hkv * p.t.row_groups * UMMA_UNIT_COST;
   const int row_blocks = ceil_div(imin(t.n * (t.H / t.Hkv), UMMA_ROWS<PAIR>), 32);
   const bool split = int64_t(B) * t.Hkv * p.t.row_groups * UMMA_MERGE_FEW < st.sm_count;      // many parts a unit
   const int64_t merge_ctas = int64_t(B) * t.Hkv * p.t.row_groups * row_blocks * (split ? UMMA_MERGE_CTAS<4, 2> : UMMA_MERGE_CTAS<8, 1>);
   if (places + st.sm_count > 0x7fffffffLL || rows > 0x7fffffffLL || merge_ctas > 0x7fffffffLL) return INTRA_ERR_UNSUPPORTED;
   const int64_t units = int64_t(B) * t.Hkv * p.t.row_groups, ctas = parts > units ? parts : units;
   const int grid = ctas < st.sm_count ? int(ctas) : st.sm_count;
-  p.t.unit_cost = UMMA_UNIT_COST<PAIR>;
+  p.t.unit_cost = UMMA_UNIT_COST;
   p.t.split_cost = umma_split_cost(imin(t.n * (t.H / t.Hkv), UMMA_ROWS<PAIR>), !t.lengths && !t.mask);
   p.t.min_tiles = UMMA_MIN_TILES;
   *scratch_needed = grid * 2 * UMMA_PARTIAL<PAIR> * int64_t(sizeof(float));

@@ -91,9 +91,11 @@ __host__ __device__ __forceinline__ bool tree_whole(uint32_t units, uint32_t til
   return split_cost > 0 && uint64_t((units + grid - 1) / grid) * longest <= uint64_t(tiles / grid) + split_cost;
 }
 
-// The list of all units' key tiles. A unit counts for `cost` places more than it has tiles, in front of them: what the end
-// of one unit and the start of the next cost the CTA that has both (parts of a few tiles would only be spread unevenly by
-// it). Where CTAs that each take the same number of whole units are done about as early as with parts of equal size - by
+// The list of all units' key tiles. A unit counts for `cost` places more than it has tiles, in front of them: what the end of one
+// unit and the start of the next cost the CTA that has both; at most a quarter of a CTA's share of tiles, since parts of a few
+// tiles would only be spread unevenly by it. 26 tokens over 8 caches of 4,096 to 8,192 keys 59.9 -> 56.5 us, 32 rows over 65,536
+// keys 62 -> 58.8, against 1 place (3 above 128 rows; 4 of 16 keys in the kernel for few rows, now 20) from 16 tiles on; with an
+// eighth 58.5 and 60.3, with a third the same, but 32 caches of 300 to 3,000 5 % more. Where CTAs that each take the same number of whole units are done about as early as with parts of equal size - by
 // p.split_cost tiles, what partial results and their merge take - the list is dealt so: every unit then has as many places as the
 // longest. At most 2^31 - 1 places.
 template <int KEYS>
@@ -122,7 +124,7 @@ struct TreeList {
     }
     const uint32_t share = tiles * units / grid;
     even = tree_whole(units * B, tiles * units, longest, grid, p.split_cost) ? longest : 0;
-    cost = share < 8 ? 0 : share < 16 ? min(p.unit_cost, 1) : p.unit_cost;
+    cost = min(share / 4, uint32_t(p.unit_cost));
     total = (even ? even * B : tiles + cost * B) * units;
     per = even ? (units * B + grid - 1) / grid * even : max((total + grid - 1) / grid, uint32_t(p.min_tiles));
     if (before) *before = (even ? even * b : front + cost * b) * units;

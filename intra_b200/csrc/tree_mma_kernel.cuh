@@ -36,7 +36,7 @@ constexpr int TREE_MIN_BLOCKS = 4 * TREE_WARPS;  // of a CTA's part: more parts 
 // Blocks that partial results and their merge are worth. Equal parts / 8 / 16, us for 16 rows: 8 units of 7 blocks 13.1 / 7.1 / 7.1,
 // of 32 blocks 11.7 / 11.7 / 13.6, 240 units of 32 blocks 23.2 / 18.6 / 18.6, 288 of 63 36.9 / 29.8 / 29.9.
 constexpr int TREE_SPLIT_COST = 8;
-constexpr int TREE_UNIT_COST = 4;                // places a unit has in front of its blocks: the merge of a piece's warps
+constexpr int TREE_UNIT_COST = 20;               // places a unit has in front of its blocks, at most: the merge of a piece's warps, the rings' start
 // Dynamic shared memory: rings (the merge's rows at the end of a piece), query tile, with a mask its bits per block and token.
 constexpr int tree_smem_bytes(int mask_tokens) { return TREE_RING_BYTES + TREE_Q_BYTES + mask_tokens * TREE_CHUNK * 2; }
 // A partial result: rows of sums, then (maximum in log2 units, weight) per row. CTA c's result of unit u is number c + u: of

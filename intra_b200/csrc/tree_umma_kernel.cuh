@@ -49,10 +49,7 @@ template <bool PAIR> constexpr int UMMA_SMEM_BYTES = (UMMA_RING + (PAIR ? 2 : 1)
 template <bool PAIR> constexpr int64_t UMMA_PARTIAL = int64_t(UMMA_ROWS<PAIR>) * (HEAD_DIM + 2);
 // A CTA's part is at least this many key tiles: a shorter one costs more in its ends and its merge than it spreads.
 constexpr int UMMA_MIN_TILES = 2;
-// Places a unit has in front of its tiles. Measured with 0 / 1 / 3: 64 tokens over 65536 keys (PAIR) 73.1 / 71.9 / 70.6 us, 26
-// tokens over 8 sequences of 4096 to 8192 keys 59.8 / 59.2 / 67.8.
-template <bool PAIR> constexpr int UMMA_UNIT_COST = PAIR ? 3 : 1;
-
+constexpr int UMMA_UNIT_COST = 5;                // places a unit has in front of its tiles, at most (TreeList)
 // Tiles that partial results and their merge are worth; more where the host can tell that the merge need not be launched
 // (`no_merge`). Measured, us, divided / whole:
 //   rows of a unit                               32          96         256
