@@ -180,6 +180,7 @@ int launch_tree_umma(const TreeParams& t, const ServingState& st, int64_t scratc
   }
   if (!t.scratch || scratch_bytes < *scratch_needed) return INTRA_NEED_SCRATCH;
   p.use_tma = cache_map(t.k, t.ks, t.S, t.Hkv, B, &p.maps[0]) && cache_map(t.v, t.vs, t.S, t.Hkv, B, &p.maps[1]);
+  p.early = grid < st.sm_count;
   p.status = st.status_word;
   cudaError_t e = cudaSuccess;
   if (t.mask) e = launch_early(tree_mask_kernel, dim3(unsigned(ceil_div(p.t.bits_words, 32)), unsigned(B)), 32 * TREE_MASK_ROWS, 0, stream, p.t);

@@ -86,9 +86,10 @@ __device__ __forceinline__ int tree_tiles(const TreeParams& p, int b, int* first
   return hi - lo;
 }
 
-// Are `units` units of at most `longest` tiles, `tiles` in all, dealt whole? See TreeList.
+// Are `units` units of at most `longest` tiles, `tiles` in all, dealt whole? See TreeList. Not where most CTAs would have none: 8 units
+// of 8 tiles on 32 CTAs take 13.4 us divided, 18 whole.
 __host__ __device__ __forceinline__ bool tree_whole(uint32_t units, uint32_t tiles, uint32_t longest, uint32_t grid, int split_cost) {
-  return split_cost > 0 && uint64_t((units + grid - 1) / grid) * longest <= uint64_t(tiles / grid) + split_cost;
+  return split_cost > 0 && units * 2 >= grid && uint64_t((units + grid - 1) / grid) * longest <= uint64_t(tiles / grid) + split_cost;
 }
 
 // The list of all units' key tiles. A unit counts for `cost` places more than it has tiles, in front of them: what the end of one
@@ -124,7 +125,7 @@ struct TreeList {
     }
     const uint32_t share = tiles * units / grid;
     even = tree_whole(units * B, tiles * units, longest, grid, p.split_cost) ? longest : 0;
-    cost = min(share / 4, uint32_t(p.unit_cost));
+    cost = share < uint32_t(p.min_tiles) ? 0 : min(share / 4, uint32_t(p.unit_cost));
     total = (even ? even * B : tiles + cost * B) * units;
     per = even ? (units * B + grid - 1) / grid * even : max((total + grid - 1) / grid, uint32_t(p.min_tiles));
     if (before) *before = (even ? even * b : front + cost * b) * units;

@@ -64,6 +64,7 @@ struct TreeUmmaParams {
   FastDiv by_rep;              // query heads per KV head
   CUtensorMap maps[2];         // K, V: (128, S, 1, Hkv, B)
   int use_tma;
+  int early;                   // the merge may be set up beside this kernel: there are SMs without a CTA of it
   int* status;
 };
 
@@ -244,6 +245,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
   }
   if (warp == 8 && lane < 2) ptx::prefetch_tensormap(&p.maps[lane]);
   cudaGridDependencySynchronize();                       // what is above ran beside the end of the kernel before this one
+  if (p.early) cudaTriggerProgrammaticLaunchCompletion();
   TreeWalk<TILE_N>& walk = walks[warp];
   const TreePiece& pc = pieces[warp];
   {
