@@ -92,17 +92,20 @@ __host__ __device__ __forceinline__ bool tree_whole(uint32_t units, uint32_t til
   return split_cost > 0 && units * 2 >= grid && uint64_t((units + grid - 1) / grid) * longest <= uint64_t(tiles / grid) + split_cost;
 }
 
-// The list of all units' key tiles. A unit counts for `cost` places more than it has tiles, in front of them: what the end of one
-// unit and the start of the next cost the CTA that has both; at most a quarter of a CTA's share of tiles, since parts of a few
-// tiles would only be spread unevenly by it. 26 tokens over 8 caches of 4,096 to 8,192 keys 59.9 -> 56.5 us, 32 rows over 65,536
-// keys 62 -> 58.8, against 1 place (3 above 128 rows; 4 of 16 keys in the kernel for few rows, now 20) from 16 tiles on; with an
-// eighth 58.5 and 60.3, with a third the same, but 32 caches of 300 to 3,000 5 % more. Where CTAs that each take the same number of whole units are done about as early as with parts of equal size - by
-// p.split_cost tiles, what partial results and their merge take - the list is dealt so: every unit then has as many places as the
-// longest. At most 2^31 - 1 places.
+// The list of all units' key tiles. A unit counts for `cost` places more than it has tiles, in front of them: what the end of
+// one unit and the start of the next cost the CTA that has both; at most a quarter of a CTA's share of tiles, since parts of a
+// few tiles would only be spread unevenly by it. 26 tokens over 8 caches of 4,096 to 8,192 keys 59.9 -> 56.5 us, 32 rows over
+// 65,536 keys 62 -> 58.8, against 1 place (3 above 128 rows; 4 of 16 keys in the kernel for few rows, now 20) from 16 tiles on;
+// with an eighth 58.5 and 60.3, with a third the same, but 32 caches of 300 to 3,000 5 % more.
+// Where CTAs that each take the same number of whole units are done about as early as with parts of equal size - by
+// p.split_cost tiles, what partial results and their merge take - the list is dealt so: every unit then has as many places as
+// the longest. With two or more CTAs a unit, each unit is divided into the same number of parts if those are not longer than
+// equal ones by more than a tile, so that no CTA has two pieces: one sequence of 8,000 keys, 32 rows 23.7 -> 19.4 us, 16 rows
+// 23.1 -> 20.7, four of 3,000 keys 24.7 -> 22.4; calls of a few tiles lose up to 0.5. At most 2^31 - 1 places.
 template <int KEYS>
 struct TreeList {
   uint32_t units, cost, per, total;      // units per sequence; places of a CTA's part, of all
-  uint32_t even;                         // places of every unit, 0: units are divided
+  uint32_t even;                         // places of every unit, 0: as many as they have tiles, and `cost`
   __device__ __forceinline__ uint32_t places(uint32_t tiles) const { return even ? even : tiles + cost; }
   // Called by whole warps; all lanes get the same. `before`: places of sequences before `b`.
   __device__ __forceinline__ TreeList(const TreeParams& p, int B, uint32_t grid, int b = 0, uint32_t* before = nullptr) {
@@ -126,8 +129,14 @@ struct TreeList {
     const uint32_t share = tiles * units / grid;
     even = tree_whole(units * B, tiles * units, longest, grid, p.split_cost) ? longest : 0;
     cost = share < uint32_t(p.min_tiles) ? 0 : min(share / 4, uint32_t(p.unit_cost));
+    per = max(((tiles + cost * B) * units + grid - 1) / grid, uint32_t(p.min_tiles));
+    if (even) {
+      per = (units * B + grid - 1) / grid * even;
+    } else if (units * B * 2 <= grid) {                            // the same number of parts of every unit
+      const uint32_t k = grid / (units * B), part = (longest + k - 1) / k;
+      if (part <= per + 1) { per = part; even = k * part; }
+    }
     total = (even ? even * B : tiles + cost * B) * units;
-    per = even ? (units * B + grid - 1) / grid * even : max((total + grid - 1) / grid, uint32_t(p.min_tiles));
     if (before) *before = (even ? even * b : front + cost * b) * units;
   }
 };
