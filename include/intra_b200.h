@@ -96,7 +96,7 @@ int intra_b200_decode(const void* q, const void* k, const void* v, const void* m
  * weights[b][hk][j] += the sum of key j's probabilities over KV head hk's query heads, fp32 by strides (in elements; unit
  * stride over keys), keys the token does not see being left as they are. `lengths` is NULL or B ints: the keys before
  * the token's own, which sees keys 0 .. lengths[b] (brought into 0 .. S - 1). Strides {batch, token, head}; the mask's
- * {batch, token}. Always wants scratch (see above): the scores pass through it. */
+ * {batch, token}. Always wants scratch (see above): the scores pass through it. B * Hkv up to 65535. */
 int intra_b200_decode_accumulate(const void* q, const void* k, const void* v, const void* mask, const int* lengths, void* out,
                                  float* weights, void* scratch, int64_t scratch_bytes, int64_t* scratch_needed, int B, int S,
                                  int H, int Hkv, const int64_t q_strides[3], const int64_t k_strides[3],
@@ -110,7 +110,7 @@ int intra_b200_decode_accumulate(const void* q, const void* k, const void* v, co
  * comes before it, an earlier one, or negative; NULL: i - 1. With all_own != 0 it sees all n own keys instead (`mask` is to
  * decide alone). `mask` is NULL or B x n x S bytes by strides {batch, token, key}
  * (0 repeats), nonzero = visible. Keys that no token of the sequence sees are not read; a token that sees nothing gets
- * zeros. Scratch as for the decode step. */
+ * zeros. Scratch as for the decode step. With a mask and more than 16 rows (n * H / Hkv) B is up to 65535. */
 int intra_b200_tree_attn(const void* q, const void* k, const void* v, const int* parents, const int* lengths, const void* mask,
                          void* out, void* scratch, int64_t scratch_bytes, int64_t* scratch_needed, int B, int S, int H, int Hkv,
                          int n, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
@@ -124,7 +124,8 @@ int intra_b200_tree_attn(const void* q, const void* k, const void* v, const int*
  * R into max(R - Z q, 0) and Z into its sum, where that is not zero. At the end one token is drawn from R: the
  * smallest t with R(0) + .. + R(t) > uniform[b][0] * sum R. Sums in 64 bits. Outputs, contiguous: accepted[b], the number
  * of accepted drafts m; path[b] = 0 and the accepted nodes, then -1; out_tokens[b]: the accepted tokens, the drawn one
- * at place m, then -1. Drafts outside 0 .. V - 1 are rejected. Strides in elements {batch, node}; unit stride over V. */
+ * at place m, then -1. Drafts outside 0 .. V - 1 are rejected. Strides in elements {batch, node}; unit stride over V, which is
+ * at most 2^30. */
 #define INTRA_PROB_F32 0
 #define INTRA_PROB_BF16 1
 #define INTRA_PROB_F16 2

@@ -557,6 +557,21 @@ def test_refusals(device):
 
 
 @pytest.mark.gpu
+def test_batches_beyond_a_launch_are_refused():
+    """65,535 heads with weights, 65,535 sequences with a mask; one more is an error, and without a mask it runs."""
+    B = 65536
+    x = torch.randn(1, 1, 17, 128, generator=_gen(1)).to(torch.bfloat16).cuda()
+    q, k = x.expand(B, 1, 17, 128), x.expand(B, 1, 17, 128)
+    mask = torch.ones(1, 1, 1, 17, dtype=torch.bool, device="cuda").expand(B, 1, 1, 17)
+    with pytest.raises(ValueError):
+        tree_attn(q, k, k, mask=mask)
+    with pytest.raises(ValueError):
+        decode_attn_accumulate(q[:, :, :1], k, k, torch.zeros(B, 1, 17, device="cuda"))
+    out = tree_attn(q, k, k)
+    assert torch.equal(out, out[:1].expand_as(out)) and torch.equal(out[:1], tree_attn(x, x, x))
+
+
+@pytest.mark.gpu
 def test_empty_batches():
     k, w = torch.zeros(0, 2, 50, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(0, 2, 50, device="cuda")
     q = torch.zeros(0, 8, 4, 128, dtype=torch.bfloat16, device="cuda")
