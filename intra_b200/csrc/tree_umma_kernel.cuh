@@ -64,7 +64,9 @@ struct TreeUmmaParams {
   FastDiv by_rep;              // query heads per KV head
   CUtensorMap maps[2];         // K, V: (128, S, 1, Hkv, B)
   int use_tma;
-  int early;                   // the merge may be set up beside this kernel: there are SMs without a CTA of it
+  // The merge may be set up beside this kernel: there are SMs without a CTA of it. 5 tokens over 3,001 keys 15.9 -> 15.1 us; with
+  // a CTA on every SM, 32 rows over 65,536 keys, 65 us for 61.
+  int early;
   int* status;
 };
 
