@@ -147,7 +147,7 @@ bool cache_map(const __nv_bfloat16* ptr, const TensorView& v, int S, int Hkv, in
 
 template <bool PAIR>
 int launch_tree_umma(const TreeParams& t, const ServingState& st, int64_t scratch_bytes, int64_t* scratch_needed, cudaStream_t stream) {
-  TreeUmmaParams p;
+  TreeUmmaParams p = {};
   p.t = t;
   const int B = t.B;
   p.t.row_groups = ceil_div(t.n * (t.H / t.Hkv), UMMA_ROWS<PAIR>);

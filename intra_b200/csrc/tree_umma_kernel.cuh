@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
     ptx::tmem_alloc(&tmem_base_smem, 512);
     ptx::tmem_relinquish();
   }
-  if (warp == 8 && lane < 2) ptx::prefetch_tensormap(&p.maps[lane]);
+  if (warp == 8 && lane < 2 && p.use_tma) ptx::prefetch_tensormap(&p.maps[lane]);      // else they describe nothing
   cudaGridDependencySynchronize();                       // what is above ran beside the end of the kernel before this one
   if (p.early) cudaTriggerProgrammaticLaunchCompletion();
   TreeWalk<TILE_N>& walk = walks[warp];
