@@ -59,19 +59,15 @@ template <> __device__ __forceinline__ double as_double(float x) { return x; }
 template <> __device__ __forceinline__ double as_double(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <> __device__ __forceinline__ double as_double(__half x) { return __half2float(x); }
 
-// A probability as a double by its bits, in one integer multiply-add: the conversion instruction runs at an eighth of the
-// rate. Zero and the denormals of fp32 come out near 2^-127; terms that decide something by themselves are converted properly.
-__device__ __forceinline__ double widen(float x) {
-  return __longlong_as_double((long long)(__float_as_int(x)) * (1 << 29) + 0x3800000000000000ll);
-}
+// A probability times 2^-896 as a double, from the bits of fp32 by one integer multiplication (the conversion instruction runs at an
+// eighth of the rate): the exponent fields differ by that in their bias, and zero and denormals come out right by themselves.
+// Negative numbers, minus zero among them, become zero. Differences are kept to 2^-178 of an unscaled number, so a sum over tokens
+// of which none has anything left is zero, and one is positive where some token has.
+constexpr double VERIFY_SCALE = 0x1p-896, VERIFY_UNSCALE = 0x1p896;
+__device__ __forceinline__ double scaled(float x) { return __longlong_as_double((long long)(max(__float_as_int(x), 0)) * (1 << 29)); }
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
-// max(x, 0) but for less than 2^-1040: only the upper word is looked at, in one integer operation.
-__device__ __forceinline__ double above_zero(double x) { return __hiloint2double(max(__double2hiint(x), 0), __double2loint(x)); }
-// A sum over a row of no more than this is none: what zeros come out as above adds up to 2^-106 at most.
-constexpr double VERIFY_NOTHING = 0x1p-100;
-
 // The sum over a warp's lanes, the same in all of them.
 __device__ __forceinline__ double warp_total(double x) {
 #pragma unroll
@@ -163,41 +159,42 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const __grid_
       const int t0 = g * EACH - off;
       if (t0 < 0 || t0 + EACH > V || (drawn && !together)) {       // the row's ends; rows that lie differently in memory
         for (int e = 0; e < EACH; ++e)
-          if (t0 + e >= 0 && t0 + e < V) part_sum[0] += left_at(t0 + e, count);
+          if (t0 + e >= 0 && t0 + e < V) part_sum[0] += left_at(t0 + e, count) * VERIFY_SCALE;
         continue;
       }
 #pragma unroll
       for (int e0 = 0; e0 < EACH; e0 += 4) {
         double r[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = widen(as_float(pt[e0 + e]));
+        for (int e = 0; e < 4; ++e) r[e] = scaled(as_float(pt[e0 + e]));
         if (drawn) {
           double q[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            q[e] = widen(as_float(qt[e0 + e]));
-            r[e] = above_zero(r[e] - q[e]);                        // the first rejection at a node, whose Z is 1
+            q[e] = scaled(as_float(qt[e0 + e]));
+            r[e] -= q[e];                                          // the first rejection at a node, whose Z is 1
           }
           for (int c = 1; c < count; ++c) {
             const double w = -weight[c];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) r[e] = above_zero(fma(w, q[e], r[e]));
+            for (int e = 0; e < 4; ++e) r[e] = fma(w, q[e], r[e]);
           }
         } else {
           for (int c = 0; c < count; ++c) {
             const double w = -weight[c];
             const long long x = gone[c] - (t0 + e0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) r[e] = x == e ? above_zero(r[e] + w) : r[e];
+            for (int e = 0; e < 4; ++e) r[e] = x == e ? fma(w, VERIFY_SCALE, r[e]) : r[e];
           }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) part_sum[e] += r[e];
+        for (int e = 0; e < 4; ++e)                                // what has become negative stays so: zero, at the end
+          if (__double2hiint(r[e]) >= 0) part_sum[e] += r[e];
       }
     }
     ptx::cp_async_wait<0>();
     double sum = (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
-    sum = warp_total(sum);
+    sum = warp_total(sum) * VERIFY_UNSCALE;
     if (lane == 0) warp_sum[warp] = sum;
     __syncthreads();
     const int slot = ++passes & 1;                                 // the pass before may still be read elsewhere
@@ -235,7 +232,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const __grid_
     if (tid == 0) { weight[rejections] = Z; gone[rejections] = tok[i]; }
     __syncthreads();
     const double rest = row_sum(rejections + 1);
-    if (rest > VERIFY_NOTHING) {
+    if (rest > 0.0) {
       ++rejections;
       Z = total = rest;
     }
@@ -244,7 +241,9 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const __grid_
 
   // ---- the last token: the CTA, the warp's part, the token whose running sum passes the threshold -----------
   const double threshold = ux[0] * total;
-  // Which of `count` parts, whose sums the lanes hold, the threshold falls into, and the sum before it.
+  // Which of `count` parts, whose sums the lanes hold, the threshold falls into, and the sum before it. Only a part with any mass is
+  // taken, so that a token that has none is not drawn: not by a threshold of zero, and not by the sums' rounding, which differs
+  // from lane to lane. Where no part passes the threshold, rounding again, it is the last one with mass.
   auto choose = [&](double sum, int count, double before, int& owner, double& start) {
     double upto = sum;
 #pragma unroll
@@ -252,10 +251,11 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const __grid_
       const double y = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += y;
     }
-    const uint32_t past = __ballot_sync(0xffffffffu, lane < count && before + upto > threshold);
-    const uint32_t any = __ballot_sync(0xffffffffu, lane < count && sum > 0.0);
-    owner = past ? __ffs(past) - 1 : any ? 31 - __clz(any) : 0;    // rounding: the last part with any mass
-    start = before + __shfl_sync(0xffffffffu, upto - sum, owner);
+    const bool mass = lane < count && sum > 0.0;
+    const uint32_t any = __ballot_sync(0xffffffffu, mass), past = __ballot_sync(0xffffffffu, mass && before + upto > threshold);
+    owner = past ? __ffs(past) - 1 : any ? 31 - __clz(any) : 0;
+    const double of_others = __shfl_sync(0xffffffffu, upto, owner > 0 ? owner - 1 : 0);
+    start = owner > 0 ? before + of_others : before;
   };
   int owner;
   double before;

@@ -349,6 +349,59 @@ def test_verification_at_its_edges():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,V", [(1, 1000), (1, 5000), (1, 70001), (200, 3000)])
+@pytest.mark.parametrize("drafts", ["none", "lookup", "sampled"])
+def test_last_token_of_sparse_rows(dtype, B, V, drafts):
+    """Targets of which all but a few tokens at the end are zero, and numbers down to zero: what is drawn has a probability."""
+    n = 1 if drafts == "none" else 2
+    target, uniform = torch.zeros(B, n, V, dtype=dtype), torch.zeros(B, n)
+    for b in range(B):
+        target[b, :, V - 4 - (7 * b) % 60] = 0.25
+        target[b, :, V - 2] = 0.75
+    draft = None
+    tokens = torch.full((B, n), 11)                          # which the target excludes
+    if drafts == "sampled":
+        draft = torch.full((B, n, V), 2.0 ** -13, dtype=dtype)
+        draft[:, :, 11] = 0.5
+    for u in (0.0, 2.0 ** -149, 2.0 ** -100, 0.2, 0.5, 1 - 2.0 ** -24):
+        uniform[:, 0] = u
+        want = _verify_reference(tokens, target, draft, uniform, None)
+        got = verify_drafts(tokens.cuda(), target.cuda(), None if draft is None else draft.cuda(), uniform.cuda())
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want)), u
+
+
+@pytest.mark.gpu
+def test_verification_down_to_the_smallest_probabilities():
+    """fp32 denormals count: in a row's sum, and as all that a rejection leaves."""
+    V = 1000
+    target, uniform, tokens = torch.zeros(1, 2, V), torch.zeros(1, 2), torch.tensor([[0, 640]])
+    target[0, :, 300], target[0, :, 640], target[0, :, 900] = 1e-42, 0.5, 0.5
+    for u in (0.0, 2.0 ** -149, 0.3):
+        uniform[0, 0] = u
+        want = _verify_reference(tokens[:, :1], target[:, :1], None, uniform[:, :1], None)
+        got = verify_drafts(tokens[:, :1].cuda(), target[:, :1].cuda(), None, uniform[:, :1].cuda())
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want)), u
+    draft = target * 2                                       # takes more of every token than there is, but for one
+    draft[:, :, 300] = 0
+    uniform[0, 1] = 1 - 2.0 ** -24
+    want = _verify_reference(tokens, target, draft, uniform, None)
+    got = verify_drafts(tokens.cuda(), target.cuda(), draft.cuda(), uniform.cuda())
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want)) and want[2].tolist() == [[300, -1]]
+
+
+@pytest.mark.gpu
+def test_an_empty_remainder_of_a_long_row():
+    """Nothing is left of a row of 2^28 tokens: their zeros do not add up to something, and the row itself stands."""
+    V = 1 << 28
+    row = torch.zeros(V, device="cuda")
+    row[V - 5] = 0.25                                        # a row that sums to a quarter
+    tokens, uniform = torch.tensor([[0, V - 5]], device="cuda"), torch.tensor([[0.5, 0.5]], device="cuda")
+    accepted, path, out = verify_drafts(tokens, row.expand(1, 2, V), None, uniform)
+    assert accepted.tolist() == [0] and path.tolist() == [[0, -1]] and out.tolist() == [[V - 5, -1]]
+
+
+@pytest.mark.gpu
 def test_verified_tokens_are_distributed_as_the_target():
     """First tokens over many draws of drafts and numbers against the target's probabilities: five standard deviations."""
     N, V, n = 40000, 12, 4
