@@ -11,11 +11,20 @@ SDPA is quicker on, one SDPA call. A few tokens behind a cache (2 to 64, e.g. th
 the reference's callable has no path for, are dense as well, on the kernel of `serving.tree_attn`: causal where there is
 no mask, else as the boolean mask (B or 1, 1, tokens or 1, keys) says.
 
-    from transformers import AttentionInterface
+    from transformers import AttentionInterface, AttentionMaskInterface
+    from transformers.masking_utils import sdpa_mask
     AttentionInterface.register("intra_b200", make_intra_attention())
+    AttentionMaskInterface.register("intra_b200", sdpa_mask)
     model = AutoModelForCausalLM.from_pretrained(..., attn_implementation="intra_b200")
+
+Both registrations are needed: transformers builds a mask only for names that are registered with `AttentionMaskInterface`, and
+without one nothing tells the rows of a static cache that are not filled, or a batch's padding, from keys. A few tokens behind a
+cache are refused where a model's attention has no such entry. (The patterns do not look at masks: padding in a prompt takes part, as
+in the reference.)
 """
 from __future__ import annotations
+
+import sys
 
 import torch
 import torch.nn.functional as F
@@ -54,6 +63,16 @@ def _kernel_is_quicker(units, S, masked):
     return units <= 512 and nbytes <= (44e6 if 24 <= units <= 256 else 28e6)
 
 
+def _masks_are_built(module):
+    """May no mask be taken for "causal, and every key is one"? Not where a transformers model calls under a name that no mask function
+    is registered for: it passes none whatever its cache holds."""
+    name = getattr(getattr(module, "config", None), "_attn_implementation", None)
+    transformers = sys.modules.get("transformers")
+    if not isinstance(name, str) or transformers is None or not hasattr(transformers, "AttentionMaskInterface"):
+        return True
+    return name in transformers.AttentionMaskInterface().valid_keys()
+
+
 def make_intra_attention(num_groups: int = NUM_GROUPS, back: int = WINDOW_BACK, chunk: int = WINDOW_CHUNK,
                          force_masktype=None):
     """Returns `fn(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0, **kw)`
@@ -76,6 +95,10 @@ def make_intra_attention(num_groups: int = NUM_GROUPS, back: int = WINDOW_BACK, 
             o = F.scaled_dot_product_attention(query, k2, v2, attn_mask=am, scale=scaling, is_causal=False)
             return o.transpose(1, 2).contiguous(), None
         if 1 < query.shape[2] < key.shape[2] and query.shape[2] <= MAX_TOKENS:     # drafted tokens behind a cache: dense, too
+            if attention_mask is None and not _masks_are_built(module):
+                raise ValueError(f"no mask function is registered for attention {module.config._attn_implementation!r}, so that unfilled "
+                                 "cache rows and padding would pass for keys: register transformers.masking_utils.sdpa_mask for it "
+                                 "with transformers.AttentionMaskInterface")
             if torch.is_grad_enabled():
                 query, key, value = query.detach(), key.detach(), value.detach()
             return _tree(query, key, value, None, None, attention_mask, scaling, attention_mask is not None), None

@@ -234,6 +234,96 @@ def test_backend_takes_a_few_tokens_behind_a_cache(H, Hkv, n, S, kind):
     assert torch.equal(again, out) and not again.requires_grad
 
 
+def _recipe():
+    """Runs what the backend's documentation says a user runs before the model is made."""
+    from intra_b200 import llm_backend
+    lines = [x.strip() for x in llm_backend.__doc__.splitlines() if x.startswith("    ")]
+    assert lines[-1].startswith("model =")
+    exec("\n".join(lines[:-1]), {"make_intra_attention": make_intra_attention})
+
+
+def _small_model(name, device, dtype):
+    from transformers import LlamaConfig, LlamaForCausalLM
+    config = LlamaConfig(hidden_size=64, num_attention_heads=8, num_key_value_heads=2, head_dim=128, num_hidden_layers=2, intermediate_size=64,
+                         vocab_size=50, attn_implementation=name)
+    torch.manual_seed(0)
+    return config, LlamaForCausalLM(config).to(device, dtype).eval()
+
+
+def _few_tokens_at_a_time(config, model, cache_kind, padded, chunks=(20, 5, 1, 12)):
+    """A left-padded batch and its cache through the model, some tokens at a time. Yields (tokens before, tokens, padding) of each call."""
+    from transformers import DynamicCache, StaticCache
+    cache = StaticCache(config=config, max_cache_len=96) if cache_kind == "static" else DynamicCache(config=config)
+    pad, before, device = [7, 0, 3] if padded else [0, 0, 0], 0, model.device
+    for n in chunks:
+        mask = (torch.arange(before + n)[None] >= torch.tensor(pad)[:, None]).long().to(device)
+        with torch.no_grad():
+            model(torch.randint(50, (3, n), generator=_gen(n)).to(device), attention_mask=mask, past_key_values=cache, use_cache=True)
+        yield before, n, pad
+        before += n
+
+
+def test_backend_asks_for_masks():
+    """The documented registration gives every call of a few tokens a mask, with any cache; a name without one is refused, and
+    does not get the unfilled rows of a static cache for keys."""
+    pytest.importorskip("transformers")
+    from transformers import AttentionInterface
+    _recipe()
+    fn, seen = make_intra_attention(), []
+
+    def record(module, query, key, value, attention_mask=None, scaling=None, **kw):
+        seen.append(None if attention_mask is None else (attention_mask.dtype, tuple(attention_mask.shape)))
+        return torch.zeros(query.shape[0], query.shape[2], query.shape[1], 128), None
+
+    AttentionInterface.register("intra_b200", record)
+    try:
+        for kind in ("static", "dynamic"):
+            config, model = _small_model("intra_b200", "cpu", torch.float32)
+            for before, n, _ in _few_tokens_at_a_time(config, model, kind, False):
+                if before and n > 1:
+                    S = 96 if kind == "static" else before + n
+                    assert seen == [(torch.bool, (3, 1, n, S))] * 2
+                seen.clear()
+    finally:
+        AttentionInterface.register("intra_b200", fn)
+    AttentionInterface.register("intra_b200_without_masks", fn)
+    config, model = _small_model("intra_b200_without_masks", "cpu", torch.float32)
+    with pytest.raises(ValueError, match="sdpa_mask"):
+        next(_few_tokens_at_a_time(config, model, "static", False))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("padded", [False, True])
+@pytest.mark.parametrize("kind", ["static", "dynamic"])
+def test_a_model_through_the_documented_registration(kind, padded):
+    """Every call of a model's attention with a few tokens, or one, behind a cache sees what has been filled and is no padding."""
+    pytest.importorskip("transformers")
+    from transformers import AttentionInterface
+    _recipe()
+    fn, calls = make_intra_attention(), []
+
+    def record(module, query, key, value, attention_mask=None, **kw):
+        out = fn(module, query, key, value, attention_mask, **kw)
+        calls.append((query.clone(), key.clone(), value.clone(), out[0].clone()))
+        return out
+
+    AttentionInterface.register("intra_b200", record)
+    try:
+        config, model = _small_model("intra_b200", "cuda", torch.bfloat16)
+        for before, n, pad in _few_tokens_at_a_time(config, model, kind, padded):
+            if before or kind == "static":                   # else a prompt, which the patterns take
+                assert len(calls) == 2
+                for q, k, v, out in calls:
+                    j, i = torch.arange(k.shape[2]), torch.arange(n)
+                    visible = ((j[None] <= (before + i)[:, None])[None] & (j[None] >= torch.tensor(pad)[:, None])[:, None]).cuda()
+                    ref, spread, _ = _reference(q, k, v, visible)
+                    real = (before + i[None] >= torch.tensor(pad)[:, None]).cuda()
+                    _check(out[real], ref[real], spread[real], 4 * n)
+            calls.clear()
+    finally:
+        AttentionInterface.register("intra_b200", fn)
+
+
 def _verify_reference(tokens, target, draft, uniform, parents):
     """The definition in Python floats (64 bits), one sequence at a time."""
     accepted, paths, outs = [], [], []
