@@ -9,7 +9,8 @@ running on the B200 kernels: query/key/value arrive as (B, H, S, D) and are hand
 library's decode kernel for bf16 caches with or without a padding mask, else, and for multi-head caches that
 SDPA is quicker on, one SDPA call. A few tokens behind a cache (2 to 64, e.g. the drafts of assisted generation), which
 the reference's callable has no path for, are dense as well, on the kernel of `serving.tree_attn`: causal where there is
-no mask, else as the boolean mask (B or 1, 1, tokens or 1, keys) says.
+no mask, else as the boolean mask (B or 1, 1, tokens or 1, keys) says; with masks that are additive or differ by head they are one SDPA
+call, like the decode step's.
 
     from transformers import AttentionInterface, AttentionMaskInterface
     from transformers.masking_utils import sdpa_mask
@@ -63,6 +64,16 @@ def _kernel_is_quicker(units, S, masked):
     return units <= 512 and nbytes <= (44e6 if 24 <= units <= 256 else 28e6)
 
 
+def _dense(query, key, value, mask, scaling):
+    """Dense attention over a cache as torch operators, for what the kernels do not take. `mask` may be longer than the cache."""
+    rep = query.shape[1] // key.shape[1]
+    k2 = key.repeat_interleave(rep, dim=1) if rep > 1 else key
+    v2 = value.repeat_interleave(rep, dim=1) if rep > 1 else value
+    am = mask[:, :, :, : k2.shape[-2]] if mask is not None else None
+    o = F.scaled_dot_product_attention(query, k2, v2, attn_mask=am, scale=scaling, is_causal=False)
+    return o.transpose(1, 2).contiguous()
+
+
 def _masks_are_built(module):
     """May no mask be taken for "causal, and every key is one"? Not where a transformers model calls under a name that no mask function
     is registered for: it passes none whatever its cache holds."""
@@ -89,11 +100,7 @@ def make_intra_attention(num_groups: int = NUM_GROUPS, back: int = WINDOW_BACK, 
                 out = decode_attn(query, key, value, attention_mask, scaling)
                 if out is not None:
                     return out, None
-            k2 = key.repeat_interleave(rep, dim=1) if rep > 1 else key
-            v2 = value.repeat_interleave(rep, dim=1) if rep > 1 else value
-            am = attention_mask[:, :, :, : k2.shape[-2]] if attention_mask is not None else None
-            o = F.scaled_dot_product_attention(query, k2, v2, attn_mask=am, scale=scaling, is_causal=False)
-            return o.transpose(1, 2).contiguous(), None
+            return _dense(query, key, value, attention_mask, scaling), None
         if 1 < query.shape[2] < key.shape[2] and query.shape[2] <= MAX_TOKENS:     # drafted tokens behind a cache: dense, too
             if attention_mask is None and not _masks_are_built(module):
                 raise ValueError(f"no mask function is registered for attention {module.config._attn_implementation!r}, so that unfilled "
@@ -101,6 +108,9 @@ def make_intra_attention(num_groups: int = NUM_GROUPS, back: int = WINDOW_BACK, 
                                  "with transformers.AttentionMaskInterface")
             if torch.is_grad_enabled():
                 query, key, value = query.detach(), key.detach(), value.detach()
+            if attention_mask is not None and (attention_mask.dtype != torch.bool or (attention_mask.dim() == 4 and attention_mask.shape[1] != 1
+                                                                                      and attention_mask.stride(1) != 0)):
+                return _dense(query, key, value, attention_mask, scaling), None
             return _tree(query, key, value, None, None, attention_mask, scaling, attention_mask is not None), None
         mt = force_masktype if force_masktype is not None else layer_masktype(getattr(module, "layer_idx", 0))
         if torch.is_grad_enabled():          # the kernels are forward-only; this callable is, too

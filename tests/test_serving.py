@@ -234,6 +234,28 @@ def test_backend_takes_a_few_tokens_behind_a_cache(H, Hkv, n, S, kind):
     assert torch.equal(again, out) and not again.requires_grad
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 4, 20])
+def test_backend_takes_masks_the_kernel_does_not(n):
+    """Additive masks and masks per head, one token or a few behind a cache."""
+    B, H, Hkv, S = 2, 8, 2, 150
+    q, (k, v), fn = _queries(B, H, n, 6), _cache(B, Hkv, S, 6), make_intra_attention()
+    seen = (torch.rand(B, H, n, S + 4, generator=_gen(n)) < 0.6).cuda()
+    seen[..., 0] = True
+    for given in (seen, seen[:, :1]):
+        additive = torch.zeros(given.shape, dtype=torch.bfloat16, device="cuda").masked_fill(~given, torch.finfo(torch.bfloat16).min)
+        s = q.double() @ k.double().repeat_interleave(H // Hkv, 1).transpose(-1, -2) * SCALE
+        p = s.masked_fill(~given[..., :S], float("-inf")).softmax(-1)
+        vv = v.double().repeat_interleave(H // Hkv, 1)
+        ref, spread = (p @ vv).transpose(1, 2), (p @ vv.abs()).transpose(1, 2)
+        for mask in (additive, given):
+            out, w = fn(None, q, k, v, mask, scaling=SCALE)
+            assert w is None and out.shape == (B, n, H, 128)
+            # SDPA's probabilities are bf16 numbers (half a step each, 2^-9), and so may its scores be (up to 8: 2^-6 absolute)
+            excess = (out.double() - ref).abs() - (2.0 ** -8 * ref.abs() + 2.0 ** -5 * spread)
+            assert float(excess.max()) <= 0
+
+
 def _recipe():
     """Runs what the backend's documentation says a user runs before the model is made."""
     from intra_b200 import llm_backend
