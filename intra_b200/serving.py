@@ -20,6 +20,7 @@ import array
 import ctypes
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _loader
 from ._loader import lib
@@ -181,6 +182,7 @@ def decode_attn_accumulate(q, k, v, weights, lengths=None, mask=None, softmax_sc
                                                 ws[0], ws[1], scale, index, stream)
 
     _with_scratch((0, B, S, H, Hkv, index), call, dev)
+    increment_version(weights)               # written through its address: autograd has to know
     return out
 
 
@@ -341,6 +343,7 @@ def keep_drafts(caches, lengths, path):
                                     nodes, path_stride, B, S, Hkv, n, index, _raw_stream(index))
     if rc != 0:
         _raise(rc)
+    increment_version(caches)
 
 
 def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
@@ -396,6 +399,7 @@ def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
             _raise(rc)
     if out is None:
         return k2, v2, w2, kept
+    increment_version((k2, v2, w2))
     return k2[:, :, :keep], v2[:, :, :keep], w2[:, :, :keep], kept
 
 

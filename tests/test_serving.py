@@ -678,6 +678,32 @@ def test_a_serving_step_in_a_graph_and_on_another_stream():
         assert all(torch.equal(a, b) for a, b in zip(result, want))
 
 
+@pytest.mark.gpu
+def test_autograd_learns_of_what_is_written_in_place():
+    """A tensor that a graph has saved and one of these calls has overwritten since: backward raises, as behind any in-place operator."""
+    k, v = _cache(2, 2, 50, 1)
+    q, base = _queries(2, 8, 1, 1), torch.rand(2, 2, 50, generator=_gen(1)).cuda()
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    out = [k.new_zeros(2, 2, 9, 128), k.new_zeros(2, 2, 9, 128), base.new_zeros(2, 2, 9)]
+    other = base.clone()
+    calls = [(lambda: decode_attn_accumulate(q, k, v, base), [base]), (lambda: keep_drafts([k, v], ints([9, 40]), ints([[0, 2], [1, -1]])), [k, v]),
+             (lambda: evict_cache(k, v, other, 7, out=out), out)]
+    for call, written in calls:
+        for x in written:
+            leaf = torch.ones((), device="cuda", dtype=x.dtype, requires_grad=True)
+            (leaf * x).sum().backward()
+            saved = (leaf * x).sum()
+            with torch.no_grad():
+                call()
+            with pytest.raises(RuntimeError, match="inplace"):
+                saved.backward()
+    assert other._version == 0
+    with torch.inference_mode():                             # whose tensors have no versions
+        w = torch.zeros(2, 2, 50, device="cuda")
+        decode_attn_accumulate(q, k, v, w)
+        keep_drafts([k.clone()], ints([9, 40]), ints([[0, 2], [1, -1]]))
+
+
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 def test_refusals(device):
     bf = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16, device=device)
