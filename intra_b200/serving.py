@@ -24,16 +24,29 @@ from torch.autograd.graph import increment_version
 
 from . import _loader
 from ._loader import lib
-from .interface import _byte_span, _c_strides, _raise, _raw_stream
+from .interface import _byte_span, _c_strides, _dispatch_modes, _forward_ad, _raise, _raw_stream, _tracing_state
 
 MAX_TOKENS = 64             # nodes of a tree: ancestors are kept as 64 bits
 _PROB_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _SCALE = 128 ** -0.5
 
 
-def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
+def _forward_only(*tensors):
+    """Refuses what these kernels would pass by without a trace: gradients, tangents, programs that are being recorded, and tensors that
+    carry out operators themselves and have no memory of their own (fake or distributed ones). None stands for an argument left out."""
+    for x in tensors:
+        if type(x) is not torch.Tensor and x is not None and type(x).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__:
+            raise ValueError(f"INTRA kernels need tensors with memory of their own, not {type(x).__name__}")
+    if torch.is_grad_enabled() and any([x is not None and x.requires_grad for x in tensors]):
         raise RuntimeError("INTRA kernels are forward-only; call them under torch.no_grad()")
+    if _tracing_state is not None and _tracing_state() is not None:
+        raise RuntimeError("INTRA kernels cannot be recorded by torch.jit.trace")
+    if _dispatch_modes is not None and _dispatch_modes() > 0:
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        if get_proxy_mode() is not None:
+            raise RuntimeError("INTRA kernels cannot be recorded by torch.fx")
+    if getattr(_forward_ad, "_current_level", -1) >= 0 and any([x is not None and _forward_ad.unpack_dual(x).tangent is not None for x in tensors]):
+        raise RuntimeError("INTRA kernels are forward-only; tangents would be lost")
 
 
 def _rows_usable(x):
@@ -49,8 +62,6 @@ def _attention_inputs(q, k, v):
     if not (q.is_cuda and q.dtype is bf16 and k.dtype is bf16 and v.dtype is bf16 and len(qn) == 4 and len(kn) == 4
             and qn[3] == 128 and kn[3] == 128):
         raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
-    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        raise RuntimeError("INTRA kernels are forward-only; call them under torch.no_grad()")
     if kn != v.shape or kn[0] != qn[0] or kn[1] == 0 or qn[1] == 0 or qn[1] % kn[1]:
         raise ValueError(f"incompatible shapes q={tuple(qn)} k={tuple(kn)} v={tuple(v.shape)}")
     if k.device != dev or v.device != dev:
@@ -126,6 +137,7 @@ def tree_attn(q, k, v, parents=None, lengths=None, mask=None, softmax_scale=None
 
 def _tree(q, k, v, parents, lengths, mask, softmax_scale, all_own):
     """tree_attn; with `all_own` the tokens see all their own keys, so that the mask decides alone."""
+    _forward_only(q, k, v, parents, lengths, mask)
     q, k, v, qs, ks, vs, dev = _attention_inputs(q, k, v)
     B, H, n, D = q.shape
     _, Hkv, S, _ = k.shape
@@ -154,6 +166,7 @@ def decode_attn_accumulate(q, k, v, weights, lengths=None, mask=None, softmax_sc
     sees rows 0 .. lengths[b], its own being the last of them; `lengths` (B,) int32, None: all S. (Values outside 0 ..
     S - 1 are brought into that range.) `mask`, bool (B or 1, 1, 1, >= S), hides further keys. Weights of keys the
     token does not see stay as they are. Returns (B, 1, H, 128)."""
+    _forward_only(q, k, v, weights, lengths, mask)
     q, k, v, qs, ks, vs, dev = _attention_inputs(q, k, v)
     B, H, n, D = q.shape
     _, Hkv, S, _ = k.shape
@@ -162,7 +175,6 @@ def decode_attn_accumulate(q, k, v, weights, lengths=None, mask=None, softmax_sc
     wn, ws = weights.shape, weights.stride()
     if weights.dtype is not torch.float32 or len(wn) != 3 or wn[0] != B or wn[1] != Hkv or wn[2] < S or weights.device != dev:
         raise ValueError(f"weights must be float32 (batch, KV heads, at least {S}) on {dev}")
-    _no_grad(weights)
     if not (ws[2] == 1 and ws[1] >= wn[2] and ws[0] >= ws[1] * Hkv):     # else look closer
         _distinct_rows(wn, ws, "weights")
     lengths, used, _ = _integers(lengths, "lengths", (B,), dev)
@@ -213,12 +225,12 @@ def verify_drafts(tokens, target_probs, draft_probs, uniform, parents=None):
 
     Returns accepted (B,) int32, the number m of accepted drafts; path (B, n) int32, the nodes from 0 on, then -1; and tokens
     (B, n) int64: the m accepted ones, the drawn one, then -1. Drafts outside the vocabulary are rejected."""
+    _forward_only(tokens, target_probs, draft_probs, uniform, parents)
     pn, kind = target_probs.shape, _PROB_TYPES.get(target_probs.dtype)
     if len(pn) != 3 or kind is None or not target_probs.is_cuda:
         raise ValueError("target_probs must be a CUDA float32, bfloat16 or float16 tensor (batch, nodes, vocabulary)")
     B, n, V = pn
     dev = target_probs.device
-    _no_grad(target_probs, draft_probs, uniform)
     if not 1 <= n <= MAX_TOKENS or V == 0:
         raise ValueError(f"expected 1 to {MAX_TOKENS} nodes and a vocabulary, got {n} and {V}")
     wide = tokens.dtype is torch.int64
@@ -300,9 +312,10 @@ def keep_drafts(caches, lengths, path):
     caches = [caches] if isinstance(caches, torch.Tensor) else list(caches)
     if not caches:
         return
+    _forward_only(lengths, path, *caches)
     first, count = caches[0], len(caches)
     dev, shape, bf16 = first.device, first.shape, torch.bfloat16
-    index, grad, alike, pointers = dev.index, torch.is_grad_enabled(), first.is_contiguous(), []
+    index, alike, pointers = dev.index, first.is_contiguous(), []
     if not first.is_cuda or len(shape) != 4 or shape[3] != 128:
         raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
     for x in caches:
@@ -310,8 +323,6 @@ def keep_drafts(caches, lengths, path):
             raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
         if x.shape != shape or x.get_device() != index:
             raise ValueError("caches must agree in shape and device")
-        if grad and x.requires_grad:
-            raise RuntimeError("INTRA kernels are forward-only; call them under torch.no_grad()")
         alike = alike and x.is_contiguous()
         pointers.append(x.data_ptr())
     layouts = {x.stride() for x in caches} if not alike else {first.stride()}
@@ -355,10 +366,10 @@ def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
     Returns (k, v, weights, kept): the kept rows, their weights and their old places (B, Hkv, keep) int32. Behind a sequence's
     last row come zeros, and -1 in `kept`; lengths are min(lengths, keep) from then on. `out` = (k, v, weights) writes into the
     caller's tensors of at least `keep` rows, whose rows from `keep` on stay as they are; they must not overlap the inputs."""
+    _forward_only(k, v, weights, lengths, *(() if out is None else out))
     kn, dev, bf16 = k.shape, k.device, torch.bfloat16
     if not k.is_cuda or k.dtype is not bf16 or v.dtype is not bf16 or len(kn) != 4 or kn[3] != 128:
         raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
-    _no_grad(k, v, weights)
     B, Hkv, S, D = kn
     if v.shape != kn or v.device != dev or S == 0:
         raise ValueError(f"incompatible shapes k={tuple(kn)} v={tuple(v.shape)}")
@@ -383,7 +394,6 @@ def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
                 raise ValueError("out needs unit stride in the last dimension and 16-byte aligned rows")
         if w2.dtype is not torch.float32 or w2.dim() != 3 or w2.shape[:2] != kn[:2] or w2.shape[2] < keep or w2.device != dev:
             raise ValueError(f"out needs float32 ({B}, {Hkv}, at least {keep}) for the weights on {dev}")
-        _no_grad(k2, v2, w2)
         for x in (k2, v2, w2):
             _distinct_rows(x.shape, x.stride(), "out")
         if _overlapping((k2, v2, w2)) or any(_overlapping((x, y)) for x in (k2, v2, w2) for y in (k, v, weights)):

@@ -704,6 +704,57 @@ def test_autograd_learns_of_what_is_written_in_place():
         keep_drafts([k.clone()], ints([9, 40]), ints([[0, 2], [1, -1]]))
 
 
+def _calls(q, k, w, probs, tok, u, ints):
+    """A call of each operator that takes the given tensors."""
+    return [lambda: tree_attn(q, k, k), lambda: decode_attn_accumulate(q[:, :, :1], k, k, w), lambda: verify_drafts(tok, probs, None, u),
+            lambda: keep_drafts([k], ints(2), ints(2, 4)), lambda: evict_cache(k, k, w, 5)]
+
+
+def test_tensors_without_memory_are_refused():
+    """Fake tensors, whose addresses are zero and an offset, before any address is looked at."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        q, k, w = torch.zeros(2, 8, 4, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 2, 60, 128, dtype=torch.bfloat16, device="cuda")[:, :, 10:], torch.zeros(2, 2, 50, device="cuda")
+        ints = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device="cuda")
+        for call in _calls(q, k, w, torch.ones(2, 4, 9, device="cuda"), torch.zeros(2, 4, dtype=torch.int64, device="cuda"), torch.zeros(2, 4, device="cuda"), ints):
+            with pytest.raises(ValueError, match="memory of their own"):
+                call()
+
+
+@pytest.mark.gpu
+def test_what_looks_inside_operators_is_refused():
+    """Tangents, recorders and batched tensors are not passed by; a subclass that leaves operators alone is a tensor like others."""
+    import torch.autograd.forward_ad as fw
+    from torch.fx.experimental.proxy_tensor import make_fx
+    ints = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device="cuda")
+    given = [_queries(2, 8, 4, 1), _cache(2, 2, 50, 1)[0], torch.rand(2, 2, 50, generator=_gen(1)).cuda(), torch.ones(2, 4, 9, device="cuda"),
+             torch.zeros(2, 4, dtype=torch.int64, device="cuda"), torch.rand(2, 4, generator=_gen(2)).cuda()]
+    with fw.dual_level():
+        duals = [x if x.dtype == torch.int64 else fw.make_dual(x, torch.ones_like(x)) for x in given]
+        for call in _calls(*duals, ints):
+            with pytest.raises(RuntimeError, match="tangents"):
+                call()
+        for call in _calls(*given, ints):                    # no tangents among these
+            call()
+    for which in range(5):
+        def one(x):
+            _calls(x, *given[1:], ints)[0]() if which == 0 else _calls(*given, ints)[which]()
+            return x + 1
+
+        with pytest.raises(RuntimeError, match="recorded"):
+            torch.jit.trace(one, (given[0],), check_trace=False)
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(one)(given[0])
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda x: tree_attn(x, given[1], given[1]))(given[0][None])
+
+    class Named(torch.Tensor):
+        pass
+
+    assert torch.equal(tree_attn(given[0].as_subclass(Named), given[1], given[1]).as_subclass(torch.Tensor), tree_attn(given[0], given[1], given[1]))
+    assert torch.equal(tree_attn(torch.nn.Parameter(given[0], requires_grad=False), given[1], given[1]), tree_attn(given[0], given[1], given[1]))
+
+
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 def test_refusals(device):
     bf = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16, device=device)
