@@ -175,6 +175,8 @@ def decode_attn_accumulate(q, k, v, weights, lengths=None, mask=None, softmax_sc
     wn, ws = weights.shape, weights.stride()
     if weights.dtype is not torch.float32 or len(wn) != 3 or wn[0] != B or wn[1] != Hkv or wn[2] < S or weights.device != dev:
         raise ValueError(f"weights must be float32 (batch, KV heads, at least {S}) on {dev}")
+    if weights.is_neg():
+        raise ValueError("weights must not be a negated view")
     if not (ws[2] == 1 and ws[1] >= wn[2] and ws[0] >= ws[1] * Hkv):     # else look closer
         _distinct_rows(wn, ws, "weights")
     lengths, used, _ = _integers(lengths, "lengths", (B,), dev)
@@ -251,6 +253,7 @@ def verify_drafts(tokens, target_probs, draft_probs, uniform, parents=None):
     out = tokens.new_empty((B, n)) if wide else uniform.new_empty((B, n), dtype=torch.int64)
     if B == 0:
         return accepted, path, out
+    target_probs, uniform = target_probs.resolve_neg(), uniform.resolve_neg()
     if target_probs.stride(2) != 1:
         target_probs = target_probs.contiguous()
     if tokens.stride(1) != 1:
@@ -259,6 +262,7 @@ def verify_drafts(tokens, target_probs, draft_probs, uniform, parents=None):
         uniform = uniform.contiguous()
     ds = None
     if draft_probs is not None:
+        draft_probs = draft_probs.resolve_neg()
         if draft_probs.stride(2) != 1:
             draft_probs = draft_probs.contiguous()
         ds = _c_strides(*draft_probs.stride())
@@ -381,6 +385,7 @@ def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
         raise ValueError(f"expected keep >= 1 and recent from 0 to keep, got {keep} and {recent}")
     lengths, used, _ = _integers(lengths, "lengths", (B,), dev)
     k, v = k if _rows_usable(k) else k.contiguous(), v if _rows_usable(v) else v.contiguous()
+    weights = weights.resolve_neg()
     if weights.stride(2) != 1:
         weights = weights.contiguous()
     if out is None:
@@ -392,7 +397,7 @@ def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
                 raise ValueError(f"out needs bfloat16 ({B}, {Hkv}, at least {keep}, 128) for k and v on {dev}")
             if not _rows_usable(x):
                 raise ValueError("out needs unit stride in the last dimension and 16-byte aligned rows")
-        if w2.dtype is not torch.float32 or w2.dim() != 3 or w2.shape[:2] != kn[:2] or w2.shape[2] < keep or w2.device != dev:
+        if w2.dtype is not torch.float32 or w2.dim() != 3 or w2.shape[:2] != kn[:2] or w2.shape[2] < keep or w2.device != dev or w2.is_neg():
             raise ValueError(f"out needs float32 ({B}, {Hkv}, at least {keep}) for the weights on {dev}")
         for x in (k2, v2, w2):
             _distinct_rows(x.shape, x.stride(), "out")

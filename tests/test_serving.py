@@ -755,6 +755,23 @@ def test_what_looks_inside_operators_is_refused():
     assert torch.equal(tree_attn(torch.nn.Parameter(given[0], requires_grad=False), given[1], given[1]), tree_attn(given[0], given[1], given[1]))
 
 
+@pytest.mark.gpu
+def test_negated_views_keep_their_sign():
+    """The imaginary part of a conjugate is a view whose sign is a flag."""
+    negated = lambda x: torch.complex(torch.zeros_like(x), -x).conj().imag
+    k, w = _cache(2, 2, 50, 1)[0], torch.rand(2, 2, 50, generator=_gen(1)).cuda()
+    probs, tok, u = torch.rand(2, 4, 9, generator=_gen(3)).cuda(), torch.randint(9, (2, 4), generator=_gen(4)).cuda(), torch.rand(2, 4, generator=_gen(2)).cuda()
+    assert negated(w).is_neg() and torch.equal(negated(w), w)
+    want = verify_drafts(tok, probs, probs.flip(-1), u)
+    for got in (verify_drafts(tok, negated(probs), probs.flip(-1), u), verify_drafts(tok, probs, negated(probs.flip(-1)), u), verify_drafts(tok, probs, probs.flip(-1), negated(u))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(evict_cache(k, k, negated(w), 9, 3), evict_cache(k, k, w, 9, 3)))
+    with pytest.raises(ValueError, match="negated"):         # written in place
+        decode_attn_accumulate(_queries(2, 8, 1, 1), k, k, negated(w))
+    with pytest.raises(ValueError):
+        evict_cache(k, k, w, 9, out=(k.new_zeros(2, 2, 9, 128), k.new_zeros(2, 2, 9, 128), negated(w)))
+
+
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 def test_refusals(device):
     bf = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16, device=device)
