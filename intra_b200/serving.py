@@ -55,6 +55,11 @@ def _rows_usable(x):
     return s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and not x.data_ptr() & 15
 
 
+def _usable(x):
+    """x, or a copy whose rows the kernels can read. (contiguous() would hand back a contiguous tensor at an odd address.)"""
+    return x if _rows_usable(x) else x.clone(memory_format=torch.contiguous_format)
+
+
 def _attention_inputs(q, k, v):
     """q (B, H, n, 128) and a cache k, v (B, Hkv, S, 128) as the kernels can read them (tensors whose rows are not 16-byte
     aligned are copied), their strides {batch, token, head} for the C ABI, and their device. Raises for others."""
@@ -69,7 +74,7 @@ def _attention_inputs(q, k, v):
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     if (qs[3] != 1 or ks[3] != 1 or vs[3] != 1 or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15
             or (qs[0] | qs[1] | qs[2] | ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & 7):
-        q, k, v = (x if _rows_usable(x) else x.contiguous() for x in (q, k, v))
+        q, k, v = _usable(q), _usable(k), _usable(v)
         qs, ks, vs = q.stride(), k.stride(), v.stride()
     return (q, k, v, _c_strides(qs[0], qs[2], qs[1]), _c_strides(ks[0], ks[2], ks[1]), _c_strides(vs[0], vs[2], vs[1]), dev)
 
@@ -384,7 +389,7 @@ def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
     if not 1 <= keep or not 0 <= recent <= keep:
         raise ValueError(f"expected keep >= 1 and recent from 0 to keep, got {keep} and {recent}")
     lengths, used, _ = _integers(lengths, "lengths", (B,), dev)
-    k, v = k if _rows_usable(k) else k.contiguous(), v if _rows_usable(v) else v.contiguous()
+    k, v = _usable(k), _usable(v)
     weights = weights.resolve_neg()
     if weights.stride(2) != 1:
         weights = weights.contiguous()

@@ -772,6 +772,30 @@ def test_negated_views_keep_their_sign():
         evict_cache(k, k, w, 9, out=(k.new_zeros(2, 2, 9, 128), k.new_zeros(2, 2, 9, 128), negated(w)))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 4, 20])
+def test_rows_at_odd_addresses_are_copied(n):
+    """Contiguous tensors that begin between two 16-byte boundaries, and a batch of one whose unused strides are odd."""
+    def odd(x):
+        room = torch.empty(x.numel() + 8, dtype=x.dtype, device="cuda")[1:x.numel() + 1].view(x.shape)
+        return room.copy_(x)
+
+    def strange(x):
+        return x.as_strided(x.shape, (3, 5, 128, 1))
+
+    (k, v), q = _cache(1, 1, 70, 2), _queries(1, 4, n, 2)
+    w = torch.rand(1, 1, 70, generator=_gen(1)).cuda()
+    want, want_cut = tree_attn(q, k, v), evict_cache(k, v, w, 9, 3)
+    want_one = decode_attn_accumulate(q[:, :, :1], k, v, w.clone())
+    for change in (odd, strange):
+        k2, v2 = change(k), change(v)
+        q2 = odd(q)
+        assert q2.is_contiguous() and k2.is_contiguous() and torch.equal(k2, k)
+        assert torch.equal(tree_attn(q2, k2, v), want) and torch.equal(tree_attn(q, k, v2), want)
+        assert torch.equal(decode_attn_accumulate(q2[:, :, :1], k2, v2, w.clone()), want_one)
+        assert all(torch.equal(a, b) for a, b in zip(evict_cache(k2, v2, w, 9, 3), want_cut))
+
+
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 def test_refusals(device):
     bf = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16, device=device)
