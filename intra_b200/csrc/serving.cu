@@ -120,7 +120,8 @@ int launch_tree_mma(TreeParams p, const ServingState& st, int64_t scratch_bytes,
     if (int64_t(p.B) * p.Hkv > 65535) return INTRA_ERR_UNSUPPORTED;      // grid.y of the accumulation
     p.score_keys = ceil_div(p.S, TREE_BLOCK) * TREE_BLOCK;
     p.scores = p.scratch + floats;
-    floats += units * TREE_ROWS * p.score_keys;
+    p.score_rows = imin(all_rows, TREE_ROWS);
+    floats += units * p.score_rows * p.score_keys;
   }
   *scratch_needed = floats * int64_t(sizeof(float));
   if (!p.scratch || scratch_bytes < *scratch_needed) return INTRA_NEED_SCRATCH;

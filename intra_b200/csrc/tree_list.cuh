@@ -35,12 +35,12 @@ struct TreeParams {
   const uint8_t* live;
   int bits_tokens, bits_words, live_words;
   // tree_mma_kernel.cuh, a decode step that accumulates: (B, Hkv, S) by strides, unit stride over keys, and the scores of
-  // every visible key, [unit][row][score_keys], times scale_log2
+  // every visible key, [unit][row][score_keys], times scale_log2; a unit has as many rows there as it has query heads at most
   float* weights;
   int64_t weights_sb, weights_sh;
   int weights_vec;             // four weights can be loaded at once
   float* scores;
-  int score_keys;
+  int score_keys, score_rows;
   int S, H, Hkv, n, B;
   int row_groups;              // units per KV head
   int unit_cost, min_tiles;    // see TreeList; a CTA's part is at least this many tiles

@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(TREE_THREADS, TREE_CTAS_PER_SM) tree_mma_kerne
               x[h][i] = (bits >> key) & 1u ? s[i >> 1][2 * h + (i & 1)] * p.scale_log2 : -CUDART_INF_F;
             }
             if (ACCUMULATE && 8 * h + g < n_rows) {                // 32 bytes of a row per four lanes
-              float* const dst = p.scores + (int64_t(unit) * TREE_ROWS + 8 * h + g) * p.score_keys + key0 + 2 * j;
+              float* const dst = p.scores + (int64_t(unit) * p.score_rows + 8 * h + g) * p.score_keys + key0 + 2 * j;
               *reinterpret_cast<float2*>(dst) = make_float2(x[h][0], x[h][1]);
               *reinterpret_cast<float2*>(dst + 8) = make_float2(x[h][2], x[h][3]);
             }
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(TREE_WEIGHT_THREADS, TREE_WEIGHT_CTAS_PER_SM) 
         for (int r = warp; r < n_rows; r += TREE_WEIGHT_THREADS / 32) tree_merge_row<4>(p, parts, unit, b, hk, rg * TREE_ROWS + r, r);
       continue;
     }
-    const float* const x = p.scores + int64_t(unit) * TREE_ROWS * p.score_keys;
+    const float* const x = p.scores + int64_t(unit) * p.score_rows * p.score_keys;
     constexpr int AT_ONCE = 4;                                     // rows whose scores are under way together
     bool first_block = true;
     for (int key0 = blockIdx.x * TREE_WEIGHT_KEYS + 4 * threadIdx.x; key0 - 4 * int(threadIdx.x) < keys; key0 += (gridDim.x - 1) * TREE_WEIGHT_KEYS) {

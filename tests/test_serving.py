@@ -796,6 +796,21 @@ def test_rows_at_odd_addresses_are_copied(n):
         assert all(torch.equal(a, b) for a, b in zip(evict_cache(k2, v2, w, 9, 3), want_cut))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,rows", [(32, 8, 4), (32, 32, 1), (36, 2, 32), (8, 1, 8)])
+def test_scratch_of_the_step_with_weights(lib, H, Hkv, rows):
+    """A score per key and query head (in groups of 16 where a KV head has more), and the partial results: no more."""
+    import ctypes
+    B, S, need = 16, 65536, ctypes.c_int64(0)
+    p = torch.zeros(64, dtype=torch.uint8, device="cuda").data_ptr()
+    qs, st = (ctypes.c_int64 * 3)(H * 128, H * 128, 128), (ctypes.c_int64 * 3)(Hkv * S * 128, 128, S * 128)
+    rc = lib.intra_b200_decode_accumulate(p, p, p, None, None, p, p, None, 0, need, B, S, H, Hkv, qs, st, st, None, S * Hkv, S, 0.1, 0, None)
+    assert rc == 1                                           # nothing is launched
+    units = B * Hkv * (1 if rows <= 16 else 2)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert need.value <= 4 * (B * Hkv * rows * S + (units + 2 * sms) * 16 * 130)
+
+
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 def test_refusals(device):
     bf = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16, device=device)
