@@ -31,17 +31,23 @@ _PROB_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _SCALE = 128 ** -0.5
 
 
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
+_tracing = _tracing_state or (lambda: None)
+_modes = _dispatch_modes or (lambda: 0)
+
+
 def _forward_only(*tensors):
     """Refuses what these kernels would pass by without a trace: gradients, tangents, programs that are being recorded, and tensors that
     carry out operators themselves and have no memory of their own (fake or distributed ones). None stands for an argument left out."""
-    for x in tensors:
-        if type(x) is not torch.Tensor and x is not None and type(x).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__:
-            raise ValueError(f"INTRA kernels need tensors with memory of their own, not {type(x).__name__}")
-    if torch.is_grad_enabled() and any([x is not None and x.requires_grad for x in tensors]):
+    if not _PLAIN.issuperset(map(type, tensors)):
+        for x in tensors:
+            if x is not None and type(x).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__:
+                raise ValueError(f"INTRA kernels need tensors with memory of their own, not {type(x).__name__}")
+    if torch.is_grad_enabled() and True in [x.requires_grad for x in tensors if x is not None]:
         raise RuntimeError("INTRA kernels are forward-only; call them under torch.no_grad()")
-    if _tracing_state is not None and _tracing_state() is not None:
+    if _tracing() is not None:
         raise RuntimeError("INTRA kernels cannot be recorded by torch.jit.trace")
-    if _dispatch_modes is not None and _dispatch_modes() > 0:
+    if _modes() > 0:
         from torch.fx.experimental.proxy_tensor import get_proxy_mode
         if get_proxy_mode() is not None:
             raise RuntimeError("INTRA kernels cannot be recorded by torch.fx")
