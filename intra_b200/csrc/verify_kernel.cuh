@@ -181,8 +181,9 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const __grid_
           }
         } else {
           for (int c = 0; c < count; ++c) {
-            const double w = -weight[c];
             const long long x = gone[c] - (t0 + e0);
+            if (x < 0 || x > 3) continue;
+            const double w = -weight[c];
 #pragma unroll
             for (int e = 0; e < 4; ++e) r[e] = x == e ? fma(w, VERIFY_SCALE, r[e]) : r[e];
           }
