@@ -124,7 +124,9 @@ int intra_b200_tree_attn(const void* q, const void* k, const void* v, const int*
  * R into max(R - Z q, 0) and Z into its sum, where that is not zero. At the end one token is drawn from R: the
  * smallest t with R(0) + .. + R(t) > uniform[b][0] * sum R. Sums in 64 bits. Outputs, contiguous: accepted[b], the number
  * of accepted drafts m; path[b] = 0 and the accepted nodes, then -1; out_tokens[b]: the accepted tokens, the drawn one
- * at place m, then -1. Drafts outside 0 .. V - 1 are rejected. Strides in elements {batch, node}; unit stride over V, which is
+ * at place m, then -1. Drafts outside 0 .. V - 1 are rejected. Tokens come
+ * out distributed as the target's if a node's children were drawn independently of one another. Probabilities are finite and not negative; a
+ * row that holds others gives some token of the vocabulary. Strides in elements {batch, node}; unit stride over V, which is
  * at most 2^30. */
 #define INTRA_PROB_F32 0
 #define INTRA_PROB_BF16 1

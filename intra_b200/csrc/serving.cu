@@ -322,8 +322,9 @@ int intra_b200_verify_drafts(const void* tokens, int tokens_int64, const void* t
   p.tokens_sb = tokens_batch_stride; p.uniform_sb = uniform_batch_stride; p.parents_sb = parents_batch_stride;
   p.n = n; p.V = V;
   // CTAs of a sequence's cluster: as many as fit the GPU at once (two CTAs an SM) and have a few thousand tokens each. Measured with
-  // 1 / 2 / 4 / 8, us: 1 x 50257 tokens 15.9 / 11.8 / 9.5 / 8.6, 32 x 128257 37.7 / 23.2 / 16.5 / 17.3, 64 x 50257 19.8 / 15.0 / 14.9 /
-  // 22.8, 150 x 30000 17.4 / 19.1 / 23.9 / 39.4; 1 x 4000 6.7 / 6.2 / 6.0 / 6.1.
+  // 1 / 2 / 4 / 8, us, fp32 with draft probabilities, chains of 9 nodes: 1 x 50257 tokens 18.6 / 13.4 / 10.4 / 9.1, 32 x 128257 39.9 / 24.3 /
+  // 17.4 / 17.3, 64 x 50257 21.4 / 16.1 / 16.6 / 24.5, 150 x 30000 21.2 / 22.7 / 28.4 / 47.0, 1 x 4000 7.9 / 7.6 / 7.3 / 7.4; trees of
+  // 26, whose slowest sequence takes several passes: 32 x 128257 114 / 65 / 41 / 33, 64 x 50257 58 / 37 / 32 / 41, 150 x 30000 41 / 39 / 40 / 61.
   int c = 1;
   while (c < VERIFY_MAX_CLUSTER && int64_t(B) * 2 * c <= 2 * st->sm_count && V >= 2048 * c) c *= 2;
   p.cluster = c;

@@ -141,8 +141,8 @@ struct TreeList {
   }
 };
 
-// A CTA's part [next, end) of the list as a cursor that every warp moves by itself. Cursor and piece stand in shared memory:
-// as registers they would make the softmax warps, which hold a row's 128 scores, spill.
+// A CTA's part [next, end) of the list as a cursor that every warp moves by itself. Cursor and piece stand in shared memory: the
+// tcgen05 kernel's softmax warps, which hold a row's 128 scores, have no registers left for them.
 template <int KEYS>
 struct TreeWalk {
   uint32_t next, end;

@@ -26,6 +26,7 @@
 //   o_done[s]          the last PV_s of a unit has completed
 //   o_free[s]          set s has read O (of both streams, but for PAIR) of a unit
 //   ml_ready[s][u & 1] not PAIR: set s has published its rows' maxima and sums of unit u
+//   drain[w]           a CTA that gives up: the products that issuing warp w had under way have completed
 // Each completes again only after its waiters have seen the completion before. A wait for "the phase before the first"
 // (parity 1 of a fresh barrier) returns at once.
 #pragma once
@@ -80,7 +81,8 @@ __device__ __forceinline__ const uint32_t* tree_bits(const TreeParams& p, int b,
 // whether they need it; 16 rows at a time, by warp-level MMAs with operands straight from global memory: finite values as such,
 // others added key by key, each only to the rows that see it. Results go over what was written. 8 sequences of 2 x 4,096 keys
 // of which one holds a NaN: 0.18 ms for 0.063 (one row at a time in 32 bits: 32 ms). Having the call costs the other inputs
-// 1 to 3 %, in registers; hence its few arguments.
+// 1 to 3 %, in registers; hence its few arguments. Spilled bytes, stored / loaded: the kernel
+// with the call 40 / 52 (PAIR), 12 / 20, with a mask 64 / 92, without it 8 / 16 in the second form alone; the redo itself 100 / 164 and 8 / 4.
 template <bool PAIR>
 __device__ __noinline__ void tree_exact_rows(const TreeUmmaParams& params, const TreePiece& pc, float m, float l, bool redo) {
   constexpr int COLS = PAIR ? 128 : 64, ROWS = UMMA_ROWS<PAIR>, NT = COLS / 8;
@@ -397,6 +399,9 @@ __global__ void __launch_bounds__(UMMA_THREADS, 1) tree_umma_kernel(const __grid
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
           if (PAIR) {
+            // Rounded to bf16, half a step (2^-9) each, their sum being taken before: tensor memory is full (scores 128 columns, P 2 x 64,
+            // O 2 x 128), so that low halves would need P of half a tile at a time. 64 tokens over 65,536 keys: error against 64 bits
+            // 0.0023 of the output's norm, where rounding the output alone makes 0.0017 and 16 bits of P no more than that.
             sm::exp_chunk<sm::EX2_FMA_PAIRS_NONE>(s, c * 32, t.scale_log2, base, pk, sum);
             ptx::tmem_st16(p_addr + c * 16, pk);
           } else {

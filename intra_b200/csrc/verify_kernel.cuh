@@ -6,7 +6,8 @@
 //
 //   R <- max(R - Z q, 0),  Z <- sum R            (both stay where nothing would be left),
 //
-// so that tokens come out distributed as p whatever q is (R / Z is the target's distribution given the rejections). When no child is
+// so that tokens come out distributed as p whatever q is, if the children of a node were drawn from q independently of one another (R / Z
+// is the target's distribution given the rejections; children drawn without replacement follow other distributions). When no child is
 // accepted the walk ends, and one more token is drawn from R: the smallest t with R(0) + .. + R(t) > u_0 sum R. Drafts
 // without a distribution count as certain: q is one at their token. All of it in 64 bits: an error of 2^-24 in a running
 // sum over 10^5 tokens decides the token in one draw of a hundred, 2^-53 in none.
@@ -18,9 +19,9 @@
 //
 // What bounds a pass is how much of the rows is under way: every thread copies 16-byte granules VERIFY_AHEAD ahead into slots of
 // its own in shared memory (its own copies are all it waits for), and then the arithmetic: 64-bit numbers are made from the bits
-// of 32-bit ones by integer multiply-adds, and compared with zero by their upper words. 32 trees of 26 nodes over 128257 tokens,
+// of 32-bit ones by integer multiplications, and compared with zero by their upper words. 32 trees of 26 nodes over 128257 tokens,
 // the slowest of which take 4 or 5 passes one after the other: 171 us with a division per rejection and token, 46 without, 42 with
-// the granules, 35 so; reading two rows of each once at the copy bandwidth takes 5.
+// the granules, 33 so; reading two rows of each once at the copy bandwidth takes 5.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -61,13 +62,14 @@ template <> __device__ __forceinline__ double as_double(__half x) { return __hal
 
 // A probability times 2^-896 as a double, from the bits of fp32 by one integer multiplication (the conversion instruction runs at an
 // eighth of the rate): the exponent fields differ by that in their bias, and zero and denormals come out right by themselves.
-// Negative numbers, minus zero among them, become zero. Differences are kept to 2^-178 of an unscaled number, so a sum over tokens
+// Negative numbers, minus zero among them, become zero; an infinity or NaN counts as 2^128 or more. Differences are kept to 2^-178 of an unscaled number, so a sum over tokens
 // of which none has anything left is zero, and one is positive where some token has.
 constexpr double VERIFY_SCALE = 0x1p-896, VERIFY_UNSCALE = 0x1p896;
 __device__ __forceinline__ double scaled(float x) { return __longlong_as_double((long long)(max(__float_as_int(x), 0)) * (1 << 29)); }
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
+
 // The sum over a warp's lanes, the same in all of them.
 __device__ __forceinline__ double warp_total(double x) {
 #pragma unroll

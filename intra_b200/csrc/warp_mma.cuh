@@ -1,4 +1,4 @@
-// Warp-level pieces of the attention kernels that read a cache (decode_kernel.cuh, tree_kernel.cuh): m16n8k16 MMAs, their
+// Warp-level pieces of the attention kernels that read a cache (decode_kernel.cuh, tree_mma_kernel.cuh, tree_umma_kernel.cuh): m16n8k16 MMAs, their
 // operands from shared memory, probabilities kept to 16 bits, merging of partial results.
 #pragma once
 #include <math_constants.h>

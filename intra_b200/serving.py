@@ -12,7 +12,8 @@ accumulates the attention each key receives, and eviction by it.
 
 Node 0 of a tree is the token sampled last; `parents` names for each node the one it follows. None of these has a counterpart in
 the reference, whose decode step is one dense token at a time (experiments/llm/intra_token_attn.py:112-134).
-Forward only; nothing synchronises, nothing is remembered between calls, every call runs on the current stream.
+Forward only: gradients, tangents and programs that are being recorded (torch.jit.trace, torch.fx) are refused. Nothing synchronises,
+nothing is remembered between calls, every call runs on the current stream; tensors written in place count as modified for autograd.
 """
 from __future__ import annotations
 
@@ -235,6 +236,10 @@ def verify_drafts(tokens, target_probs, draft_probs, uniform, parents=None):
     the target's distribution and Z = 1 at first; a rejection replaces R by max(R - Z q, 0) and Z by its sum (unless that is
     zero). When none is left the last token is drawn from R: the smallest t with R(0) + .. + R(t) > uniform * sum R. Sums
     and comparisons are in 64 bits.
+
+    Tokens come out distributed as the target's if a node's children were drawn independently of one another; children drawn without
+    replacement need other draft probabilities than one row for all of them. Probabilities are finite and not negative: a row that holds
+    others gives some token of the vocabulary.
 
     Returns accepted (B,) int32, the number m of accepted drafts; path (B, n) int32, the nodes from 0 on, then -1; and tokens
     (B, n) int64: the m accepted ones, the drawn one, then -1. Drafts outside the vocabulary are rejected."""
