@@ -20,7 +20,8 @@ call, like the decode step's.
 
 Both registrations are needed: transformers builds a mask only for names that are registered with `AttentionMaskInterface`, and
 without one nothing tells the rows of a static cache that are not filled, or a batch's padding, from keys. A few tokens behind a
-cache are refused where a model's attention has no such entry. (The patterns do not look at masks: padding in a prompt takes part, as
+cache are refused where a model's attention has no such entry. A prompt into a static cache counts as tokens behind a cache: up to 64 are
+dense, more are refused. (The patterns do not look at masks: padding in a prompt takes part, as
 in the reference.)
 """
 from __future__ import annotations

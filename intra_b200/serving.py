@@ -386,7 +386,8 @@ def evict_cache(k, v, weights, keep, recent=0, lengths=None, out=None):
     Returns (k, v, weights, kept): the kept rows, their weights and their old places (B, Hkv, keep) int32. Behind a sequence's
     last row come zeros, and -1 in `kept`; lengths are min(lengths, keep) from then on. `out` = (k, v, weights) writes into the
     caller's tensors of at least `keep` rows, whose rows from `keep` on stay as they are; they must not overlap the inputs."""
-    _forward_only(k, v, weights, lengths, *(() if out is None else out))
+    out = None if out is None else tuple(out)
+    _forward_only(k, v, weights, lengths, *(out or ()))
     kn, dev, bf16 = k.shape, k.device, torch.bfloat16
     if not k.is_cuda or k.dtype is not bf16 or v.dtype is not bf16 or len(kn) != 4 or kn[3] != 128:
         raise ValueError("INTRA kernels need CUDA bfloat16 tensors (batch, heads, tokens, 128)")
